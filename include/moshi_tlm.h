@@ -104,6 +104,66 @@ int mmi_tlm_set_taps(mmi_tlm* m, float* taps);
 /* "site\tkernel\tbytes" per launch of the last step. */
 int64_t mmi_tlm_launch_list(const mmi_tlm* m, char* buf, int64_t cap);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Key/value cache in 8 bits, by itself                                                       */
+/* ------------------------------------------------------------------------------------------ */
+/* Pages of 64 tokens: key codes [pages][kv_heads][64][dim], value codes [pages][kv_heads][vdim][64] (aligned to 16 bytes), scales
+ * [pages][kv_heads][4], one per 16 tokens and head.  A value is code * scale.  The arrays are the caller's; the device is the one they
+ * are on, and it has to be the current one. */
+typedef struct mmi_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t pages;
+    int32_t kv_heads, dim, vdim;                  /* head sizes: multiples of 16 up to 256 */
+    int32_t codes;                                /* MMI_I8 or MMI_F8E4M3 */
+    int32_t rot_dim;                              /* leading dimensions of keys and queries that are rotated, a multiple of 8; 0: none */
+    int32_t rot_halves;                           /* partners half of them apart; 0: side by side */
+    const double* rot_freq;                       /* device [rot_dim / 2]: turns per position */
+} mmi_kv_cache;
+/* The sequences of a call, all of it in device memory: sequence e brings rows row0[e] .. row0[e + 1] - 1 of the tensors, its positions
+ * position[e] .., and finds position p in page table[e][p / 64].  row0 NULL: one row each, in order.  A page number outside the cache
+ * holds nothing: rows that belong there are not written, and nobody sees its tokens.  A sequence with a negative position is passed over. */
+typedef struct mmi_kv_seqs {
+    int32_t n, rows;                              /* sequences, rows of the tensors */
+    const int32_t* row0;
+    const int32_t* position;
+    const int32_t* table;
+    int32_t table_ld;
+} mmi_kv_seqs;
+/* Rotate the keys, round keys and values to 8 bits and write them to their pages.  dtype: MMI_BF16 or MMI_F32, strides in elements, a
+ * head's dimensions side by side.  A block's scale is the largest magnitude it was handed / the largest code (127, 448); where a token makes
+ * it grow, the codes that the block holds of earlier positions are rounded again.  A NaN or infinity makes the block's scale NaN.  The pages
+ * that two sequences of a call write to are different ones. */
+int mmi_kv_append(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                  int64_t v_head, mmi_stream stream);
+/* What the cache holds for those rows: k [rows][kv_heads][dim], v [rows][kv_heads][vdim]; zeros where there is no page. */
+int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, void* k, void* v, mmi_stream stream);
+/* out = softmax(scale q k^T) v over the positions up to a row's own; window > 0: the last `window` of them and the first `keep_first`;
+ * sink: one is added to the softmax's denominator.  Query head h reads key/value head h / (heads / kv_heads).  bf16: fp32 sums of bf16
+ * products; fp32: fp32 arithmetic.  A row that sees nothing gets zeros.  workspace: device memory of mmi_kv_attend_workspace bytes (a negative
+ * status in its place where the arguments are refused), one per call in flight. */
+int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first);
+int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
+                  int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t sink, void* workspace, int64_t workspace_bytes,
+                  mmi_stream stream);
+
+/* ------------------------------------------------------------------------------------------ */
+/* Beam search                                                                                */
+/* ------------------------------------------------------------------------------------------ */
+/* Of every request's beams x vocab candidates the `beams` best.  Candidate (beam, token): score + log softmax(logits)[token], ranked by
+ * score / length^length_penalty, length counting the token; equal ranks go to the lower beam, then the lower token.  A finished beam has one
+ * candidate, `eos` at the score and the length it has.  Rows with a NaN, and beams of score -infinity, rank last.  Device memory all of it:
+ * logits bf16 or fp32 [batch * beams][vocab], `row` elements apart; score, out_* [batch][beams]; length (NULL: no penalty), finished (NULL:
+ * none is) and the outputs of either kind may be NULL.  At most 32 beams. */
+int64_t mmi_beam_select_workspace(int32_t batch, int32_t beams, int32_t vocab);
+int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int32_t dtype, const void* logits, int64_t row, const float* score, const int32_t* length,
+                    const uint8_t* finished, int32_t eos, float length_penalty, float* out_score, int32_t* out_parent, int32_t* out_token, uint8_t* out_finished,
+                    int32_t* out_length, void* workspace, int64_t workspace_bytes, mmi_stream stream);
+/* Row b * beams + i of every tensor (host arrays: device pointers, bytes from row to row, bytes of a row) becomes a copy of what row
+ * b * beams + parents[b][i] was; in place.  parents: device int32 [batch][beams]; one outside the request leaves its row alone. */
+int mmi_beam_reorder(int32_t n, void* const* tensors, const int64_t* strides, const int64_t* row_bytes, int32_t batch, int32_t beams, const int32_t* parents,
+                     mmi_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

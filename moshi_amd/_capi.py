@@ -95,6 +95,15 @@ class TLMCfg(C.Structure):
                 ("bigram_mul_cur", C.c_int64), ("max_positions", C.c_int32), ("dtype", C.c_int32)]
 
 
+class KVCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("pages", C.c_int64), ("kv_heads", C.c_int32),
+                ("dim", C.c_int32), ("vdim", C.c_int32), ("codes", C.c_int32), ("rot_dim", C.c_int32), ("rot_halves", C.c_int32), ("rot_freq", C.c_void_p)]
+
+
+class KVSeqs(C.Structure):
+    _fields_ = [("n", C.c_int32), ("rows", C.c_int32), ("row0", C.c_void_p), ("position", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int32)]
+
+
 # include/moshi_tlm.h
 TLM_MIX_LATENT_ATTENTION, TLM_MIX_MINGRU, TLM_MIX_ATTENTION, TLM_MIX_CHANNEL_DELTA, TLM_MIX_LIGHTNING = 1, 2, 3, 4, 5
 TLM_MLP_NONE, TLM_MLP_MOE, TLM_MLP_DENSE = 0, 1, 2
@@ -195,6 +204,14 @@ TLM_SIGNATURES = {
     "mmi_tlm_pages_needed": (C.c_int64, [_P, C.c_int32, C.c_int64]),
     "mmi_tlm_set_taps": (C.c_int, [_P, _P]),
     "mmi_tlm_launch_list": (C.c_int64, [_P, _P, C.c_int64]),
+    "mmi_kv_append": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P]),
+    "mmi_kv_read": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, _P, _P, _P]),
+    "mmi_kv_attend_workspace": (C.c_int64, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, C.c_int32]),
+    "mmi_kv_attend": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_float, C.c_int32,
+                                C.c_int32, C.c_int32, _P, C.c_int64, _P]),
+    "mmi_beam_select_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "mmi_beam_select": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, C.c_int32, C.c_float, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "mmi_beam_reorder": (C.c_int, [C.c_int32, _P, _P, _P, C.c_int32, C.c_int32, _P, _P]),
 }
 
 

@@ -23,7 +23,7 @@ ROOT = PKG.parent
 LIB = PKG / "libmoshi_mi.so"
 LIBS = {
     "mi": (LIB, ["api_common.hip", "mimi_engine.hip", "lm_engine.hip", "batcher.hip", "duplex.hip"]),
-    "tlm": (PKG / "libmoshi_tlm.so", ["api_common.hip", "tlm_engine.hip"]),
+    "tlm": (PKG / "libmoshi_tlm.so", ["api_common.hip", "tlm_engine.hip", "tlm_ops.hip"]),
 }
 ARCH = "gfx950"
 # no v_pk_{add,mul,fma}_f32: some operand forms of the packed fp32 instructions have returned stale elements on gfx950

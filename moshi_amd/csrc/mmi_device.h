@@ -395,6 +395,8 @@ __device__ __forceinline__ float mmi_fast_exp2f(float x) { return __builtin_amdg
 __device__ __forceinline__ float mmi_fast_log2f(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float mmi_fast_rcpf(float x) { return __builtin_amdgcn_rcpf(x); }      // ~1 ulp
 __device__ __forceinline__ float mmi_fast_logf(float x) { return __logf(x); }
+// sine and cosine of x turns, |x| <= 1/2
+__device__ __forceinline__ void mmi_sincos_turns(float x, float& s, float& c) { sincospif(2.f * x, &s, &c); }
 __device__ __forceinline__ unsigned mmi_atomic_add(unsigned* p, unsigned v) { return atomicAdd(p, v); }
 
 // Cross-stream hand-off flags (duplex.hip): a monotonic counter in device memory, published with release semantics by a

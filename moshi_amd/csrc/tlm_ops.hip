@@ -1,0 +1,306 @@
+// Operators of the token language models behind the C ABI of include/moshi_tlm.h: the 8-bit key/value cache and its attention, beam search's
+// choice and the reordering of its states.
+#include "../../include/moshi_tlm.h"
+#include "tlm_ops.h"
+#include "tlm_beam.h"
+
+namespace {
+
+constexpr long KV8_WORKGROUPS = 1024;    // that a split of the pages aims at: 4 per CU, of which 2 run at a time
+constexpr int KV8_MAX_SPLIT = 256;       // (k_tlm_kv8_combine: a lane each)
+
+int check_cache(const mmi_kv_cache* c, TlmKv8Cache* out, const char* at) {
+    auto bad = [&](int code, const char* what) { return mmi_fail(code, std::string(at) + ": " + what); };
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return bad(MMI_ERR_INVALID, "null cache");
+    if (c->pages < 1 || c->pages > 0x7fffffff) return bad(MMI_ERR_SHAPE, "the cache needs between 1 and 2^31 - 1 pages");
+    if (c->kv_heads < 1 || c->kv_heads > 65535) return bad(MMI_ERR_SHAPE, "key/value heads");
+    if (c->dim < 16 || c->dim > 256 || c->dim % 16 || c->vdim < 16 || c->vdim > 256 || c->vdim % 16)
+        return bad(MMI_ERR_UNSUPPORTED, "head sizes are multiples of 16 up to 256");
+    if (c->codes != MMI_I8 && c->codes != MMI_F8E4M3) return bad(MMI_ERR_UNSUPPORTED, "codes are int8 or e4m3");
+    if (c->rot_dim < 0 || c->rot_dim > c->dim || c->rot_dim % 8 || (c->rot_dim && !c->rot_freq)) return bad(MMI_ERR_INVALID, "rotated dimensions are a multiple of 8 up to the head size, with frequencies");
+    if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return bad(MMI_ERR_INVALID, "codes must be aligned to 16 bytes");
+    *out = TlmKv8Cache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, (int)c->pages, c->kv_heads, c->dim, c->vdim, c->codes == MMI_F8E4M3, c->rot_dim, c->rot_halves, c->rot_freq};
+    return MMI_OK;
+}
+int check_seqs(const mmi_kv_seqs* q, TlmKv8Seqs* out, const char* at) {
+    auto bad = [&](int code, const char* what) { return mmi_fail(code, std::string(at) + ": " + what); };
+    if (!q || q->n < 0 || q->rows < 0) return bad(MMI_ERR_INVALID, "bad sequences");
+    if (q->n && (!q->position || !q->table || q->table_ld < 1)) return bad(MMI_ERR_INVALID, "sequences need positions and a page table");
+    if (!q->row0 && q->rows != q->n) return bad(MMI_ERR_SHAPE, "without row starts every sequence brings one row");
+    if (q->n > 1 << 20 || q->rows > 1 << 24) return bad(MMI_ERR_SHAPE, "at most 2^20 sequences and 2^24 rows");
+    *out = TlmKv8Seqs{q->n, q->rows, q->row0, nullptr, q->position, nullptr, TlmPages{q->table, q->table_ld, q->table_ld}, 0};
+    return MMI_OK;
+}
+int check_rows(const void* p, int64_t row, int64_t head, int dtype, const char* at) {
+    if (!p) return mmi_fail(MMI_ERR_INVALID, std::string(at) + ": null tensor");
+    if (row < 0 || head < 0) return mmi_fail(MMI_ERR_INVALID, std::string(at) + ": negative stride");
+    if (dtype != MMI_BF16 && dtype != MMI_F32) return mmi_fail(MMI_ERR_UNSUPPORTED, std::string(at) + ": bf16 or fp32");
+    return MMI_OK;
+}
+// can four elements be loaded at once?
+bool aligned4(const void* p, int64_t row, int64_t head, int dtype) { return (uintptr_t)p % (dtype == MMI_F32 ? 16 : 8) == 0 && row % 4 == 0 && head % 4 == 0; }
+
+template <class F>
+int by_codes(int e4m3, F f) { return e4m3 ? f(std::true_type()) : f(std::false_type()); }
+
+int launch_read(hipStream_t s, const TlmKv8Read& a, int dtype) {
+    const long slots = kv8_slots(a.q, a.z);
+    return by_codes(a.c.e4m3, [&](auto e) {
+        if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_kv8_read<float, decltype(e)::value>), dim3((unsigned)slots, a.c.kv_heads, 2), 64, 0, s, a);
+        else MMI_LAUNCH((k_tlm_kv8_read<uint16_t, decltype(e)::value>), dim3((unsigned)slots, a.c.kv_heads, 2), 64, 0, s, a);
+        MMI_CHECK_LAUNCH();
+        return (int)MMI_OK;
+    });
+}
+
+template <class In, class Tr, int NS, int D>
+int launch_attn(hipStream_t s, const TlmKv8Attn& a) {
+    const unsigned slots = (unsigned)kv8_slots(a.q, a.z);
+    if (a.c.e4m3) MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, true>), dim3(slots, a.c.kv_heads, a.nsplit), 256, 0, s, a);
+    else MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, false>), dim3(slots, a.c.kv_heads, a.nsplit), 256, 0, s, a);
+    if (a.nsplit > 1) MMI_LAUNCH((k_tlm_kv8_combine<Tr>), dim3(slots, a.c.kv_heads, std::min(16, a.q.row0 ? 16 : a.rep)), 256, 0, s, a);
+    MMI_CHECK_LAUNCH();
+    return MMI_OK;
+}
+template <class In, class Tr, int NS>
+int launch_attn_d(hipStream_t s, const TlmKv8Attn& a) {
+    const int d = std::max(a.c.dim, a.c.vdim);
+    if (d <= 64) return launch_attn<In, Tr, NS, 64>(s, a);
+    if (d <= 128) return launch_attn<In, Tr, NS, 128>(s, a);
+    return launch_attn<In, Tr, NS, 256>(s, a);
+}
+
+}  // namespace
+
+int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype) {
+    a.z = kv8_cut(a.q, 1, KV8_BLOCK, 2);               // (a portion of n rows touches at most (n + 14) / 16 + 1 blocks)
+    const dim3 grid((unsigned)kv8_slots(a.q, a.z), a.c.kv_heads, 2);
+    return by_codes(a.c.e4m3, [&](auto e) {
+        if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_kv8_append<float, decltype(e)::value>), grid, 64, 0, s, a);
+        else MMI_LAUNCH((k_tlm_kv8_append<uint16_t, decltype(e)::value>), grid, 64, 0, s, a);
+        MMI_CHECK_LAUNCH();
+        return (int)MMI_OK;
+    });
+}
+
+size_t tlm_kv8_plan(TlmKv8Attn& a, long cap) {
+    a.z = kv8_cut(a.q, a.rep, 16, 1);
+    const long units = std::max(1l, kv8_slots(a.q, a.z) * a.c.kv_heads);
+    if (a.mask.window > 0) cap = std::min<long>(cap, (long)a.mask.window / TLM_PAGE + 3 + mmi_cdiv(a.mask.keep, TLM_PAGE));
+    cap = std::max(cap, 1l);
+    long per = std::max((cap * units + KV8_WORKGROUPS - 1) / KV8_WORKGROUPS, (cap + KV8_MAX_SPLIT - 1) / KV8_MAX_SPLIT);
+    per = std::min((per + 3) / 4 * 4, (cap + 3) / 4 * 4);      // (each of the four waves takes every fourth page)
+    a.per = (int)per;
+    a.nsplit = (int)((cap + per - 1) / per);
+    return a.nsplit > 1 ? (size_t)units * a.nsplit * (16 * a.c.vdim + 32) : 0;
+}
+
+int tlm_kv8_attend(hipStream_t s, const TlmKv8Attn& a, int dtype, bool f32) {
+    if (dtype == MMI_BF16) return launch_attn_d<uint16_t, TlmBf16, 1>(s, a);
+    return f32 ? launch_attn_d<float, TlmF32, 3>(s, a) : launch_attn_d<float, TlmBf16, 1>(s, a);
+}
+
+extern "C" int mmi_kv_append(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                             int64_t v_head, mmi_stream stream) {
+    TlmKv8Append a;
+    memset(&a, 0, sizeof(a));
+    int rc;
+    if ((rc = check_cache(cache, &a.c, "mmi_kv_append")) || (rc = check_seqs(seqs, &a.q, "mmi_kv_append"))) return rc;
+    if (!a.q.n || !a.q.T) return MMI_OK;
+    if ((rc = check_rows(k, k_row, k_head, dtype, "mmi_kv_append")) || (rc = check_rows(v, v_row, v_head, dtype, "mmi_kv_append"))) return rc;
+    a.k = k;
+    a.v = v;
+    a.k_row = k_row;
+    a.k_head = k_head;
+    a.v_row = v_row;
+    a.v_head = v_head;
+    a.wide = aligned4(k, k_row, k_head, dtype);
+    return tlm_kv8_append((hipStream_t)stream, a, dtype);
+}
+
+extern "C" int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, void* k, void* v, mmi_stream stream) {
+    TlmKv8Read a;
+    memset(&a, 0, sizeof(a));
+    int rc;
+    if ((rc = check_cache(cache, &a.c, "mmi_kv_read")) || (rc = check_seqs(seqs, &a.q, "mmi_kv_read"))) return rc;
+    if (!a.q.n || !a.q.T) return MMI_OK;
+    if ((rc = check_rows(k, 0, 0, dtype, "mmi_kv_read")) || (rc = check_rows(v, 0, 0, dtype, "mmi_kv_read"))) return rc;
+    if (((uintptr_t)k | (uintptr_t)v) % 16) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_read: outputs must be aligned to 16 bytes");
+    a.k = k;
+    a.v = v;
+    a.z = kv8_cut(a.q, 1, KV8_BLOCK, 2);
+    return launch_read((hipStream_t)stream, a, dtype);
+}
+
+namespace {
+int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first, TlmKv8Attn* a, size_t* floats) {
+    memset(a, 0, sizeof(*a));
+    int rc;
+    if ((rc = check_cache(cache, &a->c, "mmi_kv_attend")) || (rc = check_seqs(seqs, &a->q, "mmi_kv_attend"))) return rc;
+    if (heads < 1 || heads % cache->kv_heads || heads / cache->kv_heads > 1024) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: query heads are a multiple of the key/value heads, at most 1024 times");
+    if (window < 0 || keep_first < 0) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: negative window");
+    a->heads = heads;
+    a->rep = heads / cache->kv_heads;
+    a->nd = cache->vdim / 16;
+    a->mask = TlmMask{window, window > 0 ? keep_first : 0, 0.f};
+    if ((long)a->q.T * a->rep > 1l << 26) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^26 rows times query heads of a group");
+    *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1);
+    return MMI_OK;
+}
+}  // namespace
+
+extern "C" int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first) {
+    TlmKv8Attn a;
+    size_t floats;
+    const int rc = attn_args(cache, seqs, heads, window, keep_first, &a, &floats);
+    return rc ? rc : (int64_t)(floats * sizeof(float));
+}
+
+extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
+                             int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t sink, void* workspace, int64_t workspace_bytes,
+                             mmi_stream stream) {
+    TlmKv8Attn a;
+    size_t floats;
+    int rc = attn_args(cache, seqs, heads, window, keep_first, &a, &floats);
+    if (rc) return rc;
+    if (!a.q.n || !a.q.T) return MMI_OK;
+    if ((rc = check_rows(q, q_row, q_head, dtype, "mmi_kv_attend")) || (rc = check_rows(out, out_row, out_head, dtype, "mmi_kv_attend"))) return rc;
+    if (!aligned4(out, out_row, out_head, dtype)) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: four elements of the output must be aligned");
+    if (!(scale == scale) || scale - scale != 0.f) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: the scale is not finite");
+    if (floats && (!workspace || workspace_bytes < (int64_t)(floats * sizeof(float)) || (uintptr_t)workspace % 16))
+        return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: the workspace is too small (mmi_kv_attend_workspace) or not aligned to 16 bytes");
+    a.x = q;
+    a.x_row = q_row;
+    a.x_head = q_head;
+    a.wide = aligned4(q, q_row, q_head, dtype);
+    a.out = out;
+    a.out_row = out_row;
+    a.out_head = out_head;
+    a.mask.scale = scale * 1.44269504088896340736f;
+    a.sink = sink;
+    a.po = (float*)workspace;
+    a.pml = a.po + floats / (16 * a.c.vdim + 32) * (16 * a.c.vdim);
+    return tlm_kv8_attend((hipStream_t)stream, a, dtype, dtype == MMI_F32);
+}
+
+// ---- beam search ---------------------------------------------------------------------------------------------------------
+namespace {
+struct BeamSpace { size_t m, s, x, i, total; };            // where the parts of the workspace begin, in bytes
+BeamSpace beam_space(int rows, int beams, int vocab) {
+    const size_t lists = (size_t)rows * ((vocab - 1) / BEAM_CHUNK + 1);
+    BeamSpace z;
+    z.s = 0;
+    z.m = lists * sizeof(double);
+    z.x = z.m + lists * sizeof(float);
+    z.i = z.x + lists * beams * sizeof(float);
+    z.total = z.i + lists * beams * sizeof(int);
+    return z;
+}
+int check_beams(int64_t batch, int32_t beams, int32_t vocab, const char* at) {
+    if (batch < 0 || beams < 1 || vocab < 1) return mmi_fail(MMI_ERR_INVALID, std::string(at) + ": bad sizes");
+    if (beams > BEAM_MAX) return mmi_fail(MMI_ERR_UNSUPPORTED, std::string(at) + ": at most 32 beams");
+    if (batch * beams > 65535 || vocab > 1 << 20) return mmi_fail(MMI_ERR_SHAPE, std::string(at) + ": at most 65535 beams of all requests and 2^20 tokens");
+    return MMI_OK;
+}
+template <class U>
+int launch_reorder(hipStream_t s, const TlmReorder& a, unsigned blocks, int groups) {
+    const dim3 grid(blocks, (unsigned)groups);
+    if (a.beams <= 4) MMI_LAUNCH((k_tlm_reorder<U, 4>), grid, 256, 0, s, a);
+    else if (a.beams <= 8) MMI_LAUNCH((k_tlm_reorder<U, 8>), grid, 256, 0, s, a);
+    else if (a.beams <= 16) MMI_LAUNCH((k_tlm_reorder<U, 16>), grid, 256, 0, s, a);
+    else MMI_LAUNCH((k_tlm_reorder<U, 32>), grid, 256, 0, s, a);
+    MMI_CHECK_LAUNCH();
+    return MMI_OK;
+}
+}  // namespace
+
+extern "C" int64_t mmi_beam_select_workspace(int32_t batch, int32_t beams, int32_t vocab) {
+    const int rc = check_beams(batch, beams, vocab, "mmi_beam_select");
+    return rc ? rc : (int64_t)beam_space(batch * beams, beams, vocab).total;
+}
+
+extern "C" int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int32_t dtype, const void* logits, int64_t row, const float* score, const int32_t* length,
+                               const uint8_t* finished, int32_t eos, float length_penalty, float* out_score, int32_t* out_parent, int32_t* out_token, uint8_t* out_finished,
+                               int32_t* out_length, void* workspace, int64_t workspace_bytes, mmi_stream stream) {
+    int rc = check_beams(batch, beams, vocab, "mmi_beam_select");
+    if (rc || !batch) return rc;
+    if ((rc = check_rows(logits, row, 0, dtype, "mmi_beam_select"))) return rc;
+    if (!score || !out_score || !out_parent || !out_token) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: null tensor");
+    if (finished && (eos < 0 || eos >= vocab)) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: finished beams need an end token of the vocabulary");
+    if (!(length_penalty - length_penalty == 0.f) || (length_penalty != 0.f && !length)) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: a length penalty is finite and needs lengths");
+    const BeamSpace z = beam_space(batch * beams, beams, vocab);
+    if (!workspace || workspace_bytes < (int64_t)z.total || (uintptr_t)workspace % 16) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: the workspace is too small (mmi_beam_select_workspace) or not aligned to 16 bytes");
+    char* w = (char*)workspace;
+    TlmBeamArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = logits;
+    a.ld = row;
+    a.V = vocab;
+    a.beams = beams;
+    a.splits = mmi_cdiv(vocab, BEAM_CHUNK);
+    a.score = score;
+    a.length = length;
+    a.done = finished;
+    a.eos = eos;
+    a.alpha = (double)length_penalty;
+    a.wm = (float*)(w + z.m);
+    a.ws = (double*)(w + z.s);
+    a.wx = (float*)(w + z.x);
+    a.wi = (int*)(w + z.i);
+    a.out_score = out_score;
+    a.out_parent = out_parent;
+    a.out_token = out_token;
+    a.out_done = out_finished;
+    a.out_length = out_length;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_beam_rows<float>), dim3(a.splits, batch * beams), 256, 0, s, a);
+    else MMI_LAUNCH((k_tlm_beam_rows<uint16_t>), dim3(a.splits, batch * beams), 256, 0, s, a);
+    MMI_CHECK_LAUNCH();
+    MMI_LAUNCH(k_tlm_beam_pick, batch, 64, (size_t)beams * a.splits * sizeof(int), s, a);
+    MMI_CHECK_LAUNCH();
+    return MMI_OK;
+}
+
+int tlm_reorder(hipStream_t s, int n, const TlmReorderTensor* tensors, int groups, int beams, const int* parent, const int* row) {
+    // units of 16 bytes, of 4, of one: what every base, stride and row length is a multiple of
+    for (const int unit : {16, 4, 1})
+        for (int i = 0; i < n;) {
+            TlmReorder a;
+            memset(&a, 0, sizeof(a));
+            a.beams = beams;
+            a.parent = parent;
+            a.row = row;
+            unsigned blocks = 0;
+            for (; i < n && a.n < BEAM_TENSORS; ++i) {
+                const TlmReorderTensor& t = tensors[i];
+                const uintptr_t all = (uintptr_t)t.p | (uintptr_t)t.stride | (uintptr_t)t.bytes;
+                if (t.bytes == 0 || (all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1)) != unit) continue;
+                const long units = t.bytes / unit;
+                if (units > 0x7fffffffl) return mmi_fail(MMI_ERR_SHAPE, "reorder: a row is too long");
+                a.t[a.n++] = TlmReorder::T{(char*)t.p, (long)t.stride, (unsigned)units, blocks};
+                blocks += (unsigned)mmi_cdiv64(units, 256);
+            }
+            if (!a.n) continue;
+            const int rc = unit == 16 ? launch_reorder<u32x4>(s, a, blocks, groups) : (unit == 4 ? launch_reorder<uint32_t>(s, a, blocks, groups) : launch_reorder<uint8_t>(s, a, blocks, groups));
+            if (rc) return rc;
+        }
+    return MMI_OK;
+}
+
+extern "C" int mmi_beam_reorder(int32_t n, void* const* tensors, const int64_t* strides, const int64_t* row_bytes, int32_t batch, int32_t beams, const int32_t* parents,
+                                mmi_stream stream) {
+    int rc = check_beams(batch, beams, 1, "mmi_beam_reorder");
+    if (rc || !batch || !n) return rc;
+    if (n < 0 || !tensors || !strides || !row_bytes || !parents) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: null argument");
+    std::vector<TlmReorderTensor> t((size_t)n);
+    for (int i = 0; i < n; ++i) {
+        if (!tensors[i] || row_bytes[i] < 0 || strides[i] < row_bytes[i]) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: rows are apart and not null");
+        t[i] = TlmReorderTensor{tensors[i], strides[i], row_bytes[i]};
+    }
+    std::vector<std::pair<uintptr_t, uintptr_t>> span;     // (a tensor given twice would be read and written by two workgroups)
+    for (const TlmReorderTensor& x : t) span.push_back({(uintptr_t)x.p, (uintptr_t)x.p + (uintptr_t)x.stride * (uintptr_t)(batch * beams - 1) + (uintptr_t)x.bytes});
+    std::sort(span.begin(), span.end());
+    for (int i = 1; i < n; ++i)
+        if (span[i].first < span[i - 1].second) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: two tensors share memory");
+    return tlm_reorder((hipStream_t)stream, n, t.data(), batch, beams, parents, nullptr);
+}

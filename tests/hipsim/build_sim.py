@@ -15,7 +15,7 @@ CSRC = ROOT / "moshi_amd" / "csrc"
 LIB = HERE / "libmoshi_sim.so"
 TLM_LIB = HERE / "libmoshi_tlm_sim.so"
 SOURCES = ["api_common.hip", "mimi_engine.hip", "lm_engine.hip", "batcher.hip", "duplex.hip"]
-TLM_SOURCES = ["api_common.hip", "tlm_engine.hip"]
+TLM_SOURCES = ["api_common.hip", "tlm_engine.hip", "tlm_ops.hip"]
 
 
 def _cxx() -> str:

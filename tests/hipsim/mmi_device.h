@@ -434,6 +434,7 @@ inline float mmi_fast_exp2f(float x) { return mmi_flushed(exp2f(x)); }
 inline float mmi_fast_log2f(float x) { return log2f(x); }
 inline float mmi_fast_rcpf(float x) { return mmi_flushed(1.0f / mmi_flushed(x)); }
 inline float mmi_fast_logf(float x) { return logf(x); }
+inline void mmi_sincos_turns(float x, float& s, float& c) { const double a = 6.283185307179586 * (double)x; s = (float)sin(a); c = (float)cos(a); }
 inline unsigned mmi_wave_sum_u32(unsigned x) { for (int m = 1; m < 64; m <<= 1) x += mmi_shfl_xor(x, m); return x; }
 inline unsigned mmi_wave_max_u32(unsigned x) { for (int m = 1; m < 64; m <<= 1) { const unsigned o = mmi_shfl_xor(x, m); x = o > x ? o : x; } return x; }
 inline unsigned mmi_atomic_add(unsigned* p, unsigned v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
