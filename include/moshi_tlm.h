@@ -139,10 +139,10 @@ int mmi_kv_append(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dt
 /* What the cache holds for those rows: k [rows][kv_heads][dim], v [rows][kv_heads][vdim]; zeros where there is no page. */
 int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, void* k, void* v, mmi_stream stream);
 /* out = softmax(scale q k^T) v over the positions up to a row's own; window > 0: the last `window` of them and the first `keep_first`;
- * sink: one is added to the softmax's denominator.  Query head h reads key/value head h / (heads / kv_heads).  bf16: fp32 sums of bf16
- * products; fp32: fp32 arithmetic.  A row that sees nothing gets zeros.  workspace: device memory of mmi_kv_attend_workspace bytes (a negative
+ * sink: one is added to the softmax's denominator.  Query head h reads key/value head h / (heads / kv_heads).  Sums are
+ * fp32; bf16 queries and the weights beside them are fp16 operands, fp32 ones two fp16 parts each (22 bits).  A row that sees nothing gets zeros.  workspace: device memory of mmi_kv_attend_workspace bytes (a negative
  * status in its place where the arguments are refused), one per call in flight. */
-int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first);
+int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, int32_t window, int32_t keep_first);
 int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
                   int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t sink, void* workspace, int64_t workspace_bytes,
                   mmi_stream stream);

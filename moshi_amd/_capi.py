@@ -206,7 +206,7 @@ TLM_SIGNATURES = {
     "mmi_tlm_launch_list": (C.c_int64, [_P, _P, C.c_int64]),
     "mmi_kv_append": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P]),
     "mmi_kv_read": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, _P, _P, _P]),
-    "mmi_kv_attend_workspace": (C.c_int64, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, C.c_int32]),
+    "mmi_kv_attend_workspace": (C.c_int64, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "mmi_kv_attend": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_float, C.c_int32,
                                 C.c_int32, C.c_int32, _P, C.c_int64, _P]),
     "mmi_beam_select_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),

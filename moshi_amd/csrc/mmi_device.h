@@ -66,6 +66,17 @@ __device__ __forceinline__ float mmi_group_sum(float x) {
     if constexpr (W >= 16) x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x140, 0xf, 0xf, true));
     return x;
 }
+// maximum over groups of W consecutive lanes (8, 16, 32), every lane of the group gets it
+template <int W>
+__device__ __forceinline__ float mmi_group_max(float x) {
+    static_assert(W == 8 || W == 16 || W == 32, "half a DPP row, one, or two");
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xB1, 0xf, 0xf, true)));
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4E, 0xf, 0xf, true)));
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x141, 0xf, 0xf, true)));
+    if constexpr (W >= 16) x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x140, 0xf, 0xf, true)));
+    if constexpr (W >= 32) x = fmaxf(x, mmi_shfl_xor(x, 16));
+    return x;
+}
 // The same sum over rows of 16 lanes in the order of an exchange over distances 8, 4, 2, 1 (rotations by those distances inside the row: a lane
 // and its partner hold what the exchange would give them), bit for bit what the shuffles give without their trips through LDS
 __device__ __forceinline__ float mmi_row_sum(float x) {
@@ -295,6 +306,44 @@ __device__ __forceinline__ u32x2 mmi_fp8x4_to_bf16(uint32_t w) {
     return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
 }
+// ---- fp16 operands: 11 bits of significand where bf16 has 8 ----
+typedef _Float16 mmi_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 mmi_f16x8 __attribute__((ext_vector_type(8)));
+// two values -> one packed register (lo in bits 0..15), round-to-nearest-even; and back
+__device__ __forceinline__ uint32_t mmi_pack_f16x2(float lo, float hi) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, mmi_f16x2)); }
+__device__ __forceinline__ f32x2 mmi_unpack_f16x2(uint32_t w) { return __builtin_convertvector(__builtin_bit_cast(mmi_f16x2, w), f32x2); }
+// four fp8 bytes -> four fp16 (exact: subnormal codes are multiples of 2^-9)
+__device__ __forceinline__ u32x2 mmi_fp8x4_to_f16(uint32_t w) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))};
+}
+// four signed bytes -> four fp16 (exact): byte + 128 behind the exponent of 1024 is 1024 + 128 + value
+__device__ __forceinline__ u32x2 mmi_i8x4_to_f16(uint32_t w) {
+    const uint32_t u = w ^ 0x80808080u;
+    const mmi_f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(mmi_f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off),
+                 __builtin_bit_cast(uint32_t, __builtin_bit_cast(mmi_f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off)};
+}
+// the products of the bf16 forms above, same element maps
+__device__ __forceinline__ f32x4 mmi_mfma_f16_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mmi_f16x8, a), __builtin_bit_cast(mmi_f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mmi_mfma_f16_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(mmi_f16x8, a), __builtin_bit_cast(mmi_f16x8, b), c, 0, 0, 0);
+}
+// maximum / sum over lanes l and l ^ 32
+__device__ __forceinline__ float mmi_halves_max(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto v = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned v0 = v[0], v1 = v[1];
+    return fmaxf(__builtin_bit_cast(float, v0), __builtin_bit_cast(float, v1));
+}
+__device__ __forceinline__ float mmi_halves_sum(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto v = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned v0 = v[0], v1 = v[1];
+    return __builtin_bit_cast(float, v0) + __builtin_bit_cast(float, v1);
+}
 // D(32x32) += A(32x16) * B(16x32), fp8 in / fp32 acc.  Same element map as the bf16 32x32x16 form with one byte per
 // element: lane l: a[e] = A[l&31][8*(l>>5)+e], b[e] = B[8*(l>>5)+e][l&31] (8 bytes per operand per lane).
 __device__ __forceinline__ f32x16 mmi_mfma_fp8_32x32x16(u32x2 a, u32x2 b, f32x16 c) {
@@ -352,6 +401,8 @@ __device__ __forceinline__ void mmi_here(T& x) { asm volatile("" : "+v"(x)); }
 // a value that is the same in every lane (a wave index, what was loaded through one), told to the compiler: it stays in scalar registers,
 // and loads addressed by it are scalar loads - they do not queue behind the vector loads in flight
 __device__ __forceinline__ int mmi_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// lane `l`'s value (l: the same in every lane), to all of them through a scalar register
+__device__ __forceinline__ int mmi_from_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 // a load from memory that nothing writes while the kernel runs: by a uniform address a scalar load, also where the compiler cannot rule out that
 // one of the kernel's stores meets it
 __device__ __forceinline__ int mmi_load_const(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }

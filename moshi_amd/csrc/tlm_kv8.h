@@ -11,7 +11,6 @@
 // key - 16 dimensions, two k-steps of 8 - or 16 bytes of one value dimension - the 16 tokens of block kq.  For the weights of those 16 tokens
 // to be in that lane when the scores are done, row 4 a + i of score tile t is token 16 a + 4 t + i: lane kq then holds, over the four tiles,
 // the scores of block kq's tokens in order, and one key scale and one value scale are all it needs.
-// Codes become bf16 exactly (8 bits at most), so fp32 queries and weights go through the bf16 matrix core in three parts of 8 bits each.
 #pragma once
 #include "tlm_common.h"
 
@@ -52,25 +51,24 @@ __device__ __forceinline__ TlmKv8Seq kv8_seq(const TlmKv8Seqs& a, int e) {
 // page number of the sequence's tokens 64 i .. 64 i + 63; -1: there is none
 __device__ __forceinline__ int kv8_page(const TlmKv8Seqs& a, int n_pages, const int* row, int i) {
     if (!a.ring && i >= a.pages.ld) return -1;
-    const int p = a.ring ? tlm_page(a.pages, row, i) : mmi_load_const(row + i);
+    const int p = row[a.ring && i >= a.pages.keep ? a.pages.keep + (i - a.pages.keep) % (a.pages.ld - a.pages.keep) : i];
     return p < 0 || p >= n_pages ? -1 : p;
 }
 __device__ __forceinline__ const int* kv8_table(const TlmKv8Seqs& a, int e) { return a.pages.table + (long)mmi_uniform(a.slot ? a.slot[e] : e) * a.pages.ld; }
 
 // An entry's work is cut into pieces of `per` units, `mul` units a row, without anyone having counted them: entry e owns the slots from
 // row0[e] * mul / per + extra e on, which are as many as it can need, and a slot's entry is the last one that begins at or before it.
-// One row each: `extra` slots per entry.
-struct Kv8Cut { int mul, per, extra; };
-__device__ __forceinline__ int kv8_slot0(const TlmKv8Seqs& a, const Kv8Cut& z, int e) { return (a.row0 ? (int)((long)kv8_row0(a, e) * z.mul / z.per) : 0) + z.extra * e; }
+struct Kv8Cut { int mul, per, extra; };                // mul 0: `extra` slots per entry
+__device__ __forceinline__ int kv8_slot0(const TlmKv8Seqs& a, const Kv8Cut& z, int e) { return (z.mul ? (int)((long)kv8_row0(a, e) * z.mul / z.per) : 0) + z.extra * e; }
 __device__ __forceinline__ int kv8_find(const TlmKv8Seqs& a, const Kv8Cut& z, int slot) {
-    if (!a.row0) return min(slot / z.extra, a.n - 1);
+    if (!z.mul) return min(slot / z.extra, a.n - 1);
     unsigned below = 0;
     for (int e = mmi_lane(); e < a.n; e += 64) below += kv8_slot0(a, z, e) <= slot ? 1u : 0u;
     return max(mmi_uniform((int)mmi_wave_sum_u32(below) - 1), 0);
 }
-// host: the cut of `units` = mul * rows units, and how many slots there are
-inline Kv8Cut kv8_cut(const TlmKv8Seqs& a, int mul, int per, int more) { return Kv8Cut{mul, per, a.row0 ? more : mmi_cdiv(mul, per)}; }
-inline long kv8_slots(const TlmKv8Seqs& a, const Kv8Cut& z) { return (a.row0 ? (long)a.T * z.mul / z.per : 0) + (long)z.extra * a.n; }
+// host: the cut of mul * rows units (one row each: nothing to look for), and how many slots there are
+inline Kv8Cut kv8_cut(const TlmKv8Seqs& a, int mul, int per, int more) { return a.row0 ? Kv8Cut{mul, per, more} : Kv8Cut{0, per, mmi_cdiv(mul, per)}; }
+inline long kv8_slots(const TlmKv8Seqs& a, const Kv8Cut& z) { return (long)a.T * z.mul / z.per + (long)z.extra * a.n; }
 
 // ---- codes ---------------------------------------------------------------------------------------------------------------
 template <bool E4M3>
@@ -95,14 +93,10 @@ struct Kv8Code {
         }
         return o;
     }
-    static __device__ __forceinline__ u32x2 bf16(uint32_t w) {
-        if constexpr (E4M3) return mmi_fp8x4_to_bf16(w);
-        const f32x4 f = unpack(w);
-        return u32x2{mmi_pack_bf16x2(f[0], f[1]), mmi_pack_bf16x2(f[2], f[3])};
-    }
+    static __device__ __forceinline__ u32x2 f16(uint32_t w) { return E4M3 ? mmi_fp8x4_to_f16(w) : mmi_i8x4_to_f16(w); }
     // 16 codes -> two operand fragments of 8
     static __device__ __forceinline__ void fragments(u32x4 c, u32x4& lo, u32x4& hi) {
-        const u32x2 a = bf16(c[0]), b = bf16(c[1]), d = bf16(c[2]), e = bf16(c[3]);
+        const u32x2 a = f16(c[0]), b = f16(c[1]), d = f16(c[2]), e = f16(c[3]);
         lo = u32x4{a[0], a[1], b[0], b[1]};
         hi = u32x4{d[0], d[1], e[0], e[1]};
     }
@@ -331,10 +325,26 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------------
+// Numerics, both kernels.  Operands are fp16, 11 bits: codes are exact in it, queries are first brought to [2^14, 2^15) by a power of two of
+// their own, softmax weights are carried times the value scale of their block, relative to a running reference of score + log2 of that scale: so
+// the largest lie between 2^8 and 2^15 however blocks' scales differ, and the reference, with the sums, moves only where a maximum has outgrown
+// it by 2^7.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both operands come in two parts, 22 bits, good to 2^-24.
+// (bf16 operands left 1.8 times the error of the result's rounding.)  Sums, maxima and the denominator, which has the weights before they were
+// rounded, are fp32.
+constexpr int KV8_FEW = 64;              // sequences with up to so many columns go to k_tlm_kv8_attn where a call may bring longer ones
+constexpr float KV8_UP = 8.f, KV8_SLACK = 7.f;      // log2: of what weights are carried times, of what they may outgrow it by (fp16 ends at 2^16)
+constexpr int KV8_ANGLES = 2048;         // pairs of a cosine and a sine in LDS
+
+struct Kv8Share {                        // one kernel's part of a call
+    Kv8Cut z;                            // of columns (token, head of the group), by groups of z.per
+    int cols;                            // columns that a slot can have: z.per, or fewer where no group has more
+    int pages, nsplit;                   // pages per split; splits that a group can need
+    float* po;                           // nsplit > 1: [group slot][kv head][split][z.per columns][vdim] un-normalised sums
+    float* pml;                          // [group slot][kv head][split][2][z.per]: running maximum, sum of weights
+};
 struct TlmKv8Attn {
     TlmKv8Cache c;
     TlmKv8Seqs q;
-    Kv8Cut z;                            // of columns (token, head of the group), by tiles
     const void* x; long x_row, x_head;   // queries
     int wide;                            // every 4 of their elements are aligned
     void* out; long out_row, out_head;   // rows; out_ks > 0: fragment-packed rows (tlm_index), columns head * 16 nd + d
@@ -342,24 +352,22 @@ struct TlmKv8Attn {
     int heads, rep, nd;                  // rep: query heads per key/value head; nd: vdim / 16
     TlmMask mask;                        // scale: log2 e times the softmax's
     int sink;                            // one is added to the denominator
-    int per, nsplit;                     // pages per split; splits that a tile can need
-    float* po;                           // nsplit > 1: [tile slot][kv head][split][16 columns][vdim] un-normalised sums
-    float* pml;                          // [tile slot][kv head][split][2][16]: running maximum, sum of weights
+    int both;                            // sequences of more than KV8_FEW columns are `many`'s; otherwise all are `few`'s
+    Kv8Share few, many;
 };
 
-// columns (token, head of the group) c0 .. c0 + 15 of one entry, and the pages that they see: [0, n0) and [b0, b1)
+// columns c0 .. c0 + per - 1 of one entry, and the pages that they see: [0, n0) and [b0, b0 + n - n0)
 struct Kv8Cols {
     TlmKv8Seq s;
     int c0, ncol, plo, phi, n0, b0, n;
-    __device__ __forceinline__ Kv8Cols(const TlmKv8Attn& a, int slot) {
-        const int e = kv8_find(a.q, a.z, slot), per = a.z.per;
+    __device__ __forceinline__ Kv8Cols(const TlmKv8Attn& a, const Kv8Share& h, bool few, int slot) {
+        const int e = kv8_find(a.q, h.z, slot), per = h.z.per;
         s = kv8_seq(a.q, e);
-        c0 = (slot - kv8_slot0(a.q, a.z, e)) * per;
+        c0 = (slot - kv8_slot0(a.q, h.z, e)) * per;
         ncol = s.len * a.rep;
-        if (c0 >= ncol) {
-            n = n0 = b0 = 0;
-            return;
-        }
+        plo = phi = n = n0 = b0 = 0;
+        if (a.both && (ncol <= KV8_FEW) != few) ncol = 0;
+        if (c0 >= ncol) return;
         plo = s.pos0 + c0 / a.rep;
         phi = s.pos0 + min(c0 + per - 1, ncol - 1) / a.rep;
         const int w = a.mask.window;
@@ -369,23 +377,24 @@ struct Kv8Cols {
         if (!a.q.ring) n = min(n, n0 + max(a.q.pages.ld - b0, 0));
     }
     __device__ __forceinline__ int page(int i) const { return i < n0 ? i : b0 + i - n0; }
-    __device__ __forceinline__ bool seen(const TlmMask& m, int pos, int key) const { return key <= pos && (m.window <= 0 || pos - key < m.window || key < m.keep); }
-    // every column sees the whole page
-    __device__ __forceinline__ bool whole(const TlmMask& m, int key0) const { return key0 + TLM_PAGE - 1 <= plo && (m.window <= 0 || phi - key0 < m.window || key0 + TLM_PAGE <= m.keep); }
 };
-
-// fp32 -> NS parts of 8 bits of significand, pairs packed
-template <int NS>
-__device__ __forceinline__ void kv8_split2(float a, float b, uint32_t (&o)[NS]) {
-#pragma unroll
-    for (int p = 0; p < NS; ++p) {
-        o[p] = mmi_pack_bf16x2(a, b);
-        if (p + 1 < NS) {
-            a -= __builtin_bit_cast(float, o[p] << 16);
-            b -= __builtin_bit_cast(float, o[p] & 0xffff0000u);
-        }
+// The pages of a walk, 64 of them a load, a lane each: what a step's page is comes out of a register (a scalar load per step is a wait of its
+// own, and one for every LDS read in flight).  Asked for in ascending order.
+struct Kv8Pages {
+    int held, from;
+    __device__ __forceinline__ void fill(const TlmKv8Attn& a, const Kv8Cols& c, const int* bt, int i) {
+        from = i;
+        const int k = min(i + mmi_lane(), c.n - 1), p = c.page(max(k, 0));
+        held = kv8_page(a.q, a.c.n_pages, bt, p);
     }
-}
+    __device__ __forceinline__ int at(const TlmKv8Attn& a, const Kv8Cols& c, const int* bt, int i) {
+        if (i >= from + 64) fill(a, c, bt, i);
+        return mmi_from_lane(held, i - from);
+    }
+};
+__device__ __forceinline__ bool kv8_seen(const TlmMask& m, int pos, int key) { return key <= pos && (m.window <= 0 || pos - key < m.window || key < m.keep); }
+// positions plo .. phi all see the n keys from key0 on
+__device__ __forceinline__ bool kv8_whole(const TlmMask& m, int plo, int phi, int key0, int n) { return key0 + n - 1 <= plo && (m.window <= 0 || phi - key0 < m.window || key0 + n <= m.keep); }
 
 // e4m3 bytes of tokens that no column sees may hold anything, a NaN among it, which a weight of zero would not silence: cleared
 template <bool E4M3>
@@ -404,23 +413,120 @@ __device__ __forceinline__ u32x4 kv8_quiet(const Kv8Cols& c, const TlmMask& m, i
     return w;
 }
 
+// fp32 -> NS parts of fp16, pairs packed
+template <int NS>
+__device__ __forceinline__ void kv8_split2(float a, float b, uint32_t (&o)[NS]) {
+    o[0] = mmi_pack_f16x2(a, b);
+    if constexpr (NS == 2) {
+        const f32x2 h = mmi_unpack_f16x2(o[0]);
+        o[1] = mmi_pack_f16x2(a - h[0], b - h[1]);
+    }
+}
+template <int NS>
+__device__ __forceinline__ void kv8_split8(const float* x, float f, u32x4 (&q)[NS]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t o[NS];
+        kv8_split2<NS>(x[2 * j] * f, x[2 * j + 1] * f, o);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) q[s][j] = o[s];
+    }
+}
+// the power of two that brings `amax` to [2^14, 2^15), and its inverse (limits: 2^-100 and what is not finite)
+__device__ __forceinline__ float kv8_raise(float amax, float& back) {
+    const int e = max((int)(__builtin_bit_cast(unsigned, amax) >> 23) - 127, -100);
+    back = __builtin_bit_cast(float, (unsigned)(min(e, 127) - 14 + 127) << 23);
+    return __builtin_bit_cast(float, (unsigned)(14 - min(e, 127) + 127) << 23);
+}
+// dimensions d .. d + 3 of a query row, rotated (cs: its position's angles)
+template <class In>
+__device__ __forceinline__ f32x4 kv8_query4(const TlmKv8Attn& a, const In* row, int d, const float* cs) {
+    const bool wide = a.wide != 0;
+    f32x4 x = kv8_in4(row + d, wide);
+    const int rot = a.c.rot, half = rot / 2;
+    if (d >= rot) return x;
+    if (a.c.halves) {
+        const bool first = d < half;
+        const f32x4 y = kv8_in4(row + (first ? d + half : d - half), wide);
+        cs += 2 * (first ? d : d - half);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float re, im;
+            mmi_rope_rotate(first ? x[r] : y[r], first ? y[r] : x[r], cs[2 * r], cs[2 * r + 1], re, im);
+            x[r] = first ? re : im;
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            float re, im;
+            mmi_rope_rotate(x[r], x[r + 1], cs[d + r], cs[d + r + 1], re, im);
+            x[r] = re;
+            x[r + 1] = im;
+        }
+    }
+    return x;
+}
+// The group's queries into LDS as operand fragments, by the whole workgroup: D / 8 lanes a column, and a token's angles formed once for all
+// heads (a portion of the tokens at a time).  put(column, 8 dimensions d / 8 .., part): where they go; back: the columns' inverse factors.
+template <class In, int NS, int D, class Put>
+__device__ __forceinline__ void kv8_queries(const TlmKv8Attn& a, const Kv8Cols& c, int per, int g, float* angle, float* back, Put put) {
+    constexpr int G = D / 8, AT = 256 / G;                 // lanes a column, columns at a time
+    const int tid = (int)threadIdx.x, half = a.c.rot / 2, cols = min(per, c.ncol - c.c0), t1 = (c.c0 + cols - 1) / a.rep;
+    const int tokens = half ? KV8_ANGLES / half : t1 + 1;  // (half is 128 at most)
+    for (int t0 = c.c0 / a.rep; t0 <= t1; t0 += tokens) {
+        const int nt = min(tokens, t1 - t0 + 1), n0 = max(0, t0 * a.rep - c.c0), n1 = min(cols, (t0 + nt) * a.rep - c.c0);
+        if (half) {
+            __syncthreads();
+            for (int i = tid; i < nt * half; i += 256) kv8_angle(c.s.pos0 + t0 + i / half, a.c.freq[i % half], angle[2 * i], angle[2 * i + 1]);
+            __syncthreads();
+        }
+        for (int n = n0; n < n1; n += AT) {                // (every lane goes along: the maximum is taken across them)
+            const int k = min(n + tid / G, n1 - 1), col = c.c0 + k, tok = col / a.rep, d = 8 * (tid % G);
+            const In* row = (const In*)a.x + (long)(c.s.row0 + tok) * a.x_row + (g * a.rep + col - tok * a.rep) * a.x_head;
+            float x[8], top = 0.f;
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                const f32x4 v = d < a.c.dim ? kv8_query4(a, row, d + h, angle + (tok - t0) * 2 * half) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[h + r] = v[r];
+                    top = fmaxf(top, fabsf(v[r]));
+                }
+            }
+            u32x4 q[NS];
+            float b;
+            kv8_split8<NS>(x, kv8_raise(mmi_group_max<G>(top), b), q);
+            if (n + tid / G >= n1) continue;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) *put(k, tid % G, s) = q[s];
+            if (tid % G == 0) back[k] = b;
+        }
+    }
+    __syncthreads();
+}
 // four dimensions of a row's head
 template <class Tr>
 __device__ __forceinline__ void kv8_store(const TlmKv8Attn& a, int row, int head, int d, f32x4 v) {
     typedef typename Tr::elem E;
     Tr::store4((E*)a.out + (a.out_ks ? tlm_index<Tr>(row, head * 16 * a.nd + d, a.out_ks) : row * a.out_row + head * a.out_head + d), v);
 }
+// 1 / denominator of weights that were summed relative to 2^(M - KV8_UP); nothing seen: zero
+__device__ __forceinline__ float kv8_inverse(float L, float M, int sink) {
+    const float sum = sink ? L + exp2f(KV8_UP - M) : L;
+    return sum == 0.f ? 0.f : 1.f / sum;
+}
 
-// Four waves share one tile of 16 columns, each takes every fourth of its pages and their sums meet in LDS.
-// LDS: angles of the tile's tokens, then (the same memory) the waves' sums
-constexpr int KV8_LDS = 4 * 8 * 64;                        // vectors of four floats
+// Few columns: four waves share one tile of 16 columns, each takes every fourth of its pages straight from the cache - the page after it is
+// asked for before the products of this one - and their sums meet in LDS.
+// LDS: the queries and their angles, then (the same memory) the waves' sums
+constexpr int KV8_LDS = 4 * 8 * 64;                        // vectors of four floats: 8 waves' worth of 8 x 16 dimensions; queries of 256 in two parts and angles take 2048 too
 template <class In, class Tr, int NS, int D, bool E4M3>
 __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, float (*ml)[4][16], int slot, int g, int split) {
     typedef Kv8Code<E4M3> C;
     constexpr int NP = D / 64, ND = D / 16, WK = 4;
     const int lane = (int)threadIdx.x & 63, wave = mmi_uniform((int)threadIdx.x >> 6), bl = lane & 15, kq = lane >> 4;
-    const Kv8Cols c(a, slot);
-    const int i0 = split * a.per, i1 = min(c.n, i0 + a.per);
+    const Kv8Cols c(a, a.few, true, slot);
+    const int i0 = split * a.few.pages, i1 = min(c.n, i0 + a.few.pages);
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
     const int col = min(c.c0 + bl, c.ncol - 1), tok = col / a.rep, pos = c.s.pos0 + tok;
     const int* bt = kv8_table(a.q, c.s.e);
@@ -428,10 +534,13 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     float ks = 0.f, vs = 0.f;
     int nb = 0;
     bool have = false;
+    Kv8Pages pages;
+    pages.fill(a, c, bt, i0);
     // (past the end, and where there is no page: the pool's first one, unused)
     auto load = [&](int i) __attribute__((always_inline)) {
-        nb = c.page(min(i, i1 - 1));
-        const int p = kv8_page(a.q, a.c.n_pages, bt, nb);
+        i = min(i, i1 - 1);
+        nb = c.page(i);
+        const int p = pages.at(a, c, bt, i);
         have = p >= 0;
         const long unit = (long)max(p, 0) * a.c.kv_heads + g;
         const uint8_t* kp = a.c.k + (unit * TLM_PAGE + 16 * (bl >> 2) + (bl & 3)) * a.c.dim + 16 * kq;
@@ -446,62 +555,26 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         for (int d = 0; d < ND; ++d) vf[d] = mmi_load_nt((const u32x4*)(vp + min(d, a.nd - 1) * 16 * TLM_PAGE));
     };
     if (i0 + wave < i1) load(i0 + wave);
-    // the columns' queries, rotated: the tile's tokens are few, so their angles are formed once
-    float* angle = reinterpret_cast<float*>(ob);           // [token of the tile][rot / 2][cos, sin]
-    const int t0 = c.c0 / a.rep, nt = min(c.c0 + 15, c.ncol - 1) / a.rep - t0 + 1, half = a.c.rot / 2;
-    for (int i = (int)threadIdx.x; i < nt * half; i += 256) kv8_angle(c.s.pos0 + t0 + i / half, a.c.freq[i % half], angle[2 * i], angle[2 * i + 1]);
-    __syncthreads();
-    u32x4 q[NS][2 * NP];
-    {
-        const In* row = (const In*)a.x + (long)(c.s.row0 + tok) * a.x_row + (g * a.rep + col - tok * a.rep) * a.x_head;
-        const float* an = angle + (tok - t0) * 2 * half;
+    u32x4* qf = reinterpret_cast<u32x4*>(ob);              // fragments [p][part]: dimensions 64 (p / 2) + 16 kq + 8 (p & 1) ..
+    kv8_queries<In, NS, D>(a, c, 16, g, reinterpret_cast<float*>(ob + 2 * NP * NS * 64), &ml[0][0][0], [&](int n, int k, int s) __attribute__((always_inline)) {
+        return qf + ((2 * (k >> 3) + (k & 1)) * NS + s) * 64 + 16 * ((k >> 1) & 3) + n;
+    });
+    u32x4 q[2 * NP][NS];
 #pragma unroll
-        for (int p = 0; p < 2 * NP; ++p) {                 // dimensions 64 (p / 2) + 16 kq + 8 (p & 1) ..
-            const int d0 = 64 * (p >> 1) + 16 * kq + 8 * (p & 1);
+    for (int p = 0; p < 2 * NP; ++p)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int d = d0 + 4 * h;
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                if (d < a.c.dim) {
-                    x = kv8_in4(row + d, a.wide != 0);
-                    if (d < a.c.rot && a.c.halves) {
-                        const bool first = d < half;
-                        const f32x4 y = kv8_in4(row + (first ? d + half : d - half), a.wide != 0);
-                        const float* cs = an + 2 * (first ? d : d - half);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float re, im;
-                            mmi_rope_rotate(first ? x[r] : y[r], first ? y[r] : x[r], cs[2 * r], cs[2 * r + 1], re, im);
-                            x[r] = first ? re : im;
-                        }
-                    } else if (d < a.c.rot) {
-                        const float* cs = an + d;
-                        float re, im;
-                        mmi_rope_rotate(x[0], x[1], cs[0], cs[1], re, im);
-                        x[0] = re, x[1] = im;
-                        mmi_rope_rotate(x[2], x[3], cs[2], cs[3], re, im);
-                        x[2] = re, x[3] = im;
-                    }
-                }
-                uint32_t lo[NS], hi[NS];
-                kv8_split2<NS>(x[0], x[1], lo);
-                kv8_split2<NS>(x[2], x[3], hi);
-#pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    q[s][p][2 * h] = lo[s];
-                    q[s][p][2 * h + 1] = hi[s];
-                }
-            }
-        }
-    }
+        for (int s = 0; s < NS; ++s) q[p][s] = qf[(p * NS + s) * 64 + lane];
+    float back = ml[0][0][bl];
+    __syncthreads();                                       // (their memory takes the sums)
+    back *= a.mask.scale;
     f32x4 acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = a.sink ? 0.f : -INFINITY, l = 0.f;           // (a sink of score 0 takes part in the maximum)
+    float m = -INFINITY, l = 0.f;
     for (int i = i0 + wave; i < i1; i += WK) {
         const int key0 = nb * TLM_PAGE + 16 * kq;
-        const bool now = have, whole = c.whole(a.mask, nb * TLM_PAGE);
-        const float sc = ks * a.mask.scale, pv = vs;
+        const bool now = have, whole = kv8_whole(a.mask, c.plo, c.phi, nb * TLM_PAGE, TLM_PAGE);
+        const float sc = ks * back, lv = mmi_fast_log2f(fmaxf(vs, 0x1p-120f) + 0.f * vs), rv = mmi_fast_exp2f(-lv);      // (a NaN stays one)
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -512,8 +585,8 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
                 C::fragments(kf[t][p], lo, hi);
 #pragma unroll
                 for (int n = NS - 1; n >= 0; --n) {
-                    s[t] = mmi_mfma_bf16_16x16x32(lo, q[n][2 * p], s[t]);
-                    s[t] = mmi_mfma_bf16_16x16x32(hi, q[n][2 * p + 1], s[t]);
+                    s[t] = mmi_mfma_f16_16x16x32(lo, q[2 * p][n], s[t]);
+                    s[t] = mmi_mfma_f16_16x16x32(hi, q[2 * p + 1][n], s[t]);
                 }
             }
         }
@@ -523,36 +596,33 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         load(i + WK);
         mmi_sched_barrier();
         if (!now) continue;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            s[t] *= sc;
-            if (!whole)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] = c.seen(a.mask, pos, key0 + 4 * t + r) ? s[t][r] : -INFINITY;
-        }
-        float mx = m;
+        float mx = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
+            for (int r = 0; r < 4; ++r) {
+                s[t][r] = mmi_fma(s[t][r], sc, lv);
+                if (!whole) s[t][r] = kv8_seen(a.mask, pos, key0 + 4 * t + r) ? s[t][r] : -INFINITY;
+                mx = fmaxf(mx, s[t][r]);
+            }
         mx = mmi_rows_max(mx);
-        const float ms = mx == -INFINITY ? 0.f : mx;
-        if (mmi_any(mx > m)) {
-            const float al = mmi_fast_exp2f(m - ms);
+        if (mmi_any(mx > m + KV8_SLACK)) {
+            const float to = fmaxf(m, mx), al = mmi_fast_exp2f(m - (to == -INFINITY ? 0.f : to));
             l *= al;
 #pragma unroll
             for (int d = 0; d < ND; ++d) acc[d] *= al;
+            m = to;
         }
-        m = mx;
+        const float ms = (m == -INFINITY ? 0.f : m) - KV8_UP;
         u32x4 pf[NS][2];
+        float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             float e[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float x = mmi_fast_exp2f(s[t][r] - ms);
-                l += x;
-                e[r] = whole || x != 0.f ? x * pv : 0.f;   // (a masked place's scale may be anything)
+                e[r] = mmi_fast_exp2f(s[t][r] - ms);
+                sum += e[r];
             }
             uint32_t lo[NS], hi[NS];
             kv8_split2<NS>(e[0], e[1], lo);
@@ -563,14 +633,15 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
                 pf[n][t >> 1][2 * (t & 1) + 1] = hi[n];
             }
         }
+        l += sum == 0.f ? 0.f : sum * rv;                  // (the scale of a block that no column sees may be anything)
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             u32x4 lo, hi;
             C::fragments(vw[d], lo, hi);
 #pragma unroll
             for (int n = NS - 1; n >= 0; --n) {
-                acc[d] = mmi_mfma_bf16_16x16x32(lo, pf[n][0], acc[d]);
-                acc[d] = mmi_mfma_bf16_16x16x32(hi, pf[n][1], acc[d]);
+                acc[d] = mmi_mfma_f16_16x16x32(lo, pf[n][0], acc[d]);
+                acc[d] = mmi_mfma_f16_16x16x32(hi, pf[n][1], acc[d]);
             }
         }
     }
@@ -581,16 +652,16 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         ml[1][wave][bl] = l;
     }
     __syncthreads();
-    float M = a.sink ? 0.f : -INFINITY, L = 0.f;
+    float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int v = 0; v < WK; ++v) M = fmaxf(M, ml[0][v][bl]);
     const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int v = 0; v < WK; ++v) L += ml[1][v][bl] * exp2f(ml[0][v][bl] - Ms);
     const float f = exp2f(m - Ms);
-    const bool parts = a.nsplit > 1;
-    const float sum = a.sink ? L + exp2f(-Ms) : L, inv = parts ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);      // (no key seen: zeros)
-    const long part = ((long)slot * a.c.kv_heads + g) * a.nsplit + split;
+    const bool parts = a.few.nsplit > 1;
+    const float inv = parts ? 1.f : kv8_inverse(L, M, a.sink);
+    const long part = ((long)slot * a.c.kv_heads + g) * a.few.nsplit + split;
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += 8) {
         if (d0 >= a.nd) break;
@@ -609,13 +680,13 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
             v *= inv;
             if (c.c0 + bl >= c.ncol) continue;
             const int dim = (d0 + d) * 16 + 4 * kq, head = g * a.rep + col - tok * a.rep;
-            if (parts) *reinterpret_cast<f32x4*>(a.po + (part * 16 + bl) * a.c.vdim + dim) = v;
+            if (parts) *reinterpret_cast<f32x4*>(a.few.po + (part * 16 + bl) * a.c.vdim + dim) = v;
             else kv8_store<Tr>(a, c.s.row0 + tok, head, dim, v);
         }
     }
     if (parts && wave == 0 && kq == 0) {
-        a.pml[part * 32 + bl] = M;
-        a.pml[part * 32 + 16 + bl] = L;
+        a.few.pml[part * 32 + bl] = M;
+        a.few.pml[part * 32 + 16 + bl] = L;
     }
 }
 template <class In, class Tr, int NS, int D, bool E4M3>
@@ -625,48 +696,353 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8At
     tlm_kv8_attn<In, Tr, NS, D, E4M3>(a, ob, ml, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
 }
 
-// The splits of one column -> output: 16 groups of lanes take every 16th split, their sums meet in LDS.
-// grid: slots of column tiles, kv heads, columns of a tile
-template <class Tr>
-__global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a) {
-    MMI_SHARED float wt[256], red[4][2];
-    MMI_SHARED __attribute__((aligned(16))) f32x4 sum[256];
-    const Kv8Cols c(a, (int)blockIdx.x);
-    const int g = (int)blockIdx.y, bl = (int)blockIdx.z, col = c.c0 + bl, tid = (int)threadIdx.x, wave = tid >> 6;
-    if (col >= c.ncol) return;
-    const int ns = max(1, (c.n + a.per - 1) / a.per);      // (at most 256)
-    const long part = ((long)blockIdx.x * a.c.kv_heads + g) * a.nsplit;
-    float m = -INFINITY, l = 0.f;
-    if (tid < ns) {
-        m = a.pml[(part + tid) * 32 + bl];
-        l = a.pml[(part + tid) * 32 + 16 + bl];
+// Many columns: four waves x QT tiles of 32 columns of one sequence and kv head walk the same keys, 32 at a time.  Codes become operand
+// fragments on their way into LDS, once for all waves; 32 x 32 products read an operand half as often as 16 x 16 ones.  The scores of step
+// i + 1 are formed beside the softmax of step i; keys lie two steps ahead of their use and values one, one barrier a step.
+//   score rows: row 8 a + 4 h + i of the product is key 16 h + 4 a + i, so lane half h holds block h's 16 keys in order
+//   LDS, fragments of 64 lanes: key fragment j (16 dimensions) at lane ^ (j & 7), value fragment (32 dimensions, 8 keys of each block) at
+//   lane ^ 4 (lane / 32): what lets the writers, who have 16 codes of one key or dimension each, meet no bank twice
+template <int NS, int D>
+struct Kv8Tile {
+    static constexpr int QT = 1, PER = 128 * QT, KS = D / 16, DT = D / 32;
+    static constexpr int KF = KS * 64, VF = DT * 2 * 64;                       // vectors per buffer
+    static constexpr size_t smem() { return std::max((size_t)2 * (KF + VF) * 16, (size_t)PER * D * NS * 2 + PER * 4 + KV8_ANGLES * 8); }
+};
+template <class In, class Tr, int NS, int D, bool E4M3>
+__device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, int slot, int g, int split) {
+    typedef Kv8Code<E4M3> C;
+    typedef Kv8Tile<NS, D> Z;
+    constexpr int QT = Z::QT, KS = Z::KS, DT = Z::DT, KU = D > 128 ? 2 : 1;      // units of 16 codes per thread and side
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = mmi_uniform(tid >> 6), cl = lane & 31, hi = lane >> 5;
+    const Kv8Cols c(a, a.many, false, slot);
+    const int i0 = 2 * split * a.many.pages;
+    int i1 = min(2 * c.n, i0 + 2 * a.many.pages);
+    if (i1 == 2 * c.n && c.n > 0 && c.page(c.n - 1) * TLM_PAGE + 32 > c.phi) --i1;      // (the last page's second half lies ahead of every column)
+    if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
+    const int* bt = kv8_table(a.q, c.s.e);
+    const int w0 = c.c0 + wave * 32 * QT;                  // the wave's first column
+    const bool busy = w0 < c.ncol;
+    const int plo = c.s.pos0 + min(w0, c.ncol - 1) / a.rep, phi = c.s.pos0 + min(w0 + 32 * QT - 1, c.ncol - 1) / a.rep;
+    int tok[QT], head[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int col = min(w0 + 32 * t + cl, c.ncol - 1);
+        tok[t] = col / a.rep;
+        head[t] = g * a.rep + col - tok[t] * a.rep;
     }
-    const float wm = mmi_wave_max_f32(m);
-    if ((tid & 63) == 0) red[wave][0] = wm;
-    __syncthreads();
-    float M = a.sink ? 0.f : -INFINITY;
+    u32x4 q[QT][KS][NS];                                   // dimensions 16 s + 8 hi ..
+    float back[QT];
+    {
+        float* turned = reinterpret_cast<float*>(lds + Z::PER * D * NS / 8);      // inverse factors, then angles
+        kv8_queries<In, NS, D>(a, c, Z::PER, g, turned + Z::PER, turned, [&](int n, int k, int p) __attribute__((always_inline)) {
+            return lds + (((n >> 5) * KS + (k >> 1)) * NS + p) * 64 + 32 * (k & 1) + (n & 31);
+        });
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, red[w][0]);
-    M = M == -INFINITY ? 0.f : M;
-    const float w = tid < ns ? exp2f(m - M) : 0.f, wl = mmi_wave_sum_down(tid < ns ? l * w : 0.f);
-    wt[tid] = w;
-    if ((tid & 63) == 0) red[wave][1] = wl;
-    __syncthreads();
-    const float L = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]), total = a.sink ? L + exp2f(-M) : L, inv = total == 0.f ? 0.f : 1.f / total;
-    const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep, q = tid & 15, k = tid >> 4;
-    for (int d0 = 0; d0 < a.c.vdim; d0 += 64) {
-        const int d = d0 + 4 * q;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (d < a.c.vdim)
-#pragma unroll 4
-            for (int s = k; s < ns; s += 16) v += *(const f32x4*)(a.po + ((part + s) * 16 + bl) * a.c.vdim + d) * wt[s];
-        if (d0) __syncthreads();
-        sum[tid] = v;
+        for (int t = 0; t < QT; ++t) {
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int p = 0; p < NS; ++p) q[t][j][p] = lds[(((wave * QT + t) * KS + j) * NS + p) * 64 + lane];
+            back[t] = turned[(wave * QT + t) * 32 + cl] * a.mask.scale;
+        }
+        __syncthreads();                                   // (their memory takes keys and values)
+    }
+    // ---- codes -> LDS
+    u32x4 *kb = lds, *vb = lds + 2 * Z::KF;
+    for (int i = tid; i < 2 * Z::KF; i += 256)
+        if ((i % Z::KF) / 64 >= a.c.dim / 16) kb[i] = u32x4{0u, 0u, 0u, 0u};      // (dimensions past the head's)
+    u32x4 kr[KU], vr[KU];
+    int kput[KU], vput[KU];
+    bool kon[KU], von[KU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+        const int n = tid + 256 * u, nk = a.c.dim / 16, key = n / nk, j = n - key * nk;
+        kon[u] = key < 32;
+        kput[u] = j * 64 + ((8 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3)) ^ (j & 7));
+        const int d = n >> 1, b = n & 1;
+        von[u] = d < a.c.vdim;
+        vput[u] = (d >> 5) * 128 + ((b * 32 + (d & 31)) ^ (4 * b));
+    }
+    // pages of steps: a step's place is found when its keys are asked for, and handed down to its values and scales
+    struct At { long unit; int key0; bool have; };
+    Kv8Pages pages;
+    pages.fill(a, c, bt, i0 >> 1);
+    auto find = [&](int i) __attribute__((always_inline)) {       // (past the end: the last step again)
+        i = min(i, i1 - 1);
+        const int p = pages.at(a, c, bt, i >> 1);
+        return At{(long)max(p, 0) * a.c.kv_heads + g, c.page(i >> 1) * TLM_PAGE + 32 * (i & 1), p >= 0};
+    };
+    auto load_k = [&](const At& z) __attribute__((always_inline)) {
+        const uint8_t* p = a.c.k + (z.unit * TLM_PAGE + (z.key0 & 32)) * a.c.dim;
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+            if (kon[u]) kr[u] = *(const u32x4*)(p + 16 * (tid + 256 * u));
+    };
+    auto load_v = [&](const At& z) __attribute__((always_inline)) {
+        const uint8_t* p = a.c.v + z.unit * a.c.vdim * TLM_PAGE + (z.key0 & 32);
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+            if (von[u]) vr[u] = *(const u32x4*)(p + ((tid + 256 * u) >> 1) * TLM_PAGE + 16 * (tid & 1));
+    };
+    auto put_k = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            u32x4 lo, up;
+            C::fragments(kr[u], lo, up);
+            if (kon[u]) {
+                kb[buf * Z::KF + kput[u]] = lo;
+                kb[buf * Z::KF + kput[u] + 32] = up;
+            }
+        }
+    };
+    auto put_v = [&](int buf, int key0) __attribute__((always_inline)) {
+        const bool whole = kv8_whole(a.mask, c.plo, c.phi, key0, 32);
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            u32x4 lo, up;
+            C::fragments(whole ? vr[u] : kv8_quiet<E4M3>(c, a.mask, key0 + 16 * (tid & 1), vr[u]), lo, up);
+            if (von[u]) {
+                vb[buf * Z::VF + vput[u]] = lo;
+                vb[buf * Z::VF + vput[u] + 64] = up;
+            }
+        }
+    };
+    float ks = 0.f, vs = 0.f;
+    auto load_s = [&](const At& z) __attribute__((always_inline)) {
+        const long n = z.unit * KV8_PARTS + (z.key0 >> 4 & 2) + hi;
+        ks = a.c.ks[n];
+        vs = a.c.vs[n];
+    };
+    f32x16 acc[QT][DT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][d][r] = 0.f;
+    }
+    f32x16 s[2][QT];
+    u32x4 fr[8];                                           // operand fragments, asked for eight at a time
+    auto ask_k = [&](int buf, int j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < KS) fr[j] = kb[buf * Z::KF + (j0 + j) * 64 + (lane ^ j)];
+    };
+    auto scores = [&](int set, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[set][t][r] = 0.f;
+#pragma unroll
+        for (int j0 = 0; j0 < KS; j0 += 8) {
+            ask_k(buf, j0);
+            mmi_sched_barrier();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j0 + j < KS)
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+#pragma unroll
+                        for (int n = NS - 1; n >= 0; --n) s[set][t] = mmi_mfma_f16_32x32x16(fr[j], q[t][j0 + j][n], s[set][t]);
+        }
+    };
+    const int vl = lane ^ (4 * hi);
+    At z0, z1, z2;                                         // steps i, i + 1, i + 2
+    auto step = [&](int i, int set) __attribute__((always_inline)) {      // scores of step i in `set`, keys of step i + 1 in LDS, of step i + 2 in registers
+        const int key0 = z0.key0;
+        const bool now = z0.have;
+        const float ksn = ks, vsn = vs;
+        load_s(z1);
+        if (busy) scores(set ^ 1, set ^ 1);
+        if (busy && now && key0 <= phi) {
+            const bool whole = kv8_whole(a.mask, plo, phi, key0, 32);
+            const float lv = mmi_fast_log2f(fmaxf(vsn, 0x1p-120f) + 0.f * vsn), rv = mmi_fast_exp2f(-lv);
+            u32x4 pf[QT][2][NS];
+            float mx[QT];
+            bool moved = false;
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float sc = ksn * back[t];
+                const int pos = c.s.pos0 + tok[t];
+                float x = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float y = mmi_fma(s[set][t][r], sc, lv);
+                    if (!whole) y = kv8_seen(a.mask, pos, key0 + 16 * hi + r) ? y : -INFINITY;
+                    s[set][t][r] = y;
+                    x = fmaxf(x, y);
+                }
+                mx[t] = mmi_halves_max(x);
+                moved = moved || mx[t] > m[t] + KV8_SLACK;
+            }
+            if (mmi_any(moved)) {
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    const float to = fmaxf(m[t], mx[t]), al = mmi_fast_exp2f(m[t] - (to == -INFINITY ? 0.f : to));
+                    l[t] *= al;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[t][d] *= al;
+                    m[t] = to;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float ms = (m[t] == -INFINITY ? 0.f : m[t]) - KV8_UP;
+                float sum = 0.f, e[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    e[r] = mmi_fast_exp2f(s[set][t][r] - ms);
+                    sum += e[r];
+                }
+                l[t] += sum == 0.f ? 0.f : sum * rv;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) kv8_split8<NS>(e + 8 * u, 1.f, pf[t][u]);
+            }
+#pragma unroll
+            for (int d0 = 0; d0 < DT; d0 += 4) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (d0 + k / 2 < DT) fr[k] = vb[set * Z::VF + (2 * d0 + k) * 64 + vl];
+                mmi_sched_barrier();
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (d0 + k / 2 < DT)
+#pragma unroll
+                        for (int t = 0; t < QT; ++t)
+#pragma unroll
+                            for (int n = NS - 1; n >= 0; --n) acc[t][d0 + k / 2] = mmi_mfma_f16_32x32x16(fr[k], pf[t][k & 1][n], acc[t][d0 + k / 2]);
+            }
+        }
+        put_k(set);
+        put_v(set ^ 1, z1.key0);
+        z0 = z1;
+        z1 = z2;
+        z2 = find(i + 3);
+        load_k(z2);
+        load_v(z1);
         __syncthreads();
-        if (k == 0 && d < a.c.vdim) {
+    };
+    if (i0 < i1) {                                         // (step i0 is set 0: splits hold whole pages)
+        z0 = find(i0);
+        load_k(z0);
+        put_k(0);
+        z1 = find(i0 + 1);
+        load_k(z1);
+        load_v(z0);
+        load_s(z0);
+        __syncthreads();
+        if (busy) scores(0, 0);
+        put_k(1);
+        put_v(0, z0.key0);
+        z2 = find(i0 + 2);
+        load_k(z2);
+        load_v(z1);
+        __syncthreads();
+        for (int i = i0; i < i1; i += 2) {
+            step(i, 0);
+            if (i + 1 < i1) step(i + 1, 1);
+        }
+    }
+    const bool parts = a.many.nsplit > 1;
+    const long part = ((long)slot * a.c.kv_heads + g) * a.many.nsplit + split;
 #pragma unroll
-            for (int i = 1; i < 16; ++i) v += sum[16 * i + q];
-            kv8_store<Tr>(a, c.s.row0 + tok, head, d, v * inv);
+    for (int t = 0; t < QT; ++t) {
+        const int n = wave * 32 * QT + 32 * t + cl;        // column of the group
+        const float L = mmi_halves_sum(l[t]), inv = parts ? 1.f : kv8_inverse(L, m[t], a.sink);
+        if (c.c0 + n >= c.ncol) continue;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int dim = 32 * d + 8 * r + 4 * hi;
+                const f32x4 v = f32x4{acc[t][d][4 * r], acc[t][d][4 * r + 1], acc[t][d][4 * r + 2], acc[t][d][4 * r + 3]} * inv;
+                if (dim >= a.c.vdim) continue;
+                if (parts) *reinterpret_cast<f32x4*>(a.many.po + (part * Z::PER + n) * a.c.vdim + dim) = v;
+                else kv8_store<Tr>(a, c.s.row0 + tok[t], head[t], dim, v);
+            }
+        if (parts && hi == 0) {
+            a.many.pml[part * 2 * Z::PER + n] = m[t];
+            a.many.pml[part * 2 * Z::PER + Z::PER + n] = L;
+        }
+    }
+}
+// grid: kv heads x group slots (a head's groups on one XCD, the last groups, which see most keys, first), splits
+template <class In, class Tr, int NS, int D, bool E4M3>
+__global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(TlmKv8Attn a) {
+    MMI_DYN_SHARED(u32x4, lds);
+    const int b = (int)(gridDim.x - 1 - blockIdx.x);
+    tlm_kv8_tile<In, Tr, NS, D, E4M3>(a, lds, b / a.c.kv_heads, a.c.kv_heads - 1 - b % a.c.kv_heads, (int)blockIdx.y);
+}
+
+// The splits of one column -> output.  grid: columns of all slots (first the few's, then the many's), kv heads.
+// Up to 16 splits (WIDE false): a wave per column, a lane per split, then four dimensions a lane, all partial sums asked for at once.  More:
+// a workgroup per column, 16 groups of lanes take every 16th split, and their sums meet in LDS.
+template <class Tr, bool WIDE>
+__global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first_many, int columns) {
+    const int tid = (int)threadIdx.x, wave = mmi_uniform(tid >> 6), at = WIDE ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+    if (at >= columns) return;
+    const bool few = at < first_many;
+    const Kv8Share& h = few ? a.few : a.many;
+    const int b = at - (few ? 0 : first_many), slot = b / h.cols, n = b - slot * h.cols, per = h.z.per;
+    const Kv8Cols c(a, h, few, slot);
+    const int g = (int)blockIdx.y, col = c.c0 + n;
+    if (col >= c.ncol) return;
+    const int ns = max(1, (c.n + h.pages - 1) / h.pages);      // (at most 16, 256)
+    const long part = ((long)slot * a.c.kv_heads + g) * h.nsplit;
+    const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
+    if constexpr (!WIDE) {
+        const int lane = tid & 63, s = min(lane & 15, ns - 1), d = 4 * min(lane, a.c.vdim / 4 - 1);
+        const float m = h.pml[(part + s) * 2 * per + n], l = (lane & 15) < ns ? h.pml[(part + s) * 2 * per + per + n] : 0.f;
+        f32x4 v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (k < ns) v[k] = *(const f32x4*)(h.po + ((part + k) * per + n) * a.c.vdim + d);
+        const float M = mmi_group_max<16>(m), w = exp2f(m - (M == -INFINITY ? 0.f : M));
+        const float inv = kv8_inverse(mmi_row_sum(l * w), M, a.sink);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const float wk = mmi_shfl(w, k);
+            if (k < ns) o += v[k] * wk;
+        }
+        if (4 * lane < a.c.vdim) kv8_store<Tr>(a, c.s.row0 + tok, head, d, o * inv);
+    } else {
+        MMI_SHARED float wt[256], red[4][2];
+        MMI_SHARED __attribute__((aligned(16))) f32x4 sum[256];
+        float m = -INFINITY, l = 0.f;
+        if (tid < ns) {
+            m = h.pml[(part + tid) * 2 * per + n];
+            l = h.pml[(part + tid) * 2 * per + per + n];
+        }
+        const float wm = mmi_wave_max_f32(m);
+        if ((tid & 63) == 0) red[wave][0] = wm;
+        __syncthreads();
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, red[w][0]);
+        const float w = tid < ns ? exp2f(m - (M == -INFINITY ? 0.f : M)) : 0.f, wl = mmi_wave_sum_down(tid < ns ? l * w : 0.f);
+        wt[tid] = w;
+        if ((tid & 63) == 0) red[wave][1] = wl;
+        __syncthreads();
+        const float inv = kv8_inverse((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]), M, a.sink);
+        const int q = tid & 15, k = tid >> 4;
+        for (int d0 = 0; d0 < a.c.vdim; d0 += 64) {
+            const int d = d0 + 4 * q;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if (d < a.c.vdim)
+#pragma unroll 4
+                for (int s = k; s < ns; s += 16) v += *(const f32x4*)(h.po + ((part + s) * per + n) * a.c.vdim + d) * wt[s];
+            if (d0) __syncthreads();
+            sum[tid] = v;
+            __syncthreads();
+            if (k == 0 && d < a.c.vdim) {
+#pragma unroll
+                for (int i = 1; i < 16; ++i) v += sum[16 * i + q];
+                kv8_store<Tr>(a, c.s.row0 + tok, head, d, v * inv);
+            }
         }
     }
 }

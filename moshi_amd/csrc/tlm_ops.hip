@@ -6,7 +6,8 @@
 
 namespace {
 
-constexpr long KV8_WORKGROUPS = 1024;    // that a split of the pages aims at: 4 per CU, of which 2 run at a time
+constexpr long KV8_WORKGROUPS = 512;     // that a split of the pages aims at: 2 per CU, all at once
+constexpr long KV8_TILE_WORKGROUPS = 256;      // the same for many columns: one runs per CU
 constexpr int KV8_MAX_SPLIT = 256;       // (k_tlm_kv8_combine: a lane each)
 
 int check_cache(const mmi_kv_cache* c, TlmKv8Cache* out, const char* at) {
@@ -53,21 +54,44 @@ int launch_read(hipStream_t s, const TlmKv8Read& a, int dtype) {
     });
 }
 
-template <class In, class Tr, int NS, int D>
+template <class In, class Tr, int NS, int D, bool E4M3>
 int launch_attn(hipStream_t s, const TlmKv8Attn& a) {
-    const unsigned slots = (unsigned)kv8_slots(a.q, a.z);
-    if (a.c.e4m3) MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, true>), dim3(slots, a.c.kv_heads, a.nsplit), 256, 0, s, a);
-    else MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, false>), dim3(slots, a.c.kv_heads, a.nsplit), 256, 0, s, a);
-    if (a.nsplit > 1) MMI_LAUNCH((k_tlm_kv8_combine<Tr>), dim3(slots, a.c.kv_heads, std::min(16, a.q.row0 ? 16 : a.rep)), 256, 0, s, a);
+    if (a.both) {
+        constexpr size_t smem = Kv8Tile<NS, D>::smem();
+        static_assert(smem <= 160 * 1024, "LDS of a CU");
+        if (smem > 64 * 1024) {
+            static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            MMI_HIP_CHECK(attr);
+        }
+        MMI_LAUNCH((k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), dim3((unsigned)kv8_slots(a.q, a.many.z) * a.c.kv_heads, a.many.nsplit), 256, smem, s, a);
+    }
+    MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, E4M3>), dim3((unsigned)kv8_slots(a.q, a.few.z), a.c.kv_heads, a.few.nsplit), 256, 0, s, a);
+    const int few = a.few.nsplit > 1 ? (int)kv8_slots(a.q, a.few.z) * a.few.cols : 0, all = few + (a.both && a.many.nsplit > 1 ? (int)kv8_slots(a.q, a.many.z) * a.many.cols : 0);
+    if (!all) {}
+    else if (std::max(a.few.nsplit, a.both ? a.many.nsplit : 1) <= 16) MMI_LAUNCH((k_tlm_kv8_combine<Tr, false>), dim3(mmi_cdiv(all, 4), a.c.kv_heads), 256, 0, s, a, few, all);
+    else MMI_LAUNCH((k_tlm_kv8_combine<Tr, true>), dim3(all, a.c.kv_heads), 256, 0, s, a, few, all);
     MMI_CHECK_LAUNCH();
     return MMI_OK;
 }
+template <class In, class Tr, int NS, int D>
+int launch_attn_c(hipStream_t s, const TlmKv8Attn& a) { return a.c.e4m3 ? launch_attn<In, Tr, NS, D, true>(s, a) : launch_attn<In, Tr, NS, D, false>(s, a); }
+int attn_bound(const TlmKv8Cache& c) {                 // the kernels' bound on both head sizes
+    const int d = std::max(c.dim, c.vdim);
+    return d <= 64 ? 64 : (d <= 128 ? 128 : 256);
+}
 template <class In, class Tr, int NS>
 int launch_attn_d(hipStream_t s, const TlmKv8Attn& a) {
-    const int d = std::max(a.c.dim, a.c.vdim);
-    if (d <= 64) return launch_attn<In, Tr, NS, 64>(s, a);
-    if (d <= 128) return launch_attn<In, Tr, NS, 128>(s, a);
-    return launch_attn<In, Tr, NS, 256>(s, a);
+    const int d = attn_bound(a.c);
+    return d == 64 ? launch_attn_c<In, Tr, NS, 64>(s, a) : (d == 128 ? launch_attn_c<In, Tr, NS, 128>(s, a) : launch_attn_c<In, Tr, NS, 256>(s, a));
+}
+// how a kernel's groups share the pages out; floats of workspace
+size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, long workgroups) {
+    const long units = std::max(1l, groups * a.c.kv_heads);
+    long per = std::max((cap * units + workgroups - 1) / workgroups, (cap + KV8_MAX_SPLIT - 1) / KV8_MAX_SPLIT);
+    per = std::min((per + 3) / 4 * 4, (cap + 3) / 4 * 4);      // (each of a workgroup's four waves takes every fourth page)
+    h.pages = (int)per;
+    h.nsplit = (int)((cap + per - 1) / per);
+    return h.nsplit > 1 ? (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.nsplit * h.z.per * (a.c.vdim + 2) : 0;
 }
 
 }  // namespace
@@ -83,21 +107,36 @@ int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype) {
     });
 }
 
-size_t tlm_kv8_plan(TlmKv8Attn& a, long cap) {
-    a.z = kv8_cut(a.q, a.rep, 16, 1);
-    const long units = std::max(1l, kv8_slots(a.q, a.z) * a.c.kv_heads);
+size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, bool f32) {
     if (a.mask.window > 0) cap = std::min<long>(cap, (long)a.mask.window / TLM_PAGE + 3 + mmi_cdiv(a.mask.keep, TLM_PAGE));
     cap = std::max(cap, 1l);
-    long per = std::max((cap * units + KV8_WORKGROUPS - 1) / KV8_WORKGROUPS, (cap + KV8_MAX_SPLIT - 1) / KV8_MAX_SPLIT);
-    per = std::min((per + 3) / 4 * 4, (cap + 3) / 4 * 4);      // (each of the four waves takes every fourth page)
-    a.per = (int)per;
-    a.nsplit = (int)((cap + per - 1) / per);
-    return a.nsplit > 1 ? (size_t)units * a.nsplit * (16 * a.c.vdim + 32) : 0;
+    a.both = a.q.row0 != nullptr;
+    a.few.z = a.both ? Kv8Cut{0, 16, std::min(KV8_FEW / 16, mmi_cdiv(a.q.T * a.rep, 16))} : Kv8Cut{0, 16, mmi_cdiv(a.rep, 16)};
+    a.few.cols = std::min(16, a.both ? 16 : a.rep);
+    const size_t few = split_pages(a, a.few, a.both ? a.q.n : kv8_slots(a.q, a.few.z), cap, KV8_WORKGROUPS);
+    size_t many = 0;
+    if (a.both) {
+        a.many.z = Kv8Cut{a.rep, 128, 1};
+        a.many.cols = a.many.z.per;
+        many = split_pages(a, a.many, (long)a.q.T * a.rep / a.many.z.per + 1, cap, KV8_TILE_WORKGROUPS);
+    }
+    a.many.po = nullptr;
+    a.few.po = nullptr;
+    return few + many;
+}
+void tlm_kv8_workspace(TlmKv8Attn& a, float* w) {
+    for (Kv8Share* h : {&a.few, &a.many}) {
+        if (h->nsplit <= 1) continue;
+        const size_t parts = (size_t)kv8_slots(a.q, h->z) * a.c.kv_heads * h->nsplit * h->z.per;
+        h->po = w;
+        h->pml = w + parts * a.c.vdim;
+        w += parts * (a.c.vdim + 2);
+    }
 }
 
 int tlm_kv8_attend(hipStream_t s, const TlmKv8Attn& a, int dtype, bool f32) {
     if (dtype == MMI_BF16) return launch_attn_d<uint16_t, TlmBf16, 1>(s, a);
-    return f32 ? launch_attn_d<float, TlmF32, 3>(s, a) : launch_attn_d<float, TlmBf16, 1>(s, a);
+    return f32 ? launch_attn_d<float, TlmF32, 2>(s, a) : launch_attn_d<float, TlmBf16, 1>(s, a);
 }
 
 extern "C" int mmi_kv_append(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
@@ -133,7 +172,7 @@ extern "C" int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, i
 }
 
 namespace {
-int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first, TlmKv8Attn* a, size_t* floats) {
+int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t dtype, int32_t window, int32_t keep_first, TlmKv8Attn* a, size_t* floats) {
     memset(a, 0, sizeof(*a));
     int rc;
     if ((rc = check_cache(cache, &a->c, "mmi_kv_attend")) || (rc = check_seqs(seqs, &a->q, "mmi_kv_attend"))) return rc;
@@ -144,15 +183,15 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     a->nd = cache->vdim / 16;
     a->mask = TlmMask{window, window > 0 ? keep_first : 0, 0.f};
     if ((long)a->q.T * a->rep > 1l << 26) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^26 rows times query heads of a group");
-    *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1);
+    *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1, dtype == MMI_F32);
     return MMI_OK;
 }
 }  // namespace
 
-extern "C" int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first) {
+extern "C" int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, int32_t window, int32_t keep_first) {
     TlmKv8Attn a;
     size_t floats;
-    const int rc = attn_args(cache, seqs, heads, window, keep_first, &a, &floats);
+    const int rc = attn_args(cache, seqs, heads, dtype, window, keep_first, &a, &floats);
     return rc ? rc : (int64_t)(floats * sizeof(float));
 }
 
@@ -161,7 +200,7 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
                              mmi_stream stream) {
     TlmKv8Attn a;
     size_t floats;
-    int rc = attn_args(cache, seqs, heads, window, keep_first, &a, &floats);
+    int rc = attn_args(cache, seqs, heads, dtype, window, keep_first, &a, &floats);
     if (rc) return rc;
     if (!a.q.n || !a.q.T) return MMI_OK;
     if ((rc = check_rows(q, q_row, q_head, dtype, "mmi_kv_attend")) || (rc = check_rows(out, out_row, out_head, dtype, "mmi_kv_attend"))) return rc;
@@ -178,8 +217,7 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
     a.out_head = out_head;
     a.mask.scale = scale * 1.44269504088896340736f;
     a.sink = sink;
-    a.po = (float*)workspace;
-    a.pml = a.po + floats / (16 * a.c.vdim + 32) * (16 * a.c.vdim);
+    tlm_kv8_workspace(a, (float*)workspace);
     return tlm_kv8_attend((hipStream_t)stream, a, dtype, dtype == MMI_F32);
 }
 

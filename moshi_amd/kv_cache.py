@@ -66,7 +66,7 @@ class PagedKVCache:
             self._freq = torch.tensor(turns, dtype=torch.float64, device=self.device)
         self._desc = _capi.KVCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages, self.kv_heads, self.dim, self.vdim, _CODES[k.dtype],
                                        self.rot_dim, int(self.rot_halves), self._freq.data_ptr() if rot_dim else None)
-        self._lib.check(min(0, self._workspace(_capi.KVSeqs(), self.kv_heads, 0, 0)))      # (sizes that the kernels do not take are refused here)
+        self._lib.check(min(0, self._workspace(_capi.KVSeqs(), _capi.MMI_BF16, self.kv_heads, 0, 0)))      # (sizes that the kernels do not take are refused here)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, dim: int, vdim: Optional[int] = None, codes: str = "int8", device: torch.device | str = "cuda", **rotation) -> "PagedKVCache":
@@ -100,8 +100,8 @@ class PagedKVCache:
             raise ValueError(f"a head's dimensions lie side by side in {name}")
         return t.data_ptr(), t.stride(0), t.stride(1)
 
-    def _workspace(self, seqs: _capi.KVSeqs, heads: int, window: int, keep_first: int) -> int:
-        return self._lib.mmi_kv_attend_workspace(C.byref(self._desc), C.byref(seqs), heads, window, keep_first)
+    def _workspace(self, seqs: _capi.KVSeqs, dtype: int, heads: int, window: int, keep_first: int) -> int:
+        return self._lib.mmi_kv_attend_workspace(C.byref(self._desc), C.byref(seqs), dtype, heads, window, keep_first)
 
     # ---- computation -------------------------------------------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
@@ -128,7 +128,7 @@ class PagedKVCache:
             raise AssertionError("out is [rows, heads, vdim] in the queries' type")
         op = self._rows(out, "out", heads, self.vdim)
         with _capi.device_scope(self.device):
-            need = self._workspace(seqs, heads, window, keep_first)
+            need = self._workspace(seqs, _DTYPES[q.dtype], heads, window, keep_first)
             self._lib.check(min(0, need))
             work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
             self._lib.check(self._lib.mmi_kv_attend(C.byref(self._desc), C.byref(seqs), _DTYPES[q.dtype], heads, *qp, *op, self.dim ** -0.5 if scale is None else scale, window,

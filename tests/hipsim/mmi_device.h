@@ -219,6 +219,91 @@ inline u32x2 mmi_fp8x4_to_bf16(uint32_t w) {
     return u32x2{(b[0] >> 16) | (b[1] & 0xffff0000u), (b[2] >> 16) | (b[3] & 0xffff0000u)};
 }
 
+// ---- fp16 operands: software conversions (round-to-nearest-even, subnormals kept) ----
+namespace hipsim_detail {
+inline uint16_t f32_to_f16(float x) {
+    uint32_t u; memcpy(&u, &x, 4);
+    const uint16_t sign = (uint16_t)((u >> 16) & 0x8000u);
+    const float a = fabsf(x);
+    if (!(a == a)) return (uint16_t)(sign | 0x7e00u);
+    if (a >= 65520.f) return (uint16_t)(sign | 0x7c00u);
+    if (a < 6.103515625e-05f) return (uint16_t)(sign | (int)nearbyintf(a * 16777216.f));      // below 2^-14: a grid of 2^-24
+    int e; const float m = frexpf(a, &e);
+    int q = (int)nearbyintf((m * 2.f - 1.f) * 1024.f), E = e - 1 + 15;
+    if (q == 1024) { q = 0; E += 1; }
+    return (uint16_t)(sign | (E << 10) | q);
+}
+inline float f16_to_f32(uint16_t h) {
+    const int E = (h >> 10) & 31, m = h & 1023;
+    float v = E == 0 ? ldexpf((float)m, -24) : (E == 31 ? (m ? NAN : INFINITY) : ldexpf(1.f + (float)m / 1024.f, E - 15));
+    return (h & 0x8000u) ? -v : v;
+}
+}  // namespace hipsim_detail
+inline uint32_t mmi_pack_f16x2(float lo, float hi) { return (uint32_t)hipsim_detail::f32_to_f16(lo) | ((uint32_t)hipsim_detail::f32_to_f16(hi) << 16); }
+inline f32x2 mmi_unpack_f16x2(uint32_t w) { return f32x2{hipsim_detail::f16_to_f32((uint16_t)w), hipsim_detail::f16_to_f32((uint16_t)(w >> 16))}; }
+inline u32x2 mmi_fp8x4_to_f16(uint32_t w) {
+    float f[4];
+    mmi_fp8x4_to_f32(w, f);
+    return u32x2{mmi_pack_f16x2(f[0], f[1]), mmi_pack_f16x2(f[2], f[3])};
+}
+inline u32x2 mmi_i8x4_to_f16(uint32_t w) {
+    float f[4];
+    for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w >> (8 * i));
+    return u32x2{mmi_pack_f16x2(f[0], f[1]), mmi_pack_f16x2(f[2], f[3])};
+}
+inline f32x4 mmi_mfma_f16_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
+    using namespace hipsim_detail;
+    hipsim::Slot* s = hipsim::wave_slots();
+    const int l = hipsim::lane_id();
+    OpBF me;
+    memcpy(me.a, &a, 16);
+    memcpy(me.b, &b, 16);
+    memcpy(s[l].b, &me, sizeof(me));
+    hipsim::sync_wave();
+    f32x4 d;
+    const int j = l & 15;
+    for (int r = 0; r < 4; ++r) {
+        const int i = 4 * (l >> 4) + r;
+        float acc = c[r];
+        for (int k = 0; k < 32; ++k) {
+            OpBF oa, ob;
+            memcpy(&oa, s[i + 16 * (k >> 3)].b, sizeof(oa));
+            memcpy(&ob, s[j + 16 * (k >> 3)].b, sizeof(ob));
+            acc = fmaf(f16_to_f32(oa.a[k & 7]), f16_to_f32(ob.b[k & 7]), acc);
+        }
+        d[r] = acc;
+    }
+    hipsim::sync_wave();
+    return d;
+}
+inline f32x16 mmi_mfma_f16_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
+    using namespace hipsim_detail;
+    hipsim::Slot* s = hipsim::wave_slots();
+    const int l = hipsim::lane_id();
+    OpBF me;
+    memcpy(me.a, &a, 16);
+    memcpy(me.b, &b, 16);
+    memcpy(s[l].b, &me, sizeof(me));
+    hipsim::sync_wave();
+    f32x16 d;
+    const int j = l & 31;
+    for (int r = 0; r < 16; ++r) {
+        const int i = (r & 3) + 8 * (r >> 2) + 4 * (l >> 5);
+        float acc = c[r];
+        for (int k = 0; k < 16; ++k) {
+            OpBF oa, ob;
+            memcpy(&oa, s[i + 32 * (k >> 3)].b, sizeof(oa));
+            memcpy(&ob, s[j + 32 * (k >> 3)].b, sizeof(ob));
+            acc = fmaf(f16_to_f32(oa.a[k & 7]), f16_to_f32(ob.b[k & 7]), acc);
+        }
+        d[r] = acc;
+    }
+    hipsim::sync_wave();
+    return d;
+}
+inline float mmi_halves_max(float x) { return fmaxf(x, mmi_shfl_xor(x, 32)); }
+inline float mmi_halves_sum(float x) { return x + mmi_shfl_xor(x, 32); }
+
 inline f32x16 mmi_mfma_fp8_32x32x16(u32x2 a, u32x2 b, f32x16 c) {
     using namespace hipsim_detail;
     hipsim::Slot* s = hipsim::wave_slots();
@@ -399,6 +484,11 @@ inline float mmi_group_sum(float x) {
     for (int m = 1; m < W; m <<= 1) x += mmi_shfl_xor(x, m);
     return x;
 }
+template <int W>
+inline float mmi_group_max(float x) {
+    for (int m = 1; m < W; m <<= 1) x = fmaxf(x, mmi_shfl_xor(x, m));
+    return x;
+}
 inline float mmi_fma(float a, float b, float c) { return fmaf(a, b, c); }
 inline float mmi_dot2_bf16(uint32_t a, uint32_t b, float c) {
     using hipsim_detail::bf;
@@ -417,6 +507,7 @@ inline void mmi_sched_barrier() {}
 template <class T>
 inline void mmi_here(T&) {}
 inline int mmi_uniform(int v) { return v; }
+inline int mmi_from_lane(int v, int l) { return mmi_shfl(v, l); }
 inline int mmi_load_const(const int* p) { return *p; }
 inline bool mmi_any(bool v) { unsigned x = v ? 1u : 0u; for (int m = 1; m < 64; m <<= 1) { const unsigned o = mmi_shfl_xor(x, m); x = o > x ? o : x; } return x != 0; }
 inline void mmi_load_lds(const void* base, unsigned off, u32x4* lds, int at) { lds[at + (int)(threadIdx.x & 63)] = *(const u32x4*)((const char*)base + off); }
