@@ -319,6 +319,24 @@ def stream_ptr(device: torch.device) -> Optional[int]:
     return None
 
 
+class LaunchOn:
+    """Calls entry points on a GPU's current stream, with the GPU made current where it is not: what stream_ptr and device_scope do, without
+    building torch's objects for either (2 of 12 us of an operator's call)."""
+
+    def __init__(self, device: torch.device):
+        self.index = -1 if device.type != "cuda" else (torch.cuda.current_device() if device.index is None else device.index)
+
+    def stream(self) -> Optional[int]:
+        return None if self.index < 0 else torch._C._cuda_getCurrentRawStream(self.index)
+
+    def call(self, fn, *args) -> int:
+        """fn(*args, stream); its status."""
+        if self.index < 0 or torch._C._cuda_getDevice() == self.index:
+            return fn(*args, self.stream())
+        with torch.cuda.device(self.index):
+            return fn(*args, self.stream())
+
+
 def read_text(call) -> str:
     """A `(buf, cap) -> bytes needed` text getter of the ABI, sized and read."""
     need = int(call(None, 0))

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Dict, Optional, Sequence
 
 import torch
 
@@ -27,12 +27,20 @@ class BeamChoice:
     lengths: Optional[torch.Tensor]      # int32: tokens that it has (None without lengths)
 
 
-def _library(device: torch.device, lib: Optional[_capi.Lib]) -> _capi.Lib:
+_on: Dict[torch.device, _capi.LaunchOn] = {}
+_need: Dict[tuple, int] = {}             # bytes that a selection of (requests, beams, vocabulary) works in
+_I32, _F32, _BOOL = torch.int32, torch.float32, torch.bool
+
+
+def _place(device: torch.device, lib: Optional[_capi.Lib]):
     if lib is None:
         if device.type != "cuda":
             raise RuntimeError("moshi_amd.beam runs on an MI355X (device='cuda'); there is no CPU path")
         lib = _capi.load_tlm()
-    return lib
+    on = _on.get(device)
+    if on is None:
+        on = _on[device] = _capi.LaunchOn(device)
+    return lib, on
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[torch.Tensor] = None, finished: Optional[torch.Tensor] = None, eos: int = -1,
@@ -47,53 +55,59 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
         length_penalty: candidates are ranked by score / length ** length_penalty.
     Equal ranks go to the lower beam, then the lower token.  At most 32 beams.
     """
-    device = logits.device
-    lib = _library(device, lib)
-    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
+    device, shape = logits.device, scores.shape
+    lib, on = _place(device, lib)
+    if len(shape) != 2 or logits.dim() != 2 or logits.shape[0] != shape[0] * shape[1]:
         raise AssertionError("logits are [requests * beams, vocab], scores [requests, beams]")
-    if logits.dtype not in _DTYPES or (logits.stride(1) != 1 and logits.numel()):
+    (batch, beams), vocab, dtype, (row, step) = shape, logits.shape[1], _DTYPES.get(logits.dtype), logits.stride()
+    if dtype is None or (step != 1 and vocab > 1):
         raise ValueError("logits are bf16 or fp32, a row's side by side")
-    want = [("scores", scores, torch.float32), ("lengths", lengths, torch.int32), ("finished", finished, torch.bool)]
-    for name, t, dtype in want:
-        if t is not None and (t.shape != scores.shape or t.dtype != dtype or not t.is_contiguous() or t.device != device):
-            raise ValueError(f"{name} is a contiguous {dtype} tensor [requests, beams] on the logits' device")
+    where = logits.get_device()
+    for name, t, kind in (("scores", scores, _F32), ("lengths", lengths, _I32), ("finished", finished, _BOOL)):
+        if t is not None and (t.dtype is not kind or t.shape != shape or t.get_device() != where or not t.is_contiguous()):
+            raise ValueError(f"{name} is a contiguous {kind} tensor [requests, beams] on the logits' device")
     if length_penalty and lengths is None:
         raise ValueError("a length penalty needs lengths")
-    batch, beams = scores.shape
-    vocab = logits.shape[1]
-    new = lambda dtype: torch.empty((batch, beams), dtype=dtype, device=device)  # noqa: E731
-    r = BeamChoice(new(torch.float32), new(torch.int32), new(torch.int32), new(torch.bool) if eos >= 0 else None, None if lengths is None else new(torch.int32))
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with _capi.device_scope(device):
+    need = _need.get((batch, beams, vocab))
+    if need is None:
         need = lib.mmi_beam_select_workspace(batch, beams, vocab)
         lib.check(min(0, need))
-        work = torch.empty(need, dtype=torch.uint8, device=device)
-        lib.check(lib.mmi_beam_select(batch, beams, vocab, _DTYPES[logits.dtype], ptr(logits), logits.stride(0), ptr(scores), ptr(lengths), ptr(finished), int(eos),
-                                      float(length_penalty), ptr(r.scores), ptr(r.parents), ptr(r.tokens), ptr(r.finished), ptr(r.lengths), ptr(work), need,
-                                      _capi.stream_ptr(device)))
+        if len(_need) > 4096:
+            _need.clear()
+        _need[batch, beams, vocab] = need
+    parents, tokens, grown = torch.empty((3, batch, beams), dtype=_I32, device=device).unbind()
+    r = BeamChoice(torch.empty(shape, dtype=_F32, device=device), parents, tokens, torch.empty(shape, dtype=_BOOL, device=device) if eos >= 0 else None,
+                   None if lengths is None else grown)
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    lib.check(on.call(lib.mmi_beam_select, batch, beams, vocab, dtype, logits.data_ptr(), row, scores.data_ptr(), None if lengths is None else lengths.data_ptr(),
+                      None if finished is None else finished.data_ptr(), eos, length_penalty, r.scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                      None if eos < 0 else r.finished.data_ptr(), None if lengths is None else grown.data_ptr(), work.data_ptr(), need))
     return r
 
 
 def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, lib: Optional[_capi.Lib] = None) -> None:
     """In place, for every tensor [requests * beams, ...] of any type: row b * beams + i becomes a copy of what row b * beams + parents[b, i] was.
     parents: int32 [requests, beams]; one outside the request leaves its row alone.  A row's elements lie together; no two tensors share memory."""
-    device = parents.device
-    lib = _library(device, lib)
-    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous():
+    lib, on = _place(parents.device, lib)
+    if parents.dim() != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
         raise ValueError("parents is a contiguous int32 tensor [requests, beams]")
-    batch, beams = parents.shape
-    n = len(states)
-    at, stride, size = (C.c_void_p * max(1, n))(), (C.c_int64 * max(1, n))(), (C.c_int64 * max(1, n))()
-    k = 0
+    (batch, beams), where = parents.shape, parents.get_device()
+    total, at, stride, size = batch * beams, [], [], []
     for t in states:
-        if t.dim() < 1 or t.shape[0] != batch * beams:
+        if t.dim() < 1 or t.shape[0] != total:
             raise AssertionError("states are [requests * beams, ...]")
-        if t.device != device or not (t.is_contiguous() or t[:1].is_contiguous()):
+        if t.get_device() != where:
             raise ValueError("a state's rows are contiguous, on the parents' device")
-        if t.numel():
-            item = t.element_size()
-            at[k], size[k] = t.data_ptr(), t.numel() // t.shape[0] * item
-            stride[k] = t.stride(0) * item if t.shape[0] > 1 else size[k]
-            k += 1
-    with _capi.device_scope(device):
-        lib.check(lib.mmi_beam_reorder(k, at, stride, size, batch, beams, parents.data_ptr(), _capi.stream_ptr(device)))
+        nbytes = t.nbytes
+        if not nbytes:
+            continue
+        at.append(t.data_ptr())
+        size.append(nbytes // total)
+        if t.is_contiguous():
+            stride.append(nbytes // total)
+        else:
+            if not t[:1].is_contiguous():
+                raise ValueError("a state's rows are contiguous, on the parents' device")
+            stride.append(t.stride(0) * t.element_size())
+    n = len(at)
+    lib.check(on.call(lib.mmi_beam_reorder, n, (C.c_void_p * n)(*at), (C.c_int64 * n)(*stride), (C.c_int64 * n)(*size), batch, beams, parents.data_ptr()))

@@ -406,6 +406,11 @@ __device__ __forceinline__ int mmi_from_lane(int v, int l) { return __builtin_am
 // a load from memory that nothing writes while the kernel runs: by a uniform address a scalar load, also where the compiler cannot rule out that
 // one of the kernel's stores meets it
 __device__ __forceinline__ int mmi_load_const(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
+// what a wave's lanes wrote to LDS is there for its other lanes
+__device__ __forceinline__ void mmi_wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+// a bit per lane; lanes below this one among a mask's
+__device__ __forceinline__ uint64_t mmi_ballot(bool v) { return __ballot(v); }
+__device__ __forceinline__ int mmi_below(uint64_t m) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)); }
 // true in every lane when any lane's flag is set
 __device__ __forceinline__ bool mmi_any(bool v) { return __any(v) != 0; }
 

@@ -3,40 +3,30 @@
 //   candidate (beam k, token v) of a request: score s[k] + x[k, v] - log sum exp x[k, :], ranked by score / length^alpha
 //   finished beam: one candidate, its end token at the score it has
 //
-// Two launches: every workgroup takes BEAM_CHUNK logits of a row - its maximum, its sum of exponentials, and the best BEAMS of it in order - and one
-// wave per request merges these lists.  A row's own order is that of its logits, compared as they are; rows are compared in 64 bits.
+// Two launches: every wave takes BEAM_CHUNK logits of a row - its maximum, its sum of exponentials, and the best `beams` of it - and a workgroup per
+// request ranks what the waves found.  A row's own order is that of its logits, compared as they are; rows are compared in 64 bits.
 #pragma once
 #include "tlm_common.h"
 
-constexpr int BEAM_MAX = 32, BEAM_CHUNK = 4096, BEAM_TENSORS = 48;
+constexpr int BEAM_MAX = 32, BEAM_CHUNK = 1024, BEAM_TENSORS = 48;
 
 struct TlmBeamArgs {
     const void* x; long ld;              // logits, row stride in elements
-    int V, beams, splits;                // splits = ceil(V / BEAM_CHUNK)
+    int V, beams, chunks;                // chunks = ceil(V / BEAM_CHUNK)
     const float* score;                  // [batch][beams]
     const int* length;                   // null: no lengths
     const uint8_t* done;                 // null: none is finished
     int eos;
     double alpha;
-    float* wm; double* ws;               // [row][split]: maximum, sum of e^(x - maximum)
-    float* wx; int* wi;                  // [row][split][beams]: best logits and their tokens
+    float* wm; double* ws;               // [row][chunk]: maximum, sum of e^(x - maximum)
+    float* wx; int* wi;                  // [row][chunk][beams]: best logits and their tokens, in order; BEAM_NONE where there are fewer
     float* out_score; int* out_parent; int* out_token; uint8_t* out_done; int* out_length;
 };
+constexpr int BEAM_NONE = 0x7fffffff;
 
-// the larger of two (value, index) pairs, the lower index where the values are equal
+// before in the order: the larger value, the lower index where they are equal
 template <class T>
 __device__ __forceinline__ bool beam_better(T x, int i, T y, int j) { return x > y || (x == y && i < j); }
-template <class T>
-__device__ __forceinline__ void beam_wave_best(T& x, int& i) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const T ox = mmi_shfl_xor(x, m);
-        const int oi = mmi_shfl_xor(i, m);
-        const bool take = beam_better(ox, oi, x, i);
-        x = take ? ox : x;
-        i = take ? oi : i;
-    }
-}
 
 typedef f32x4 f32x4_loose __attribute__((aligned(4)));       // (rows of odd lengths begin anywhere)
 typedef u32x2 u32x2_loose __attribute__((aligned(2)));
@@ -49,17 +39,18 @@ __device__ __forceinline__ f32x4 beam_load4(const uint16_t* p) {
 __device__ __forceinline__ float beam_load(const float* p) { return *p; }
 __device__ __forceinline__ float beam_load(const uint16_t* p) { return mmi_bf16_to_f32(*p); }
 
-// grid: chunks, rows
+// A wave's best: the `beams`-th largest of the lanes' maxima is a bound that as many logits reach, and few more do, one or two beyond `beams` of
+// 1024 distinct ones: these are put side by side and ranked by counting who is before whom.  Where more than 64 reach it (equal logits), they are
+// taken out one at a time.  grid: chunks / 4, rows
 template <class In>
 __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
-    constexpr int N = BEAM_CHUNK / 256;                    // logits per lane, in runs of four
-    MMI_SHARED float lm[4], lx[4][BEAM_MAX];
-    MMI_SHARED double ls[4];
-    MMI_SHARED int li[4][BEAM_MAX];
-    const int row = (int)blockIdx.y, split = (int)blockIdx.x, lane = mmi_lane(), wave = mmi_uniform((int)threadIdx.x >> 6);
-    if (a.done && a.done[row]) return;
+    constexpr int N = BEAM_CHUNK / 64;                     // logits per lane, in runs of four
+    MMI_SHARED float cx[4][64];
+    MMI_SHARED int ci[4][64];
+    const int row = (int)blockIdx.y, lane = mmi_lane(), wave = mmi_uniform((int)threadIdx.x >> 6), chunk = (int)blockIdx.x * 4 + wave, K = a.beams;
+    if (chunk >= a.chunks || (a.done && a.done[row])) return;
     const In* x = (const In*)a.x + (long)row * a.ld;
-    const int v0 = split * BEAM_CHUNK + wave * (BEAM_CHUNK / 4) + 4 * lane;
+    const int v0 = chunk * BEAM_CHUNK + 4 * lane;
     float v[N];
 #pragma unroll
     for (int j = 0; j < N / 4; ++j) {
@@ -74,10 +65,10 @@ __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
         }
     }
     auto token = [&](int n) __attribute__((always_inline)) { return v0 + 256 * (n >> 2) + (n & 3); };
-    float m = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
-    for (int n = 0; n < N; ++n) m = fmaxf(m, v[n]);        // (NaN is passed over here and makes the sum one)
-    m = mmi_wave_max_f32(m);
+    for (int n = 0; n < N; ++n) top = fmaxf(top, v[n]);    // (NaN is passed over here and makes the sum one)
+    const float m = mmi_wave_max_f32(top);
     // e^d as 2^(d log2 e) with the product's low part carried along: the sum's relative error stays near 2^-28, where its logarithm is added to
     // scores whose order it decides.  Places past the vocabulary's end hold -infinity.
     constexpr float L = 1.44269504f, LL = 1.92596299e-8f;
@@ -92,181 +83,292 @@ __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
     double sum = (double)s;
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) sum += mmi_shfl_xor(sum, k);
-    // the wave's best, one at a time: every lane keeps its best one, and looks through the rest when that is taken
-    float best;
-    int at;
-    auto look = [&](float below, int after) __attribute__((always_inline)) {      // the best behind (below, after) in the order
-        best = -INFINITY;
-        at = 0x7fffffff;
+    const long part = (long)row * a.chunks + chunk;
+    if (lane == 0) {
+        a.wm[part] = m;
+        a.ws[part] = sum;
+    }
+    float* wx = a.wx + part * K;
+    int* wi = a.wi + part * K;
+    // the bound (of lanes with equal maxima each counts)
+    float bound = m;
+    {
+        float left = top;
+        for (int found = 0;;) {
+            const uint64_t at = mmi_ballot(left == bound);
+            found += __builtin_popcountll(at);
+            if (found >= K || bound == -INFINITY) break;
+            if (left == bound) left = -INFINITY;
+            bound = mmi_wave_max_f32(left);
+        }
+    }
+    int count = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const bool in = v[n] >= bound && token(n) < a.V;
+        const uint64_t at = mmi_ballot(in);
+        if (!at) continue;
+        const int k = count + mmi_below(at);
+        if (in && k < 64) {
+            cx[wave][k] = v[n];
+            ci[wave][k] = token(n);
+        }
+        count += __builtin_popcountll(at);
+    }
+    if (count <= 64) {
+        mmi_wave_sync();
+        const float y = lane < count ? cx[wave][lane] : -INFINITY;
+        const int i = lane < count ? ci[wave][lane] : BEAM_NONE;
+        int rank = 0;
+        for (int k = 0; k < count; ++k) rank += beam_better(cx[wave][k], ci[wave][k], y, i) ? 1 : 0;
+        if (lane < count && rank < K) {
+            wx[rank] = y;
+            wi[rank] = i;
+        }
+        if (lane >= count && lane < K) {
+            wx[lane] = -INFINITY;
+            wi[lane] = BEAM_NONE;
+        }
+        return;
+    }
+    float px = INFINITY;                                   // the one taken last
+    int pi = -1;
+    for (int k = 0; k < K; ++k) {
+        float y = -INFINITY;
+        int i = BEAM_NONE;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const float y = v[n] == v[n] ? v[n] : -INFINITY;
-            const int i = token(n);
-            const bool left = i < a.V && beam_better(below, after, y, i);
-            if (left && beam_better(y, i, best, at)) best = y, at = i;
+            const float z = v[n] == v[n] ? v[n] : -INFINITY;
+            if (token(n) < a.V && beam_better(px, pi, z, token(n)) && beam_better(z, token(n), y, i)) y = z, i = token(n);
         }
-    };
-    look(INFINITY, -1);
-    for (int k = 0; k < a.beams; ++k) {
-        float y = best;
-        int i = at;
-        beam_wave_best(y, i);
-        if (lane == 0) lx[wave][k] = y, li[wave][k] = i;
-        if (at == i && i != 0x7fffffff) look(y, i);
-    }
-    if (lane == 0) lm[wave] = m, ls[wave] = sum;
-    __syncthreads();
-    if (wave) return;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, lm[w]);
-    const long part = (long)row * a.splits + split;
-    if (lane == 0) {
-        double S = 0.;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) S += ls[w] == 0. ? 0. : ls[w] * exp((double)lm[w] - (double)M);
-        a.wm[part] = M;
-        a.ws[part] = S;
-    }
-    // the four waves' lists: 16 lanes a wave, two entries each
-    float y[2];
-    int i[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int k = (lane & 15) + 16 * h;
-        y[h] = k < a.beams ? lx[lane >> 4][k] : -INFINITY;
-        i[h] = k < a.beams ? li[lane >> 4][k] : 0x7fffffff;
-    }
-    for (int k = 0; k < a.beams; ++k) {
-        const bool second = beam_better(y[1], i[1], y[0], i[0]);
-        float b = second ? y[1] : y[0];
-        int j = second ? i[1] : i[0];
-        beam_wave_best(b, j);
-        if (lane == 0) a.wx[part * a.beams + k] = b, a.wi[part * a.beams + k] = j;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (i[h] == j) y[h] = -INFINITY, i[h] = 0x7fffffff;
+        px = mmi_wave_max_f32(y);
+        pi = (int)(0x7fffffffu - mmi_wave_max_u32(y == px ? 0x7fffffffu - (unsigned)i : 0u));
+        if (lane == 0) {
+            wx[k] = px;
+            wi[k] = pi;
+        }
     }
 }
 
-// One wave per request.  A list is a row's split, in order; a lane looks after every 64th and keeps the best head among them.
-__global__ __launch_bounds__(64) void k_tlm_beam_pick(TlmBeamArgs a) {
-    MMI_DYN_SHARED(int, head);                             // [beams * splits]: entries of a list that are taken
-    MMI_SHARED double base[BEAM_MAX], div[BEAM_MAX];       // score - log sum exp, length^alpha
-    MMI_SHARED int kind[BEAM_MAX];                         // 0: a row of logits; 1: finished; 2: no candidate with a chance
-    const int b = (int)blockIdx.x, lane = mmi_lane(), K = a.beams;
-    if (lane < K) {
-        const int row = b * K + lane;
+// A workgroup per request: 4096 of its candidates at a time in registers, 16 a lane, beside the best found so far.  As in the rows, a bound that
+// `beams` lanes of one wave reach leaves few to be ranked by counting; ranks rounded to 32 bits keep their order, which is all a bound needs.  A
+// candidate's place is beam * V + token.  (One at a time, a maximum over the workgroup for each: 25 us for 8 beams, 16 requests.)
+__global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
+    constexpr int N = 16;
+    MMI_SHARED double base[BEAM_MAX], inv[BEAM_MAX], bx[2][4], kx[2][BEAM_MAX];      // base: score - log sum exp; inv: 1 / length^alpha; kx: the best, in order
+    MMI_SHARED int kind[BEAM_MAX], bi[2][4], kp[2][BEAM_MAX];                        // kind 0: a row of logits; 1: finished; 2: no candidate with a chance
+    MMI_SHARED float ks[2][BEAM_MAX], wb[4], cs[4][64];
+    MMI_SHARED double cx[4][64];
+    MMI_SHARED int cp[4][64], cn[4];
+    const int b = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.beams;
+    // candidate n of the request: entry n % K of chunk n / K % chunks of beam n / K / chunks
+    const unsigned per = (unsigned)a.chunks * (unsigned)K;
+    const int all = K * (int)per;
+    const long first = (long)b * all;
+    double x[N + 1];
+    int p[N + 1];
+    float y[N + 1];
+    auto ask = [&](int n0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int n = min(n0 + tid + 256 * j, all - 1);
+            p[j] = a.wi[first + n];
+            y[j] = a.wx[first + n];
+        }
+    };
+    ask(0);
+    for (int k = wave; k < K; k += 4) {
+        const int row = b * K + k;
         const bool done = a.done && a.done[row];
-        const int len = a.length ? a.length[row] + (done ? 0 : 1) : 1;
         const double s = (double)a.score[row];
         double z = s;
         if (!done) {
             float M = -INFINITY;
-            for (int i = 0; i < a.splits; ++i) M = fmaxf(M, a.wm[(long)row * a.splits + i]);
+            for (int i = lane; i < a.chunks; i += 64) M = fmaxf(M, a.wm[(long)row * a.chunks + i]);
+            M = mmi_wave_max_f32(M);
             double S = 0.;
-            for (int i = 0; i < a.splits; ++i) {
-                const double w = a.ws[(long)row * a.splits + i];
-                S += w == 0. ? 0. : w * exp((double)a.wm[(long)row * a.splits + i] - (double)M);
+            for (int i = lane; i < a.chunks; i += 64) {
+                const double w = a.ws[(long)row * a.chunks + i];
+                S += w == 0. ? 0. : w * exp((double)a.wm[(long)row * a.chunks + i] - (double)M);
             }
+#pragma unroll
+            for (int i = 1; i < 64; i <<= 1) S += mmi_shfl_xor(S, i);
             z = s - ((double)M + log(S));
         }
-        base[lane] = z;
-        div[lane] = a.alpha == 0. ? 1. : pow((double)max(len, 1), a.alpha);
-        kind[lane] = z > -INFINITY && z < INFINITY ? (done ? 1 : 0) : 2;
+        if (lane == 0) {
+            const int len = a.length ? a.length[row] + (done ? 0 : 1) : 1;
+            base[k] = z;
+            inv[k] = a.alpha == 0. ? 1. : pow((double)max(len, 1), -a.alpha);
+            kind[k] = z > -INFINITY && z < INFINITY ? (done ? 1 : 0) : 2;
+        }
     }
-    const int lists = K * a.splits;
-    for (int i = lane; i < lists; i += 64) head[i] = 0;
-    __syncthreads();
-    // entry h of list i: its rank, and its place beam * V + token (as 64 bits: 32 beams of a vocabulary above 2^26)
-    auto entry = [&](int i, int h, double& rank, double& score, int& token) __attribute__((always_inline)) {
-        const int k = i / a.splits, split = i - k * a.splits;
-        token = 0x7fffffff;
-        score = rank = -INFINITY;
-        if (h >= K) return;
-        if (kind[k] != 0) {                                // a list in the first split alone: the end token, and what else there is, in order
-            if (split) return;
-            const int skip = kind[k] == 1 ? a.eos : a.V;
-            token = kind[k] == 1 ? (h == 0 ? skip : (h - 1 < skip ? h - 1 : h)) : h;
-            if (token >= a.V) token = 0x7fffffff;
-            if (kind[k] == 1 && h == 0) score = base[k];
-        } else {
-            const long at = ((long)(b * K + k) * a.splits + split) * K + h;
-            token = a.wi[at];
-            score = token == 0x7fffffff ? -INFINITY : base[k] + (double)a.wx[at];
+    x[N] = -INFINITY;
+    p[N] = BEAM_NONE;
+    y[N] = -INFINITY;
+    int set = 0;
+    for (int n0 = 0; n0 < all; n0 += 256 * N, set ^= 1) {
+        if (n0) ask(n0);
+        __syncthreads();
+        if (n0 && tid < K) {                               // (place BEAM_NONE: there was none)
+            x[N] = kx[set ^ 1][tid];
+            p[N] = kp[set ^ 1][tid];
+            y[N] = ks[set ^ 1][tid];
         }
-        rank = score / div[k];
-    };
-    double best, bscore;
-    int blist, btoken;
-    auto look = [&]() __attribute__((always_inline)) {
-        best = bscore = -INFINITY;
-        blist = btoken = 0x7fffffff;
-        for (int i = lane; i < lists; i += 64) {
-            double r, s;
-            int t;
-            entry(i, head[i], r, s, t);
-            // equal ranks: the lower beam, then the lower token; lists of one lane come in the order of their beams
-            const bool same = blist != 0x7fffffff && i / a.splits == blist / a.splits;
-            if (t != 0x7fffffff && (blist == 0x7fffffff || r > best || (r == best && same && t < btoken))) best = r, bscore = s, blist = i, btoken = t;
-        }
-    };
-    look();
-    for (int n = 0; n < K; ++n) {
-        double r = best;
-        int k = blist == 0x7fffffff ? 0x7fffffff : blist / a.splits, t = btoken;
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const double ro = mmi_shfl_xor(r, m);
-            const int ko = mmi_shfl_xor(k, m), to = mmi_shfl_xor(t, m);
-            const bool take = ko != 0x7fffffff && (k == 0x7fffffff || ro > r || (ro == r && (ko < k || (ko == k && to < t))));
-            r = take ? ro : r;
-            k = take ? ko : k;
-            t = take ? to : t;
+        for (int j = 0; j < N; ++j) {
+            const int n = n0 + tid + 256 * j, k = min((int)((unsigned)n / per), K - 1), h = n - k * (int)per;
+            int token = n < all ? p[j] : BEAM_NONE;
+            double s = -INFINITY;
+            if (kind[k] == 0) {
+                if (token != BEAM_NONE) s = base[k] + (double)y[j];
+            } else {                                       // no logits to choose from: the end token, then what else there is, in order, as the first entries
+                token = kind[k] == 2 ? h : (h == 0 ? a.eos : (h - 1 < a.eos ? h - 1 : h));
+                if (h >= K || n >= all || token >= a.V) token = BEAM_NONE;
+                if (kind[k] == 1 && h == 0) s = base[k];
+            }
+            x[j] = s * inv[k];
+            y[j] = (float)s;
+            p[j] = token == BEAM_NONE ? BEAM_NONE : k * a.V + token;      // (below 2^25)
         }
-        if (blist != 0x7fffffff && blist / a.splits == k && btoken == t) {      // one lane's
-            const int o = b * K + n, row = b * K + k;
-            const bool done = a.done && a.done[row];
-            a.out_score[o] = (float)bscore;
-            a.out_parent[o] = k;
-            a.out_token[o] = t;
-            if (a.out_done) a.out_done[o] = done || t == a.eos;
-            if (a.out_length) a.out_length[o] = (a.length ? a.length[row] : 0) + (done ? 0 : 1);
-            ++head[blist];
-            look();
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j <= N; ++j) top = fmaxf(top, p[j] == BEAM_NONE ? -INFINITY : (float)x[j]);
+        float bound = mmi_wave_max_f32(top);
+        {
+            float left = top;
+            for (int found = 0;;) {
+                found += __builtin_popcountll(mmi_ballot(left == bound));
+                if (found >= K || bound == -INFINITY) break;
+                if (left == bound) left = -INFINITY;
+                bound = mmi_wave_max_f32(left);
+            }
         }
+        if (lane == 0) wb[wave] = bound;
+        __syncthreads();
+        bound = fmaxf(fmaxf(wb[0], wb[1]), fmaxf(wb[2], wb[3]));
+        int count = 0;
+#pragma unroll
+        for (int j = 0; j <= N; ++j) {
+            const bool in = p[j] != BEAM_NONE && (float)x[j] >= bound;
+            const uint64_t at = mmi_ballot(in);
+            if (!at) continue;
+            const int k = count + mmi_below(at);
+            if (in && k < 64) {
+                cx[wave][k] = x[j];
+                cp[wave][k] = p[j];
+                cs[wave][k] = y[j];
+            }
+            count += __builtin_popcountll(at);
+        }
+        if (lane == 0) cn[wave] = count;
+        if (tid < K) kp[set][tid] = BEAM_NONE;             // (fewer candidates than beams so far)
+        __syncthreads();
+        if (max(max(cn[0], cn[1]), max(cn[2], cn[3])) <= 64) {
+            if (lane < count) {
+                const double m = cx[wave][lane];
+                const int q = cp[wave][lane];
+                int rank = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    for (int k = 0; k < cn[w]; ++k) rank += beam_better(cx[w][k], cp[w][k], m, q) ? 1 : 0;
+                if (rank < K) {
+                    kx[set][rank] = m;
+                    kp[set][rank] = q;
+                    ks[set][rank] = cs[wave][lane];
+                }
+            }
+            continue;
+        }
+        // many candidates of equal rank: one at a time
+        for (int n = 0; n < K; ++n) {
+            double m = -INFINITY;
+            int q = BEAM_NONE;
+            float s = -INFINITY;
+#pragma unroll
+            for (int j = 0; j <= N; ++j)
+                if (p[j] != BEAM_NONE && beam_better(x[j], p[j], m, q)) m = x[j], q = p[j], s = y[j];
+            const int mine = q;
+            double least = -m;
+            mmi_wave_pair_min(least, q);
+            if (lane == 0) {
+                bx[n & 1][wave] = least;
+                bi[n & 1][wave] = q;
+            }
+            __syncthreads();
+            least = bx[n & 1][0];
+            q = bi[n & 1][0];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) mmi_pair_min(least, q, bx[n & 1][w], bi[n & 1][w]);
+            if (mine == q && q != BEAM_NONE) {             // (places differ: one lane's)
+                kx[set][n] = -least;
+                kp[set][n] = q;
+                ks[set][n] = s;
+#pragma unroll
+                for (int j = 0; j <= N; ++j) p[j] = p[j] == q ? BEAM_NONE : p[j];
+            }
+        }
+    }
+    __syncthreads();
+    set ^= 1;
+    if (tid < K) {
+        const int o = b * K + tid, k = kp[set][tid] / a.V, t = kp[set][tid] - k * a.V, row = b * K + k;
+        const bool done = a.done && a.done[row];
+        a.out_score[o] = ks[set][tid];
+        a.out_parent[o] = k;
+        a.out_token[o] = t;
+        if (a.out_done) a.out_done[o] = done || t == a.eos;
+        if (a.out_length) a.out_length[o] = (a.length ? a.length[row] : 0) + (done ? 0 : 1);
     }
 }
 
 // ---- reorder: row r of a request's `beams` rows becomes a copy of what row parent[r] was, in place ------------------------------
 struct TlmReorder {
-    struct T { char* p; long stride; unsigned units, block0; } t[BEAM_TENSORS];      // base, bytes from row to row, units per row, first workgroup
+    struct T { char* p; long stride; unsigned units, block0; int unit; } t[BEAM_TENSORS];      // base, bytes from row to row, units per row and their bytes, first workgroup
     int n, beams;
     const int* parent;                   // [requests][beams], within the request
     const int* row;                      // null: rows in order
 };
-// U bytes a unit.  A lane owns a column of a request: it has read all of it before it writes any, so rows may change places.
-// grid: column blocks of all tensors, requests
+// A lane owns a unit of the request's rows: it has read all of it before it writes any, so rows may change places.  Rows that stay are not written,
+// and in their place a row that some other one needs is asked for again: a load behind a branch would wait for the one before it (315 us
+// instead of 195 for 64 rows of 13 MB).
 template <class U, int K>
+__device__ __forceinline__ void beam_move(const TlmReorder::T& t, const int (&from)[K], const int (&to)[K], unsigned moved, unsigned u) {
+    U v[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = ((const U*)(t.p + (long)from[i] * t.stride))[u];
+    mmi_sched_barrier();
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+        if (moved >> i & 1) ((U*)(t.p + (long)to[i] * t.stride))[u] = v[i];
+}
+// grid: blocks of units of all tensors, requests
+template <int K>
 __global__ __launch_bounds__(256) void k_tlm_reorder(TlmReorder a) {
+    const int base = (int)blockIdx.y * a.beams;
+    int from[K], to[K], some = -1;
+    unsigned moved = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        to[i] = min(i, a.beams - 1);
+        from[i] = mmi_load_const(a.parent + base + to[i]);
+        if (i < a.beams && from[i] != i && from[i] >= 0 && from[i] < a.beams) {      // (a parent that does not exist: the row stays)
+            moved |= 1u << i;
+            some = from[i];
+        }
+    }
+    if (!moved) return;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const int f = base + (moved >> i & 1 ? from[i] : some), r = base + to[i];
+        from[i] = a.row ? mmi_load_const(a.row + f) : f;
+        to[i] = a.row ? mmi_load_const(a.row + r) : r;
+    }
     int n = 0;
     while (n + 1 < a.n && a.t[n + 1].block0 <= blockIdx.x) ++n;
     const TlmReorder::T t = a.t[n];
     const unsigned u = (blockIdx.x - t.block0) * 256u + threadIdx.x;
     if (u >= t.units) return;
-    const int base = (int)blockIdx.y * a.beams;
-    U v[K];
-    int p[K];
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-        p[i] = i < a.beams ? a.parent[base + i] : i;
-        if (p[i] < 0 || p[i] >= a.beams) p[i] = i;         // (a parent that does not exist: the row stays)
-    }
-    auto at = [&](int i) __attribute__((always_inline)) { return (U*)(t.p + (long)(a.row ? a.row[base + i] : base + i) * t.stride) + u; };
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-        if (p[i] != i) v[i] = *at(p[i]);
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-        if (p[i] != i) *at(i) = v[i];
+    if (t.unit == 16) beam_move<u32x4, K>(t, from, to, moved, u);
+    else if (t.unit == 4) beam_move<uint32_t, K>(t, from, to, moved, u);
+    else beam_move<uint8_t, K>(t, from, to, moved, u);
 }

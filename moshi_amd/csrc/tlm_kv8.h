@@ -120,32 +120,33 @@ __device__ __forceinline__ void kv8_angle(int pos, double freq, float& c, float&
     const double t = (double)pos * freq;
     mmi_sincos_turns((float)(t - rint(t)), s, c);
 }
-// dimensions d .. d + 3 (d a multiple of 4) of a row, rotated
-template <class In>
-__device__ __forceinline__ f32x4 kv8_rotated4(const In* row, int d, int pos, int rot, int halves, const double* freq, bool wide) {
-    f32x4 x = kv8_in4(row + d, wide);
-    if (d >= rot) return x;
-    if (halves) {
-        const int h = rot / 2, i = d < h ? d : d - h;
-        const f32x4 y = kv8_in4(row + (d < h ? d + h : d - h), wide);
+// dimensions d .. d + 3 (d a multiple of 4) turned (cs: the position's angles; y: the partners, where these lie half of the dimensions apart)
+__device__ __forceinline__ f32x4 kv8_turned4(const TlmKv8Cache& c, f32x4 x, f32x4 y, int d, const float* cs) {
+    if (d >= c.rot) return x;
+    if (c.halves) {
+        const bool first = d < c.rot / 2;
+        cs += 2 * (first ? d : d - c.rot / 2);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float c, s, re, im;
-            kv8_angle(pos, freq[i + r], c, s);
-            mmi_rope_rotate(d < h ? x[r] : y[r], d < h ? y[r] : x[r], c, s, re, im);
-            x[r] = d < h ? re : im;
+            float re, im;
+            mmi_rope_rotate(first ? x[r] : y[r], first ? y[r] : x[r], cs[2 * r], cs[2 * r + 1], re, im);
+            x[r] = first ? re : im;
         }
     } else {
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-            float c, s, re, im;
-            kv8_angle(pos, freq[(d + r) / 2], c, s);
-            mmi_rope_rotate(x[r], x[r + 1], c, s, re, im);
+            float re, im;
+            mmi_rope_rotate(x[r], x[r + 1], cs[d + r], cs[d + r + 1], re, im);
             x[r] = re;
             x[r + 1] = im;
         }
     }
     return x;
+}
+template <class In>
+__device__ __forceinline__ f32x4 kv8_partners4(const TlmKv8Cache& c, const In* row, int d, bool wide) {
+    const int rot = c.halves ? c.rot : 0, half = rot / 2;
+    return d < rot ? kv8_in4(row + (d < half ? d + half : d - half), wide) : f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
 // ---- append --------------------------------------------------------------------------------------------------------------
@@ -194,32 +195,48 @@ __device__ __forceinline__ unsigned kv8_bits(f32x4 x) {
     return m;
 }
 
-// One wave per block, head and side.  grid: slots of blocks, kv heads, 2 (keys, values)
+// One wave per block, head and side; four heads a workgroup, which form the angles of the block's tokens once.
+// grid: slots of blocks, kv heads / 4, 2 (keys, values)
 //   keys: four lanes per token, granules of 4 dimensions in turn      values: a lane per dimension, its 16 tokens side by side
 template <class In, bool E4M3>
-__global__ __launch_bounds__(64) void k_tlm_kv8_append(TlmKv8Append a) {
+__global__ __launch_bounds__(256) void k_tlm_kv8_append(TlmKv8Append a) {
     typedef Kv8Code<E4M3> C;
+    MMI_SHARED float angle[KV8_BLOCK * 2 * 128];           // [token][pair][cos, sin]
     const Kv8Span s = kv8_span(a.q, a.z, a.c.n_pages, (int)blockIdx.x);
     if (s.none) return;
-    const int lane = mmi_lane(), g = (int)blockIdx.y, part = s.part;
+    const int lane = mmi_lane(), g = (int)blockIdx.y * 4 + mmi_uniform((int)threadIdx.x >> 6), part = s.part;
     const bool held = s.lo > 0, wide = a.wide != 0;
     const long unit = (long)s.page * a.c.kv_heads + g;
     if (blockIdx.z == 0) {
-        const int t = lane >> 2, c = lane & 3, n = a.c.dim / 16;
-        const In* row = (const In*)a.k + (long)(s.row + t) * a.k_row + g * a.k_head;
+        const int t = lane >> 2, c = lane & 3, n = a.c.dim / 16, half = a.c.rot / 2;
+        const In* row = (const In*)a.k + (long)(s.row + t) * a.k_row + (long)g * a.k_head;
         uint32_t* out = (uint32_t*)(a.c.k + (unit * TLM_PAGE + part * KV8_BLOCK + t) * a.c.dim);
-        const bool fresh = t >= s.lo && t < s.hi;
-        f32x4 x[16];
+        const bool fresh = t >= s.lo && t < s.hi && g < a.c.kv_heads;
+        f32x4 x[16], y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < n && fresh) {
+                x[i] = kv8_in4(row + 4 * (c + 4 * i), wide);
+                y[i] = kv8_partners4(a.c, row, 4 * (c + 4 * i), wide);
+            }
+        float* scale = a.c.ks + unit * KV8_PARTS + part, ratio;
+        const float before = held && g < a.c.kv_heads ? *scale : 0.f;
+        if (half) {
+            for (int i = (int)threadIdx.x; i < (s.hi - s.lo) * half; i += 256) {
+                const int u = s.lo + i / half, p = i % half;
+                kv8_angle(s.pos + u, a.c.freq[p], angle[(u * half + p) * 2], angle[(u * half + p) * 2 + 1]);
+            }
+            __syncthreads();
+        }
         unsigned bits = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (i < n && fresh) {
-                x[i] = kv8_rotated4(row, 4 * (c + 4 * i), s.pos + t, a.c.rot, a.c.halves, a.c.freq, wide);
+                x[i] = kv8_turned4(a.c, x[i], y[i], 4 * (c + 4 * i), angle + t * 2 * half);
                 bits = max(bits, kv8_bits(x[i]));
             }
-        float* scale = a.c.ks + unit * KV8_PARTS + part, ratio;
-        const float before = held ? *scale : 0.f;
         bits = mmi_wave_max_u32(bits);
+        if (g >= a.c.kv_heads) return;
         const float after = kv8_grown<E4M3>(before, held, bits, ratio), inv = 1.f / after;
         const bool bad = !(after == after);
         if (fresh) {
@@ -231,8 +248,9 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_append(TlmKv8Append a) {
         }
         if (lane == 0) *scale = after;
     } else {
+        if (g >= a.c.kv_heads) return;
         const int n = (a.c.vdim + 63) / 64;
-        const In* v = (const In*)a.v + (long)s.row * a.v_row + g * a.v_head;
+        const In* v = (const In*)a.v + (long)s.row * a.v_row + (long)g * a.v_head;
         float x[4][KV8_BLOCK];
         unsigned bits = 0;
 #pragma unroll
@@ -331,7 +349,7 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
 // it by 2^7.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both operands come in two parts, 22 bits, good to 2^-24.
 // (bf16 operands left 1.8 times the error of the result's rounding.)  Sums, maxima and the denominator, which has the weights before they were
 // rounded, are fp32.
-constexpr int KV8_FEW = 64;              // sequences with up to so many columns go to k_tlm_kv8_attn where a call may bring longer ones
+constexpr int KV8_FEW = 16;              // sequences with up to so many columns, one tile, are the few's where a call may bring longer ones
 constexpr float KV8_UP = 8.f, KV8_SLACK = 7.f;      // log2: of what weights are carried times, of what they may outgrow it by (fp16 ends at 2^16)
 constexpr int KV8_ANGLES = 2048;         // pairs of a cosine and a sine in LDS
 
@@ -438,33 +456,19 @@ __device__ __forceinline__ float kv8_raise(float amax, float& back) {
     back = __builtin_bit_cast(float, (unsigned)(min(e, 127) - 14 + 127) << 23);
     return __builtin_bit_cast(float, (unsigned)(14 - min(e, 127) + 127) << 23);
 }
-// dimensions d .. d + 3 of a query row, rotated (cs: its position's angles)
+// a lane's 8 dimensions of a query row, and their rotation partners where these lie half of the dimensions apart
+struct Kv8Raw { f32x4 x[2], y[2]; };
 template <class In>
-__device__ __forceinline__ f32x4 kv8_query4(const TlmKv8Attn& a, const In* row, int d, const float* cs) {
+__device__ __forceinline__ Kv8Raw kv8_raw(const TlmKv8Attn& a, const In* row, int d) {
     const bool wide = a.wide != 0;
-    f32x4 x = kv8_in4(row + d, wide);
-    const int rot = a.c.rot, half = rot / 2;
-    if (d >= rot) return x;
-    if (a.c.halves) {
-        const bool first = d < half;
-        const f32x4 y = kv8_in4(row + (first ? d + half : d - half), wide);
-        cs += 2 * (first ? d : d - half);
+    Kv8Raw o;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float re, im;
-            mmi_rope_rotate(first ? x[r] : y[r], first ? y[r] : x[r], cs[2 * r], cs[2 * r + 1], re, im);
-            x[r] = first ? re : im;
-        }
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-            float re, im;
-            mmi_rope_rotate(x[r], x[r + 1], cs[d + r], cs[d + r + 1], re, im);
-            x[r] = re;
-            x[r + 1] = im;
-        }
+    for (int h = 0; h < 2; ++h) {
+        const int e = d + 4 * h;
+        o.x[h] = e < a.c.dim ? kv8_in4(row + e, wide) : f32x4{0.f, 0.f, 0.f, 0.f};
+        o.y[h] = kv8_partners4(a.c, row, e, wide);
     }
-    return x;
+    return o;
 }
 // The group's queries into LDS as operand fragments, by the whole workgroup: D / 8 lanes a column, and a token's angles formed once for all
 // heads (a portion of the tokens at a time).  put(column, 8 dimensions d / 8 .., part): where they go; back: the columns' inverse factors.
@@ -480,26 +484,36 @@ __device__ __forceinline__ void kv8_queries(const TlmKv8Attn& a, const Kv8Cols& 
             for (int i = tid; i < nt * half; i += 256) kv8_angle(c.s.pos0 + t0 + i / half, a.c.freq[i % half], angle[2 * i], angle[2 * i + 1]);
             __syncthreads();
         }
-        for (int n = n0; n < n1; n += AT) {                // (every lane goes along: the maximum is taken across them)
-            const int k = min(n + tid / G, n1 - 1), col = c.c0 + k, tok = col / a.rep, d = 8 * (tid % G);
-            const In* row = (const In*)a.x + (long)(c.s.row0 + tok) * a.x_row + (g * a.rep + col - tok * a.rep) * a.x_head;
-            float x[8], top = 0.f;
+        // four rounds of columns are asked for at once; every lane goes along, the maximum is taken across them
+        for (int nb = n0; nb < n1; nb += 4 * AT) {
+            Kv8Raw raw[4];
 #pragma unroll
-            for (int h = 0; h < 8; h += 4) {
-                const f32x4 v = d < a.c.dim ? kv8_query4(a, row, d + h, angle + (tok - t0) * 2 * half) : f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < 4; ++u) {
+                const int col = c.c0 + min(nb + u * AT + tid / G, n1 - 1), tok = col / a.rep;
+                if (nb + u * AT < n1) raw[u] = kv8_raw(a, (const In*)a.x + (long)(c.s.row0 + tok) * a.x_row + (g * a.rep + col - tok * a.rep) * a.x_head, 8 * (tid % G));
+            }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[h + r] = v[r];
-                    top = fmaxf(top, fabsf(v[r]));
+            for (int u = 0; u < 4; ++u) {
+                if (nb + u * AT >= n1) break;
+                const int n = nb + u * AT + tid / G, k = min(n, n1 - 1), tok = (c.c0 + k) / a.rep, d = 8 * (tid % G);
+                float x[8], top = 0.f, b;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 v = kv8_turned4(a.c, raw[u].x[h], raw[u].y[h], d + 4 * h, angle + (tok - t0) * 2 * half);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[4 * h + r] = v[r];
+                        top = fmaxf(top, fabsf(v[r]));
+                    }
+                }
+                u32x4 q[NS];
+                kv8_split8<NS>(x, kv8_raise(mmi_group_max<G>(top), b), q);
+                if (n < n1) {
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) *put(k, tid % G, s) = q[s];
+                    if (tid % G == 0) back[k] = b;
                 }
             }
-            u32x4 q[NS];
-            float b;
-            kv8_split8<NS>(x, kv8_raise(mmi_group_max<G>(top), b), q);
-            if (n + tid / G >= n1) continue;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) *put(k, tid % G, s) = q[s];
-            if (tid % G == 0) back[k] = b;
         }
     }
     __syncthreads();
@@ -689,6 +703,7 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         a.few.pml[part * 32 + 16 + bl] = L;
     }
 }
+// grid: slots of tiles, kv heads, splits
 template <class In, class Tr, int NS, int D, bool E4M3>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8Attn a) {
     MMI_SHARED __attribute__((aligned(16))) f32x4 ob[KV8_LDS];
@@ -706,7 +721,7 @@ template <int NS, int D>
 struct Kv8Tile {
     static constexpr int QT = 1, PER = 128 * QT, KS = D / 16, DT = D / 32;
     static constexpr int KF = KS * 64, VF = DT * 2 * 64;                       // vectors per buffer
-    static constexpr size_t smem() { return std::max((size_t)2 * (KF + VF) * 16, (size_t)PER * D * NS * 2 + PER * 4 + KV8_ANGLES * 8); }
+    static constexpr size_t smem() { return std::max({(size_t)2 * (KF + VF) * 16, (size_t)PER * D * NS * 2 + PER * 4 + KV8_ANGLES * 8, (size_t)KV8_LDS * 16}); }
 };
 template <class In, class Tr, int NS, int D, bool E4M3>
 __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, int slot, int g, int split) {
@@ -730,27 +745,8 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         tok[t] = col / a.rep;
         head[t] = g * a.rep + col - tok[t] * a.rep;
     }
-    u32x4 q[QT][KS][NS];                                   // dimensions 16 s + 8 hi ..
-    float back[QT];
-    {
-        float* turned = reinterpret_cast<float*>(lds + Z::PER * D * NS / 8);      // inverse factors, then angles
-        kv8_queries<In, NS, D>(a, c, Z::PER, g, turned + Z::PER, turned, [&](int n, int k, int p) __attribute__((always_inline)) {
-            return lds + (((n >> 5) * KS + (k >> 1)) * NS + p) * 64 + 32 * (k & 1) + (n & 31);
-        });
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-#pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int p = 0; p < NS; ++p) q[t][j][p] = lds[(((wave * QT + t) * KS + j) * NS + p) * 64 + lane];
-            back[t] = turned[(wave * QT + t) * 32 + cl] * a.mask.scale;
-        }
-        __syncthreads();                                   // (their memory takes keys and values)
-    }
     // ---- codes -> LDS
     u32x4 *kb = lds, *vb = lds + 2 * Z::KF;
-    for (int i = tid; i < 2 * Z::KF; i += 256)
-        if ((i % Z::KF) / 64 >= a.c.dim / 16) kb[i] = u32x4{0u, 0u, 0u, 0u};      // (dimensions past the head's)
     u32x4 kr[KU], vr[KU];
     int kput[KU], vput[KU];
     bool kon[KU], von[KU];
@@ -784,6 +780,30 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         for (int u = 0; u < KU; ++u)
             if (von[u]) vr[u] = *(const u32x4*)(p + ((tid + 256 * u) >> 1) * TLM_PAGE + 16 * (tid & 1));
     };
+    At z0, z1, z2;                                         // steps i, i + 1, i + 2
+    if (i0 < i1) {
+        z0 = find(i0);
+        load_k(z0);
+    }
+    u32x4 q[QT][KS][NS];                                   // dimensions 16 s + 8 hi ..
+    float back[QT];
+    {
+        float* turned = reinterpret_cast<float*>(lds + Z::PER * D * NS / 8);      // inverse factors, then angles
+        kv8_queries<In, NS, D>(a, c, Z::PER, g, turned + Z::PER, turned, [&](int n, int k, int p) __attribute__((always_inline)) {
+            return lds + (((n >> 5) * KS + (k >> 1)) * NS + p) * 64 + 32 * (k & 1) + (n & 31);
+        });
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int p = 0; p < NS; ++p) q[t][j][p] = lds[(((wave * QT + t) * KS + j) * NS + p) * 64 + lane];
+            back[t] = turned[(wave * QT + t) * 32 + cl] * a.mask.scale;
+        }
+        __syncthreads();                                   // (their memory takes keys and values)
+    }
+    for (int i = tid; i < 2 * Z::KF; i += 256)
+        if ((i % Z::KF) / 64 >= a.c.dim / 16) kb[i] = u32x4{0u, 0u, 0u, 0u};      // (dimensions past the head's)
     auto put_k = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
@@ -850,7 +870,6 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         }
     };
     const int vl = lane ^ (4 * hi);
-    At z0, z1, z2;                                         // steps i, i + 1, i + 2
     auto step = [&](int i, int set) __attribute__((always_inline)) {      // scores of step i in `set`, keys of step i + 1 in LDS, of step i + 2 in registers
         const int key0 = z0.key0;
         const bool now = z0.have;
@@ -926,8 +945,6 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         __syncthreads();
     };
     if (i0 < i1) {                                         // (step i0 is set 0: splits hold whole pages)
-        z0 = find(i0);
-        load_k(z0);
         put_k(0);
         z1 = find(i0 + 1);
         load_k(z1);
@@ -969,49 +986,77 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         }
     }
 }
-// grid: kv heads x group slots (a head's groups on one XCD, the last groups, which see most keys, first), splits
+// Calls that may bring sequences of either kind: both in one launch, they share nothing.  grid: the many's kv heads x group slots (a head's groups
+// on one XCD; the last groups, which see most keys, first) x splits, then the few's kv heads x slots x splits
 template <class In, class Tr, int NS, int D, bool E4M3>
-__global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(TlmKv8Attn a) {
+__global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(TlmKv8Attn a, int many, int few_slots) {
     MMI_DYN_SHARED(u32x4, lds);
-    const int b = (int)(gridDim.x - 1 - blockIdx.x);
-    tlm_kv8_tile<In, Tr, NS, D, E4M3>(a, lds, b / a.c.kv_heads, a.c.kv_heads - 1 - b % a.c.kv_heads, (int)blockIdx.y);
+    MMI_SHARED float ml[2][4][16];
+    const int G = a.c.kv_heads;
+    int b = (int)blockIdx.x;
+    if (b < many) {
+        const int slots = many / (G * a.many.nsplit), split = b / (G * slots);
+        b -= split * G * slots;
+        tlm_kv8_tile<In, Tr, NS, D, E4M3>(a, lds, slots - 1 - b / G, b % G, split);
+    } else {
+        b -= many;
+        tlm_kv8_attn<In, Tr, NS, D, E4M3>(a, reinterpret_cast<f32x4*>(lds), ml, b / G % few_slots, b % G, b / (G * few_slots));
+    }
 }
 
 // The splits of one column -> output.  grid: columns of all slots (first the few's, then the many's), kv heads.
-// Up to 16 splits (WIDE false): a wave per column, a lane per split, then four dimensions a lane, all partial sums asked for at once.  More:
-// a workgroup per column, 16 groups of lanes take every 16th split, and their sums meet in LDS.
+// Up to 16 splits (WIDE false): a wave for every 64 / (vdim / 4) columns, four dimensions a lane, all partial sums asked for at once.  More: a
+// workgroup per column, 16 groups of lanes take every 16th split, and their sums meet in LDS.
+MMI_HD int kv8_joined(int cols, int vdim, bool wide) { return wide ? cols : (cols + 256 / vdim - 1) / (256 / vdim); }      // waves (wide: workgroups) per slot
 template <class Tr, bool WIDE>
-__global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first_many, int columns) {
+__global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first_many, int all) {
     const int tid = (int)threadIdx.x, wave = mmi_uniform(tid >> 6), at = WIDE ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
-    if (at >= columns) return;
+    if (at >= all) return;
     const bool few = at < first_many;
     const Kv8Share& h = few ? a.few : a.many;
-    const int b = at - (few ? 0 : first_many), slot = b / h.cols, n = b - slot * h.cols, per = h.z.per;
-    const Kv8Cols c(a, h, few, slot);
-    const int g = (int)blockIdx.y, col = c.c0 + n;
-    if (col >= c.ncol) return;
-    const int ns = max(1, (c.n + h.pages - 1) / h.pages);      // (at most 16, 256)
+    const int b = at - (few ? 0 : first_many), each = kv8_joined(h.cols, a.c.vdim, WIDE), slot = b / each, per = h.z.per, g = (int)blockIdx.y;
     const long part = ((long)slot * a.c.kv_heads + g) * h.nsplit;
-    const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
     if constexpr (!WIDE) {
-        const int lane = tid & 63, s = min(lane & 15, ns - 1), d = 4 * min(lane, a.c.vdim / 4 - 1);
-        const float m = h.pml[(part + s) * 2 * per + n], l = (lane & 15) < ns ? h.pml[(part + s) * 2 * per + per + n] : 0.f;
+        const int lane = tid & 63, G = a.c.vdim / 4, at_once = 64 / G, n = (b - slot * each) * at_once + lane / G, d = 4 * (lane % G);
+        const bool on = lane / G < at_once && n < h.cols;
+        // (asked for before it is known how many splits there were)
+        const long p = part * per + (on ? n : 0);
+        float m[16], l[16];
         f32x4 v[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-            if (k < ns) v[k] = *(const f32x4*)(h.po + ((part + k) * per + n) * a.c.vdim + d);
-        const float M = mmi_group_max<16>(m), w = exp2f(m - (M == -INFINITY ? 0.f : M));
-        const float inv = kv8_inverse(mmi_row_sum(l * w), M, a.sink);
+            if (k < h.nsplit) {
+                const float* ml = h.pml + (part + k) * 2 * per + (on ? n : 0);
+                m[k] = ml[0];
+                l[k] = ml[per];
+                v[k] = *(const f32x4*)(h.po + (p + (long)k * per) * a.c.vdim + d);
+            }
+        const Kv8Cols c(a, h, few, slot);
+        const int col = c.c0 + n, ns = max(1, (c.n + h.pages - 1) / h.pages);
+        if (!on || col >= c.ncol) return;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (k < ns) M = fmaxf(M, m[k]);
+        const float Ms = M == -INFINITY ? 0.f : M;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float wk = mmi_shfl(w, k);
-            if (k < ns) o += v[k] * wk;
-        }
-        if (4 * lane < a.c.vdim) kv8_store<Tr>(a, c.s.row0 + tok, head, d, o * inv);
+        for (int k = 0; k < 16; ++k)
+            if (k < ns) {
+                const float w = exp2f(m[k] - Ms);
+                L += l[k] * w;
+                o += v[k] * w;
+            }
+        const int tok = col / a.rep;
+        kv8_store<Tr>(a, c.s.row0 + tok, g * a.rep + col - tok * a.rep, d, o * kv8_inverse(L, M, a.sink));
     } else {
         MMI_SHARED float wt[256], red[4][2];
         MMI_SHARED __attribute__((aligned(16))) f32x4 sum[256];
+        const int n = b - slot * each;
+        const Kv8Cols c(a, h, few, slot);
+        const int col = c.c0 + n, ns = max(1, (c.n + h.pages - 1) / h.pages);      // (at most 256)
+        if (col >= c.ncol) return;
+        const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
         float m = -INFINITY, l = 0.f;
         if (tid < ns) {
             m = h.pml[(part + tid) * 2 * per + n];

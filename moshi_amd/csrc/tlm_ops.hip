@@ -63,13 +63,16 @@ int launch_attn(hipStream_t s, const TlmKv8Attn& a) {
             static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             MMI_HIP_CHECK(attr);
         }
-        MMI_LAUNCH((k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), dim3((unsigned)kv8_slots(a.q, a.many.z) * a.c.kv_heads, a.many.nsplit), 256, smem, s, a);
+        const int slots = (int)kv8_slots(a.q, a.few.z), many = (int)kv8_slots(a.q, a.many.z) * a.c.kv_heads * a.many.nsplit;
+        MMI_LAUNCH((k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), (unsigned)many + (unsigned)slots * a.c.kv_heads * a.few.nsplit, 256, smem, s, a, many, slots);
+    } else {
+        MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, E4M3>), dim3((unsigned)kv8_slots(a.q, a.few.z), a.c.kv_heads, a.few.nsplit), 256, 0, s, a);
     }
-    MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, E4M3>), dim3((unsigned)kv8_slots(a.q, a.few.z), a.c.kv_heads, a.few.nsplit), 256, 0, s, a);
-    const int few = a.few.nsplit > 1 ? (int)kv8_slots(a.q, a.few.z) * a.few.cols : 0, all = few + (a.both && a.many.nsplit > 1 ? (int)kv8_slots(a.q, a.many.z) * a.many.cols : 0);
-    if (!all) {}
-    else if (std::max(a.few.nsplit, a.both ? a.many.nsplit : 1) <= 16) MMI_LAUNCH((k_tlm_kv8_combine<Tr, false>), dim3(mmi_cdiv(all, 4), a.c.kv_heads), 256, 0, s, a, few, all);
-    else MMI_LAUNCH((k_tlm_kv8_combine<Tr, true>), dim3(all, a.c.kv_heads), 256, 0, s, a, few, all);
+    const bool wide = std::max(a.few.nsplit, a.both ? a.many.nsplit : 1) > 16;
+    auto joined = [&](const Kv8Share& h) { return h.nsplit > 1 ? (int)kv8_slots(a.q, h.z) * kv8_joined(h.cols, a.c.vdim, wide) : 0; };
+    const int few = joined(a.few), all = few + (a.both ? joined(a.many) : 0);
+    if (all && wide) MMI_LAUNCH((k_tlm_kv8_combine<Tr, true>), dim3(all, a.c.kv_heads), 256, 0, s, a, few, all);
+    else if (all) MMI_LAUNCH((k_tlm_kv8_combine<Tr, false>), dim3(mmi_cdiv(all, 4), a.c.kv_heads), 256, 0, s, a, few, all);
     MMI_CHECK_LAUNCH();
     return MMI_OK;
 }
@@ -98,10 +101,10 @@ size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, long
 
 int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype) {
     a.z = kv8_cut(a.q, 1, KV8_BLOCK, 2);               // (a portion of n rows touches at most (n + 14) / 16 + 1 blocks)
-    const dim3 grid((unsigned)kv8_slots(a.q, a.z), a.c.kv_heads, 2);
+    const dim3 grid((unsigned)kv8_slots(a.q, a.z), mmi_cdiv(a.c.kv_heads, 4), 2);
     return by_codes(a.c.e4m3, [&](auto e) {
-        if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_kv8_append<float, decltype(e)::value>), grid, 64, 0, s, a);
-        else MMI_LAUNCH((k_tlm_kv8_append<uint16_t, decltype(e)::value>), grid, 64, 0, s, a);
+        if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_kv8_append<float, decltype(e)::value>), grid, 256, 0, s, a);
+        else MMI_LAUNCH((k_tlm_kv8_append<uint16_t, decltype(e)::value>), grid, 256, 0, s, a);
         MMI_CHECK_LAUNCH();
         return (int)MMI_OK;
     });
@@ -225,7 +228,7 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
 namespace {
 struct BeamSpace { size_t m, s, x, i, total; };            // where the parts of the workspace begin, in bytes
 BeamSpace beam_space(int rows, int beams, int vocab) {
-    const size_t lists = (size_t)rows * ((vocab - 1) / BEAM_CHUNK + 1);
+    const size_t lists = (size_t)rows * mmi_cdiv(vocab, BEAM_CHUNK);
     BeamSpace z;
     z.s = 0;
     z.m = lists * sizeof(double);
@@ -238,16 +241,6 @@ int check_beams(int64_t batch, int32_t beams, int32_t vocab, const char* at) {
     if (batch < 0 || beams < 1 || vocab < 1) return mmi_fail(MMI_ERR_INVALID, std::string(at) + ": bad sizes");
     if (beams > BEAM_MAX) return mmi_fail(MMI_ERR_UNSUPPORTED, std::string(at) + ": at most 32 beams");
     if (batch * beams > 65535 || vocab > 1 << 20) return mmi_fail(MMI_ERR_SHAPE, std::string(at) + ": at most 65535 beams of all requests and 2^20 tokens");
-    return MMI_OK;
-}
-template <class U>
-int launch_reorder(hipStream_t s, const TlmReorder& a, unsigned blocks, int groups) {
-    const dim3 grid(blocks, (unsigned)groups);
-    if (a.beams <= 4) MMI_LAUNCH((k_tlm_reorder<U, 4>), grid, 256, 0, s, a);
-    else if (a.beams <= 8) MMI_LAUNCH((k_tlm_reorder<U, 8>), grid, 256, 0, s, a);
-    else if (a.beams <= 16) MMI_LAUNCH((k_tlm_reorder<U, 16>), grid, 256, 0, s, a);
-    else MMI_LAUNCH((k_tlm_reorder<U, 32>), grid, 256, 0, s, a);
-    MMI_CHECK_LAUNCH();
     return MMI_OK;
 }
 }  // namespace
@@ -275,7 +268,7 @@ extern "C" int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int3
     a.ld = row;
     a.V = vocab;
     a.beams = beams;
-    a.splits = mmi_cdiv(vocab, BEAM_CHUNK);
+    a.chunks = mmi_cdiv(vocab, BEAM_CHUNK);
     a.score = score;
     a.length = length;
     a.done = finished;
@@ -291,37 +284,42 @@ extern "C" int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int3
     a.out_done = out_finished;
     a.out_length = out_length;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_beam_rows<float>), dim3(a.splits, batch * beams), 256, 0, s, a);
-    else MMI_LAUNCH((k_tlm_beam_rows<uint16_t>), dim3(a.splits, batch * beams), 256, 0, s, a);
+    if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_beam_rows<float>), dim3(mmi_cdiv(a.chunks, 4), batch * beams), 256, 0, s, a);
+    else MMI_LAUNCH((k_tlm_beam_rows<uint16_t>), dim3(mmi_cdiv(a.chunks, 4), batch * beams), 256, 0, s, a);
     MMI_CHECK_LAUNCH();
-    MMI_LAUNCH(k_tlm_beam_pick, batch, 64, (size_t)beams * a.splits * sizeof(int), s, a);
+    MMI_LAUNCH(k_tlm_beam_pick, batch, 256, 0, s, a);
     MMI_CHECK_LAUNCH();
     return MMI_OK;
 }
 
 int tlm_reorder(hipStream_t s, int n, const TlmReorderTensor* tensors, int groups, int beams, const int* parent, const int* row) {
-    // units of 16 bytes, of 4, of one: what every base, stride and row length is a multiple of
-    for (const int unit : {16, 4, 1})
-        for (int i = 0; i < n;) {
-            TlmReorder a;
-            memset(&a, 0, sizeof(a));
-            a.beams = beams;
-            a.parent = parent;
-            a.row = row;
-            unsigned blocks = 0;
-            for (; i < n && a.n < BEAM_TENSORS; ++i) {
-                const TlmReorderTensor& t = tensors[i];
-                const uintptr_t all = (uintptr_t)t.p | (uintptr_t)t.stride | (uintptr_t)t.bytes;
-                if (t.bytes == 0 || (all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1)) != unit) continue;
-                const long units = t.bytes / unit;
-                if (units > 0x7fffffffl) return mmi_fail(MMI_ERR_SHAPE, "reorder: a row is too long");
-                a.t[a.n++] = TlmReorder::T{(char*)t.p, (long)t.stride, (unsigned)units, blocks};
-                blocks += (unsigned)mmi_cdiv64(units, 256);
-            }
-            if (!a.n) continue;
-            const int rc = unit == 16 ? launch_reorder<u32x4>(s, a, blocks, groups) : (unit == 4 ? launch_reorder<uint32_t>(s, a, blocks, groups) : launch_reorder<uint8_t>(s, a, blocks, groups));
-            if (rc) return rc;
+    for (int i = 0; i < n;) {
+        TlmReorder a;
+        memset(&a, 0, sizeof(a));
+        a.beams = beams;
+        a.parent = parent;
+        a.row = row;
+        unsigned blocks = 0;
+        for (; i < n && a.n < BEAM_TENSORS; ++i) {
+            const TlmReorderTensor& t = tensors[i];
+            const uintptr_t all = (uintptr_t)t.p | (uintptr_t)t.stride | (uintptr_t)t.bytes;
+            const int unit = all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
+            const long units = t.bytes / unit;
+            if (units > 0x3fffffffl) return mmi_fail(MMI_ERR_SHAPE, "reorder: a row is too long");
+            if (!units) continue;
+            const unsigned more = (unsigned)mmi_cdiv64(units, 256);
+            if (blocks + more > 0x7fffffu) break;          // (2^31 lanes a launch)
+            a.t[a.n++] = TlmReorder::T{(char*)t.p, (long)t.stride, (unsigned)units, blocks, unit};
+            blocks += more;
         }
+        if (!a.n) continue;
+        const dim3 grid(blocks, (unsigned)groups);
+        if (beams <= 4) MMI_LAUNCH((k_tlm_reorder<4>), grid, 256, 0, s, a);
+        else if (beams <= 8) MMI_LAUNCH((k_tlm_reorder<8>), grid, 256, 0, s, a);
+        else if (beams <= 16) MMI_LAUNCH((k_tlm_reorder<16>), grid, 256, 0, s, a);
+        else MMI_LAUNCH((k_tlm_reorder<32>), grid, 256, 0, s, a);
+        MMI_CHECK_LAUNCH();
+    }
     return MMI_OK;
 }
 

@@ -66,7 +66,10 @@ class PagedKVCache:
             self._freq = torch.tensor(turns, dtype=torch.float64, device=self.device)
         self._desc = _capi.KVCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages, self.kv_heads, self.dim, self.vdim, _CODES[k.dtype],
                                        self.rot_dim, int(self.rot_halves), self._freq.data_ptr() if rot_dim else None)
-        self._lib.check(min(0, self._workspace(_capi.KVSeqs(), _capi.MMI_BF16, self.kv_heads, 0, 0)))      # (sizes that the kernels do not take are refused here)
+        self._on = _capi.LaunchOn(self.device)
+        self._where = k.get_device()
+        self._need = {}
+        self._workspace(_capi.KVSeqs(), (0, 0, 0, _capi.MMI_BF16, self.kv_heads, 0, 0, True))      # (sizes that the kernels do not take are refused here)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, dim: int, vdim: Optional[int] = None, codes: str = "int8", device: torch.device | str = "cuda", **rotation) -> "PagedKVCache":
@@ -81,58 +84,68 @@ class PagedKVCache:
 
     # ---- arguments --------------------------------------------------------------------------------------------------
     def _seqs(self, table: torch.Tensor, positions: torch.Tensor, rows: Optional[torch.Tensor], total: int) -> _capi.KVSeqs:
-        n = positions.shape[0]
-        if positions.dim() != 1 or table.dim() != 2 or table.shape[0] != n or (rows is not None and rows.shape != (n + 1,)):
+        where, (n, *more), shape = self._where, positions.shape, table.shape
+        if more or len(shape) != 2 or shape[0] != n or (rows is not None and rows.shape != (n + 1,)):
             raise AssertionError("table is [sequences, pages], positions [sequences], rows [sequences + 1]")
         for t in (table, positions) if rows is None else (table, positions, rows):
-            if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+            if t.dtype is not torch.int32 or t.get_device() != where or not t.is_contiguous():
                 raise ValueError("table, positions and rows are contiguous int32 tensors on the cache's device")
         if rows is None and total != n:
             raise AssertionError(f"{total} rows for {n} sequences: without `rows` every sequence brings one")
-        return _capi.KVSeqs(n, total, None if rows is None else rows.data_ptr(), positions.data_ptr(), table.data_ptr(), table.shape[1])
+        return _capi.KVSeqs(n, total, None if rows is None else rows.data_ptr(), positions.data_ptr(), table.data_ptr(), shape[1])
 
     def _rows(self, t: torch.Tensor, name: str, heads: Optional[int], dim: int):
-        if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        """Heads and type of a tensor of rows, and its address and strides."""
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
             raise AssertionError(f"{name} is [rows, {'heads' if heads is None else heads}, {dim}]")
-        if t.dtype not in _DTYPES or t.device != self.device:
+        dtype = _DTYPES.get(t.dtype)
+        if dtype is None or t.get_device() != self._where:
             raise ValueError(f"{name} is bf16 or fp32, on the cache's device")
-        if t.stride(2) != 1 and t.numel():
+        if stride[2] != 1 and t.numel():
             raise ValueError(f"a head's dimensions lie side by side in {name}")
-        return t.data_ptr(), t.stride(0), t.stride(1)
+        return shape[1], dtype, (t.data_ptr(), stride[0], stride[1])
 
-    def _workspace(self, seqs: _capi.KVSeqs, dtype: int, heads: int, window: int, keep_first: int) -> int:
-        return self._lib.mmi_kv_attend_workspace(C.byref(self._desc), C.byref(seqs), dtype, heads, window, keep_first)
+    def _workspace(self, seqs: _capi.KVSeqs, key) -> int:
+        """Bytes that an attention of these sizes (sequences, rows, pages of a sequence, type, heads, window, first tokens, one row each?) works in."""
+        need = self._need.get(key)
+        if need is None:
+            need = self._lib.mmi_kv_attend_workspace(C.byref(self._desc), C.byref(seqs), *key[3:7])
+            self._lib.check(min(0, need))
+            if len(self._need) > 4096:
+                self._need.clear()
+            self._need[key] = need
+        return need
 
     # ---- computation -------------------------------------------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
         """Write the rows' keys [rows, kv_heads, dim] (rotated on the way) and values [rows, kv_heads, vdim], bf16 or fp32, to their pages.
         The pages that two sequences of a call write to are different ones."""
-        if k.shape[:2] != v.shape[:2] or k.dtype != v.dtype:
-            raise AssertionError("keys and values come in the same number and type")
         seqs = self._seqs(table, positions, rows, k.shape[0])
-        kp, vp = self._rows(k, "k", self.kv_heads, self.dim), self._rows(v, "v", self.kv_heads, self.vdim)
-        with _capi.device_scope(self.device):
-            self._lib.check(self._lib.mmi_kv_append(C.byref(self._desc), C.byref(seqs), _DTYPES[k.dtype], *kp, *vp, _capi.stream_ptr(self.device)))
+        (_, dtype, kp), (_, vtype, vp) = self._rows(k, "k", self.kv_heads, self.dim), self._rows(v, "v", self.kv_heads, self.vdim)
+        if dtype != vtype or v.shape[0] != seqs.rows:
+            raise AssertionError("keys and values come in the same number and type")
+        self._lib.check(self._on.call(self._lib.mmi_kv_append, C.byref(self._desc), C.byref(seqs), dtype, *kp, *vp))
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, rows: Optional[torch.Tensor] = None, scale: Optional[float] = None, window: int = 0,
                keep_first: int = 0, sink: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of queries [rows, heads, dim] over the positions up to their own, those rows' keys having been appended: [rows, heads, vdim]
         in the queries' type.  scale: default dim ** -0.5.  window > 0: the last `window` positions and the first `keep_first`.  sink: one is
         added to the softmax's denominator.  Rows that see nothing are zeros; rows behind the last sequence are left as they were."""
-        qp = self._rows(q, "q", None, self.dim)
-        total, heads = q.shape[:2]
+        heads, dtype, qp = self._rows(q, "q", None, self.dim)
+        total = q.shape[0]
         seqs = self._seqs(table, positions, rows, total)
         if out is None:
             out = torch.empty((total, heads, self.vdim), dtype=q.dtype, device=self.device)
-        elif out.shape != (total, heads, self.vdim) or out.dtype != q.dtype:
-            raise AssertionError("out is [rows, heads, vdim] in the queries' type")
-        op = self._rows(out, "out", heads, self.vdim)
-        with _capi.device_scope(self.device):
-            need = self._workspace(seqs, _DTYPES[q.dtype], heads, window, keep_first)
-            self._lib.check(min(0, need))
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            self._lib.check(self._lib.mmi_kv_attend(C.byref(self._desc), C.byref(seqs), _DTYPES[q.dtype], heads, *qp, *op, self.dim ** -0.5 if scale is None else scale, window,
-                                                    keep_first, int(sink), work.data_ptr() if need else None, need, _capi.stream_ptr(self.device)))
+            op = (out.data_ptr(), heads * self.vdim, self.vdim)
+        else:
+            if out.shape != (total, heads, self.vdim) or out.dtype != q.dtype:
+                raise AssertionError("out is [rows, heads, vdim] in the queries' type")
+            op = self._rows(out, "out", heads, self.vdim)[2]
+        need = self._workspace(seqs, (seqs.n, total, seqs.table_ld, dtype, heads, window, keep_first, rows is None))
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._lib.check(self._on.call(self._lib.mmi_kv_attend, C.byref(self._desc), C.byref(seqs), dtype, heads, *qp, *op, self.dim ** -0.5 if scale is None else scale, window,
+                                      keep_first, sink, work.data_ptr() if need else None, need))
         return out
 
     def read(self, table: torch.Tensor, positions: torch.Tensor, rows: Optional[torch.Tensor] = None, tokens: Optional[int] = None,
@@ -147,6 +160,5 @@ class PagedKVCache:
         seqs = self._seqs(table, positions, rows, total)
         k = torch.empty((total, self.kv_heads, self.dim), dtype=dtype, device=self.device)
         v = torch.empty((total, self.kv_heads, self.vdim), dtype=dtype, device=self.device)
-        with _capi.device_scope(self.device):
-            self._lib.check(self._lib.mmi_kv_read(C.byref(self._desc), C.byref(seqs), _DTYPES[dtype], k.data_ptr(), v.data_ptr(), _capi.stream_ptr(self.device)))
+        self._lib.check(self._on.call(self._lib.mmi_kv_read, C.byref(self._desc), C.byref(seqs), _DTYPES[dtype], k.data_ptr(), v.data_ptr()))
         return k, v

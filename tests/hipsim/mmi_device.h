@@ -510,6 +510,9 @@ inline int mmi_uniform(int v) { return v; }
 inline int mmi_from_lane(int v, int l) { return mmi_shfl(v, l); }
 inline int mmi_load_const(const int* p) { return *p; }
 inline bool mmi_any(bool v) { unsigned x = v ? 1u : 0u; for (int m = 1; m < 64; m <<= 1) { const unsigned o = mmi_shfl_xor(x, m); x = o > x ? o : x; } return x != 0; }
+inline void mmi_wave_sync() { hipsim::sync_wave(); }
+inline uint64_t mmi_ballot(bool v) { uint64_t x = v ? 1ull << hipsim::lane_id() : 0; for (int m = 1; m < 64; m <<= 1) x |= mmi_shfl_xor(x, m); return x; }
+inline int mmi_below(uint64_t m) { return __builtin_popcountll(m & ((1ull << hipsim::lane_id()) - 1)); }
 inline void mmi_load_lds(const void* base, unsigned off, u32x4* lds, int at) { lds[at + (int)(threadIdx.x & 63)] = *(const u32x4*)((const char*)base + off); }
 inline void mmi_load_lds(const u32x4* from, u32x4* lds, int at) { lds[at + (int)(threadIdx.x & 63)] = *from; }
 template <int N>
