@@ -64,6 +64,7 @@ typedef struct mmi_tlm_cfg {
     int64_t bigram_mul_prev, bigram_mul_cur;
     int32_t max_positions;                        /* 0: no learned positions; otherwise also the longest sequence */
     int32_t dtype;                                /* MMI_BF16 or MMI_F32: operands of the matrix products, activations and cache */
+    int32_t cache;                                /* keys and values of MMI_TLM_MIX_ATTENTION layers: 0 like the operands, MMI_I8 or MMI_F8E4M3: in 8 bits */
 } mmi_tlm_cfg;
 
 typedef struct mmi_tlm mmi_tlm;
@@ -142,7 +143,7 @@ int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtyp
  * sink: one is added to the softmax's denominator.  Query head h reads key/value head h / (heads / kv_heads).  Sums are
  * fp32; bf16 queries and the weights beside them are fp16 operands, fp32 ones two fp16 parts each (22 bits).  A row that sees nothing gets zeros.  workspace: device memory of mmi_kv_attend_workspace bytes (a negative
  * status in its place where the arguments are refused), one per call in flight. */
-int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, int32_t window, int32_t keep_first);
+int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first);
 int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
                   int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t sink, void* workspace, int64_t workspace_bytes,
                   mmi_stream stream);

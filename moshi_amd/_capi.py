@@ -92,7 +92,7 @@ class TLMCfg(C.Structure):
                 ("loop_start", C.c_int32), ("loop_stop", C.c_int32), ("loop_times", C.c_int32), ("norm_groups", C.c_int32),
                 ("norm_eps", C.c_float), ("logit_scale", C.c_float), ("loop_inject", C.c_int32), ("norms", C.c_int32), ("layer_scales", C.c_int32),
                 ("tied_head", C.c_int32), ("embed_scale", C.c_float), ("bigram_buckets", C.c_int32), ("bigram_mul_prev", C.c_int64),
-                ("bigram_mul_cur", C.c_int64), ("max_positions", C.c_int32), ("dtype", C.c_int32)]
+                ("bigram_mul_cur", C.c_int64), ("max_positions", C.c_int32), ("dtype", C.c_int32), ("cache", C.c_int32)]
 
 
 class KVCacheDesc(C.Structure):
@@ -206,7 +206,7 @@ TLM_SIGNATURES = {
     "mmi_tlm_launch_list": (C.c_int64, [_P, _P, C.c_int64]),
     "mmi_kv_append": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P]),
     "mmi_kv_read": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, _P, _P, _P]),
-    "mmi_kv_attend_workspace": (C.c_int64, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "mmi_kv_attend_workspace": (C.c_int64, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, C.c_int32]),
     "mmi_kv_attend": (C.c_int, [C.POINTER(KVCacheDesc), C.POINTER(KVSeqs), C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_float, C.c_int32,
                                 C.c_int32, C.c_int32, _P, C.c_int64, _P]),
     "mmi_beam_select_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),

@@ -15,6 +15,7 @@
 #include "tlm_kernels.h"
 #include "tlm_gqa.h"
 #include "tlm_linear.h"
+#include "tlm_ops.h"
 
 #include <math.h>
 #include <stdio.h>
@@ -50,7 +51,7 @@ struct Layer {
     float *qw = nullptr, *cw = nullptr;
     int qp = 0, kvp = 0, rp = 0, hp = 0, dim_p = 0, vdim_p = 0, lat_ks = 0, k_ks = 0, nd = 0, q_ks = 0, qn_ks = 0;
     int rope = -1, geo = -1;
-    // grouped attention: `in` is [queries | keys | values]; k_ks, nd as above
+    // grouped attention: `in` is [queries | keys | values]; k_ks, nd as above; with a cache in 8 bits it gives fp32 rows (in_ld)
     // channel delta: `in` is [q | k | v | beta], `lr` the low-rank halves of decay and gate, `a2` and `g2` the others; lightning: [q | k | v | gate]
     Mat lr, a2, g2;
     float *conv_w = nullptr, *decay = nullptr, *nw = nullptr;      // decay: (summand, factor) per column / powers of the constants
@@ -66,6 +67,7 @@ struct Run {                       // one execution of a layer: repeated layers 
     bool add_emb = false;
     int pass = -1;                 // first layer of a pass that starts with the projection of [x; embedding]
     void *kc = nullptr, *vc = nullptr;
+    float *ks = nullptr, *vs = nullptr;      // scales of a cache in 8 bits
     float *state = nullptr, *conv = nullptr;
 };
 
@@ -92,6 +94,7 @@ struct Meta {
 
 struct Shape {                     // what a launch list depends on
     int T = 0, n_want = 0, n_entries = 0, n_seg = 0, nsplit = 1;
+    int span = 0;                  // cache in 8 bits: log2 of pages that no sequence has more of
     bool pairs = false;            // some sequence spans several scan segments
     int n_small = 0, n_unit = 0, n_chunk = 0;      // sequences stepped token by token, sequences cut into chunks, their chunks
     std::vector<int> tiles;        // attention column tiles per head count
@@ -156,10 +159,12 @@ struct mmi_tlm {
     bool say_forms = false;        // test hook (MMI_TLM_FORMS): a line on stderr for every launch of the tiled kernels
     int force_wide = 0;            // test hook (MMI_TLM_WIDE): every product that k_tlm_gemm_wide can take goes there, in blocks of so many rows
     long weight_bytes = 0;
+    float* kv8_work = nullptr;     // partial sums of the attention over a cache in 8 bits
 };
 
 namespace {
 
+constexpr size_t KV8_ROOM = (size_t)16 << 20;      // floats of mmi_tlm::kv8_work
 constexpr int MAX_SPLIT = 8;
 constexpr int TILE_SPLIT = 8, TILE_BLOCKS = 512;      // the tiled kernel: K splits, blocks that a split aims at
 constexpr int ROWS_MAX = 64;       // up to here a step takes the weight-streaming kernel
@@ -406,10 +411,11 @@ int load_attention(Loader& ld, Layer& L, const std::string& p) {
     mmi_tlm* m = ld.m;
     const mmi_tlm_layer& c = L.c;
     const int D = m->cfg.width, H = c.heads, G = c.kv_heads, ks = m->kstep;
-    L.dim_p = round_up(c.dim, ks);
+    L.dim_p = round_up(c.dim, m->cfg.cache ? 16 : ks);
     L.vdim_p = round_up(c.vdim, 16);
     L.k_ks = L.dim_p / ks;
     L.nd = L.vdim_p / 16;
+    L.in_ld = (H + G) * L.dim_p + G * L.vdim_p;
     const std::string mx = p + ".mix.";
     int rc;
     if ((rc = ld.alloc(&L.in, 1, ((H + G) * L.dim_p + G * L.vdim_p) / 16, round_up(D, ks) / ks)) || (rc = ld.heads(mx + "q", H, c.dim, L.dim_p, D, &L.in, 0)) ||
@@ -545,6 +551,9 @@ int load_moe(Loader& ld, Layer& L, const std::string& p) {
 int check_cfg(const mmi_tlm_cfg& c) {
     if (c.vocab < 1 || c.width < 1 || c.n_layers < 1 || !c.layers) return mmi_fail(MMI_ERR_INVALID, "token LM: empty configuration");
     if (c.dtype != MMI_BF16 && c.dtype != MMI_F32) return mmi_fail(MMI_ERR_UNSUPPORTED, "token LM: dtype must be bf16 or fp32");
+    if (c.cache != 0 && c.cache != MMI_I8 && c.cache != MMI_F8E4M3) return mmi_fail(MMI_ERR_UNSUPPORTED, "token LM: the cache is of the operands' type, int8 or e4m3");
+    if (c.cache != 0 && std::none_of(c.layers, c.layers + c.n_layers, [](const mmi_tlm_layer& l) { return l.mixer == MMI_TLM_MIX_ATTENTION; }))
+        return mmi_fail(MMI_ERR_UNSUPPORTED, "token LM: a cache in 8 bits is for grouped attention, which no layer has");
     if (c.norm_groups < 1 || c.width % c.norm_groups) return mmi_fail(MMI_ERR_INVALID, "token LM: width must be a multiple of the norm groups");
     if (c.width > 8192) return mmi_fail(MMI_ERR_UNSUPPORTED, "token LM: width above 8192");
     if (c.loop_start < 0 || c.loop_stop < c.loop_start || c.loop_stop > c.n_layers || (c.loop_stop > c.loop_start && c.loop_times < 1))
@@ -626,9 +635,13 @@ int alloc_buffers(mmi_tlm* m) {
             gru_w = std::max(gru_w, L.wp);
             y_ks = std::max(y_ks, L.out.KS);
         } else if (L.c.mixer == MMI_TLM_MIX_ATTENTION) {
-            q_elems = std::max(q_elems, (long)((T * (long)L.c.heads + 15) / 16) * L.k_ks);
             o_ks = std::max(o_ks, L.out.KS);
-            nd = std::max(nd, L.nd);
+            if (c.cache) {
+                lin_ld = std::max(lin_ld, (long)L.in_ld);
+            } else {
+                q_elems = std::max(q_elems, (long)((T * (long)L.c.heads + 15) / 16) * L.k_ks);
+                nd = std::max(nd, L.nd);
+            }
         } else if (L.linear()) {
             lin_ld = std::max(lin_ld, (long)L.in_ld);
             conv_c = std::max(conv_c, (long)L.conv_c);
@@ -663,9 +676,11 @@ int alloc_buffers(mmi_tlm* m) {
     }
     if (c.norms == 2 && (rc = alloc_packed(m, &m->h2, std::max(T, m->max_slots), m->h_ks))) return rc;
     if (m->loop_in.wp && (rc = alloc_packed(m, &m->cat, T, 2 * m->h_ks))) return rc;
+    if (lin_ld && (rc = alloc_f32(m, &m->lin, (size_t)T * lin_ld))) return rc;
+    if (c.cache && (rc = alloc_f32(m, &m->kv8_work, KV8_ROOM))) return rc;
     if (m->has_linear) {
         const size_t n_chunk = (size_t)T / TLM_CHUNK + std::min(m->max_slots, T / (TLM_SMALL + 1)) + 1;      // only sequences above TLM_SMALL tokens have any
-        if ((rc = alloc_f32(m, &m->lin, (size_t)T * lin_ld)) || (rc = alloc_f32(m, &m->qkv, (size_t)T * conv_c)) || (rc = alloc_f32(m, &m->dec, (size_t)T * dec_ld)) ||
+        if ((rc = alloc_f32(m, &m->qkv, (size_t)T * conv_c)) || (rc = alloc_f32(m, &m->dec, (size_t)T * dec_ld)) ||
             (rc = alloc_f32(m, &m->lgate, (size_t)T * lgate_ld)) || (rc = alloc_f32(m, &m->lo, (size_t)T * lo_ld)) || (rc = alloc_packed(m, &m->lr, T, std::max(1, lr_ks))) ||
             (rc = alloc_f32(m, &m->cw, conv_c ? n_chunk * TLM_CHUNK * hd : 1)) || (rc = alloc_f32(m, &m->cq_g, n_chunk * TLM_CHUNK * hd)) ||
             (rc = alloc_f32(m, &m->ckt, n_chunk * TLM_CHUNK * hd)) || (rc = alloc_f32(m, &m->cu0, conv_c ? n_chunk * TLM_CHUNK * hv : 1)) ||
@@ -749,6 +764,19 @@ int alloc_state(mmi_tlm* m) {
                 MMI_HIP_CHECK(m->st.alloc(&r.conv, nc));
                 MMI_HIP_CHECK(hipMemset(r.conv, 0, nc * sizeof(float)));
             }
+        } else if (L.c.mixer == MMI_TLM_MIX_ATTENTION && m->cfg.cache) {
+            const size_t units = (size_t)m->max_pages * L.c.kv_heads, nk = units * TLM_PAGE * L.dim_p, nv = units * TLM_PAGE * L.vdim_p;
+            uint8_t *k = nullptr, *v = nullptr;
+            MMI_HIP_CHECK(m->st.alloc(&k, nk));
+            MMI_HIP_CHECK(hipMemset(k, 0, nk));
+            MMI_HIP_CHECK(m->st.alloc(&v, nv));
+            MMI_HIP_CHECK(hipMemset(v, 0, nv));
+            for (float** p : {&r.ks, &r.vs}) {
+                MMI_HIP_CHECK(m->st.alloc(p, units * KV8_PARTS));
+                MMI_HIP_CHECK(hipMemset(*p, 0, units * KV8_PARTS * sizeof(float)));
+            }
+            r.kc = k;
+            r.vc = v;
         } else if (L.c.mixer == MMI_TLM_MIX_ATTENTION) {
             const size_t nk = (size_t)m->max_pages * L.c.kv_heads * 4 * L.k_ks * 64, nv = (size_t)m->max_pages * L.c.kv_heads * (TLM_PAGE / m->kstep) * L.nd * 64;
             u32x4 *k = nullptr, *v = nullptr;
@@ -1391,7 +1419,58 @@ MixerOut build_latent_attention(mmi_tlm* m, MmiProgram& P, const Shape& sh, cons
     return MixerOut{&L.out, m->o, L.out.KS};
 }
 
+// over a cache in 8 bits: the projection gives fp32 rows, which are rounded into the cache, then attended with
+MixerOut build_attention_8(mmi_tlm* m, MmiProgram& P, const Shape& sh, const Layer& L, const Run& r, TlmJobs first, const Plan& p, const std::string& site) {
+    const int T = sh.T, H = L.c.heads, G = L.c.kv_heads;
+    const bool f32 = m->f32;
+    TlmJob j = dense_job(L.in, m->h, m->h_ks, T);
+    j.epi = TLM_EPI_F32;
+    j.out = m->lin;
+    j.out_ld = L.in_ld;
+    first.j[first.n++] = j;
+    P.site(site + "in");
+    plan_jobs(m, p, first, 0);
+    add_jobs(m, P, p, first, L.in.bytes());
+
+    TlmKv8Append u;
+    memset(&u, 0, sizeof(u));
+    u.c = TlmKv8Cache{(uint8_t*)r.kc, (uint8_t*)r.vc, r.ks, r.vs, m->max_pages, G, L.dim_p, L.vdim_p, m->cfg.cache == MMI_F8E4M3, 0, 0, nullptr};
+    const bool one = T == sh.n_entries;                  // a row each
+    u.q = TlmKv8Seqs{sh.n_entries, T, one ? nullptr : m->meta + sh.m.erow0, one ? nullptr : m->meta + sh.m.elen, m->meta + sh.m.epos0, m->meta + sh.m.eslot,
+                     TlmPages{m->block_table, table_ld(m), m->keep_pages}, 1};
+    u.k = m->lin + H * L.dim_p;
+    u.v = m->lin + (H + G) * L.dim_p;
+    u.k_row = u.v_row = L.in_ld;
+    u.k_head = L.dim_p;
+    u.v_head = L.vdim_p;
+    u.wide = 1;
+    P.site(site + "append");
+    P.add([=](hipStream_t s) { return tlm_kv8_append(s, u, MMI_F32); });
+
+    TlmKv8Attn a;
+    memset(&a, 0, sizeof(a));
+    a.c = u.c;
+    a.q = u.q;
+    a.x = m->lin;
+    a.x_row = L.in_ld;
+    a.x_head = L.dim_p;
+    a.wide = 1;
+    a.out = m->o;
+    a.out_ks = L.out.KS;
+    a.heads = H;
+    a.rep = H / G;
+    a.nd = L.nd;
+    a.mask = TlmMask{L.c.window, L.c.window > 0 ? L.c.keep_first : 0, L.c.scale * 1.44269504088896340736f};
+    a.sink = L.c.sink;
+    tlm_kv8_plan(a, 1l << sh.span, KV8_ROOM);
+    tlm_kv8_workspace(a, m->kv8_work);
+    P.site(site + "attn");
+    P.add([=](hipStream_t s) { return tlm_kv8_attend(s, a, MMI_F32, f32); });
+    return MixerOut{&L.out, m->o, L.out.KS};
+}
+
 MixerOut build_attention(mmi_tlm* m, MmiProgram& P, const Shape& sh, const Layer& L, const Run& r, TlmJobs first, const Plan& p, const std::string& site) {
+    if (m->cfg.cache) return build_attention_8(m, P, sh, L, r, first, p, site);
     const int T = sh.T, H = L.c.heads, G = L.c.kv_heads;
     const bool f32 = m->f32;
     TlmJob j = dense_job(L.in, m->h, m->h_ks, T);
@@ -2180,6 +2259,8 @@ extern "C" int mmi_tlm_step(mmi_tlm* m, int32_t n_entries, const int32_t* slots,
         int64_t span = S.pos + counts[e];
         if (m->max_window > 0) span = std::min<int64_t>(span, m->max_window + counts[e] + m->keep_pages * TLM_PAGE);
         blocks = std::max(blocks, span / 32 + 1);
+        if (m->cfg.cache)
+            while ((int64_t)1 << sh.span < (S.pos + counts[e] - 1) / TLM_PAGE + 1) ++sh.span;
         S.pos += counts[e];
         S.par ^= 1;
     }
@@ -2199,7 +2280,7 @@ extern "C" int mmi_tlm_step(mmi_tlm* m, int32_t n_entries, const int32_t* slots,
     const bool decode = T == n_entries && T <= ROWS_MAX && !m->taps;
     if (decode) {
         sh.logits = m->logits;
-        auto& prog = m->progs[std::make_tuple(T, n_want, sh.nsplit)];
+        auto& prog = m->progs[std::make_tuple(T, n_want, sh.nsplit * 64 + sh.span)];
         if (!prog) {
             prog.reset(new MmiProgram());
             build_program(m, *prog, sh);

@@ -58,8 +58,13 @@ __device__ __forceinline__ const int* kv8_table(const TlmKv8Seqs& a, int e) { re
 
 // An entry's work is cut into pieces of `per` units, `mul` units a row, without anyone having counted them: entry e owns the slots from
 // row0[e] * mul / per + extra e on, which are as many as it can need, and a slot's entry is the last one that begins at or before it.
-struct Kv8Cut { int mul, per, extra; };                // mul 0: `extra` slots per entry
-__device__ __forceinline__ int kv8_slot0(const TlmKv8Seqs& a, const Kv8Cut& z, int e) { return (z.mul ? (int)((long)kv8_row0(a, e) * z.mul / z.per) : 0) + z.extra * e; }
+// (by > 0: only entries with at least `by` units need a slot; one more for each `by` units is then enough, where that is fewer than one per entry.)
+struct Kv8Cut { int mul, per, extra, by; };            // mul 0: `extra` slots per entry
+MMI_HD int kv8_slots_before(const Kv8Cut& z, int row, int e) {
+    const long u = (long)row * z.mul;
+    return (int)(u / z.per) + (z.by ? (int)(u / z.by) : z.extra * e);
+}
+__device__ __forceinline__ int kv8_slot0(const TlmKv8Seqs& a, const Kv8Cut& z, int e) { return z.mul ? kv8_slots_before(z, kv8_row0(a, e), e) : z.extra * e; }
 __device__ __forceinline__ int kv8_find(const TlmKv8Seqs& a, const Kv8Cut& z, int slot) {
     if (!z.mul) return min(slot / z.extra, a.n - 1);
     unsigned below = 0;
@@ -67,8 +72,8 @@ __device__ __forceinline__ int kv8_find(const TlmKv8Seqs& a, const Kv8Cut& z, in
     return max(mmi_uniform((int)mmi_wave_sum_u32(below) - 1), 0);
 }
 // host: the cut of mul * rows units (one row each: nothing to look for), and how many slots there are
-inline Kv8Cut kv8_cut(const TlmKv8Seqs& a, int mul, int per, int more) { return a.row0 ? Kv8Cut{mul, per, more} : Kv8Cut{0, per, mmi_cdiv(mul, per)}; }
-inline long kv8_slots(const TlmKv8Seqs& a, const Kv8Cut& z) { return (long)a.T * z.mul / z.per + (long)z.extra * a.n; }
+inline Kv8Cut kv8_cut(const TlmKv8Seqs& a, int mul, int per, int more) { return a.row0 ? Kv8Cut{mul, per, more, 0} : Kv8Cut{0, per, mmi_cdiv(mul, per), 0}; }
+inline long kv8_slots(const TlmKv8Seqs& a, const Kv8Cut& z) { return z.mul ? kv8_slots_before(z, a.T, a.n) + (z.by ? 1 : 0) : (long)z.extra * a.n; }
 
 // ---- codes ---------------------------------------------------------------------------------------------------------------
 template <bool E4M3>
@@ -344,13 +349,14 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
 
 // ---- attention -----------------------------------------------------------------------------------------------------------
 // Numerics, both kernels.  Operands are fp16, 11 bits: codes are exact in it, queries are first brought to [2^14, 2^15) by a power of two of
-// their own, softmax weights are carried times the value scale of their block, relative to a running reference of score + log2 of that scale: so
-// the largest lie between 2^8 and 2^15 however blocks' scales differ, and the reference, with the sums, moves only where a maximum has outgrown
-// it by 2^7.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both operands come in two parts, 22 bits, good to 2^-24.
+// their own, softmax weights are carried times the value scale of their block, relative to a running reference of score + exponent of that scale:
+// so the largest lie between 2^8 and 2^15 however blocks' scales differ, and the reference, with the sums, moves only where a maximum has outgrown
+// it by 2^6.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both operands come in two parts, 22 bits, good to 2^-24.
 // (bf16 operands left 1.8 times the error of the result's rounding.)  Sums, maxima and the denominator, which has the weights before they were
 // rounded, are fp32.
 constexpr int KV8_FEW = 16;              // sequences with up to so many columns, one tile, are the few's where a call may bring longer ones
-constexpr float KV8_UP = 8.f, KV8_SLACK = 7.f;      // log2: of what weights are carried times, of what they may outgrow it by (fp16 ends at 2^16)
+constexpr int KV8_MANY = 128;            // columns of a workgroup of the many's
+constexpr float KV8_UP = 8.f, KV8_SLACK = 6.f;      // log2: of what weights are carried times, of what they may outgrow it by (fp16 ends at 2^16)
 constexpr int KV8_ANGLES = 2048;         // pairs of a cosine and a sine in LDS
 
 struct Kv8Share {                        // one kernel's part of a call
@@ -410,7 +416,20 @@ struct Kv8Pages {
         return mmi_from_lane(held, i - from);
     }
 };
-__device__ __forceinline__ bool kv8_seen(const TlmMask& m, int pos, int key) { return key <= pos && (m.window <= 0 || pos - key < m.window || key < m.keep); }
+// a value scale = fraction 2^exponent (at least 2^-120; a NaN's fraction is one), and 2^-exponent
+__device__ __forceinline__ float kv8_fraction(float scale, float& exponent, float& back) {
+    const float v = scale < 0x1p-120f ? 0x1p-120f : scale;
+    const int e = min((int)(__builtin_bit_cast(unsigned, v) >> 23 & 255u) - 127, 126);
+    exponent = (float)e;
+    back = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
+    return v * back;
+}
+// scores of keys key0 .. key0 + 15 for a query at `pos`, -infinity where it does not see them
+__device__ __forceinline__ void kv8_masked(const TlmMask& m, int pos, int key0, float (&y)[16]) {
+    const int behind = m.window > 0 ? pos - m.window : -1;      // the last position that a window has passed
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[r] = (key0 + r <= pos) & ((key0 + r > behind) | (key0 + r < m.keep)) ? y[r] : -INFINITY;
+}
 // positions plo .. phi all see the n keys from key0 on
 __device__ __forceinline__ bool kv8_whole(const TlmMask& m, int plo, int phi, int key0, int n) { return key0 + n - 1 <= plo && (m.window <= 0 || phi - key0 < m.window || key0 + n <= m.keep); }
 
@@ -418,13 +437,14 @@ __device__ __forceinline__ bool kv8_whole(const TlmMask& m, int plo, int phi, in
 template <bool E4M3>
 __device__ __forceinline__ u32x4 kv8_quiet(const Kv8Cols& c, const TlmMask& m, int key0, u32x4 w) {
     if constexpr (!E4M3) return w;
+    const int behind = m.window > 0 ? c.plo - m.window : -1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         uint32_t keep = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int key = key0 + 4 * j + r;
-            keep |= key <= c.phi && (m.window <= 0 || c.plo - key < m.window || key < m.keep) ? 0xffu << (8 * r) : 0u;
+            keep |= (key <= c.phi) & ((key > behind) | (key < m.keep)) ? 0xffu << (8 * r) : 0u;
         }
         w[j] &= keep;
     }
@@ -543,6 +563,7 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     const int i0 = split * a.few.pages, i1 = min(c.n, i0 + a.few.pages);
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
     const int col = min(c.c0 + bl, c.ncol - 1), tok = col / a.rep, pos = c.s.pos0 + tok;
+    const bool live = c.c0 + bl < c.ncol;
     const int* bt = kv8_table(a.q, c.s.e);
     u32x4 kf[4][NP], vf[ND];
     float ks = 0.f, vs = 0.f;
@@ -557,14 +578,14 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         const int p = pages.at(a, c, bt, i);
         have = p >= 0;
         const long unit = (long)max(p, 0) * a.c.kv_heads + g;
-        const uint8_t* kp = a.c.k + (unit * TLM_PAGE + 16 * (bl >> 2) + (bl & 3)) * a.c.dim + 16 * kq;
+        const uint8_t* kp = a.c.k + (unit * TLM_PAGE + 16 * (bl >> 2) + (bl & 3)) * a.c.dim;
         const uint8_t* vp = a.c.v + (unit * a.c.vdim + bl) * TLM_PAGE + 16 * kq;
         ks = a.c.ks[unit * KV8_PARTS + kq];
         vs = a.c.vs[unit * KV8_PARTS + kq];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int p = 0; p < NP; ++p) kf[t][p] = mmi_load_nt((const u32x4*)(kp + 4 * t * a.c.dim + (64 * p + 16 * kq < a.c.dim ? 64 * p : 0)));
+            for (int p = 0; p < NP; ++p) kf[t][p] = mmi_load_nt((const u32x4*)(kp + 4 * t * a.c.dim + (64 * p + 16 * kq < a.c.dim ? 64 * p + 16 * kq : 0)));      // (dimensions past the head's meet zeros)
 #pragma unroll
         for (int d = 0; d < ND; ++d) vf[d] = mmi_load_nt((const u32x4*)(vp + min(d, a.nd - 1) * 16 * TLM_PAGE));
     };
@@ -588,7 +609,8 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     for (int i = i0 + wave; i < i1; i += WK) {
         const int key0 = nb * TLM_PAGE + 16 * kq;
         const bool now = have, whole = kv8_whole(a.mask, c.plo, c.phi, nb * TLM_PAGE, TLM_PAGE);
-        const float sc = ks * back, lv = mmi_fast_log2f(fmaxf(vs, 0x1p-120f) + 0.f * vs), rv = mmi_fast_exp2f(-lv);      // (a NaN stays one)
+        float lv, rv;
+        const float sc = ks * back, fraction = kv8_fraction(vs, lv, rv);
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -610,17 +632,15 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         load(i + WK);
         mmi_sched_barrier();
         if (!now) continue;
-        float mx = -INFINITY;
+        // (scalars: an element of a vector written behind a branch has come out as its neighbour where the vector was kept in accumulation registers)
+        float y[16], mx = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int r = 0; r < 16; ++r) y[r] = mmi_fma(s[r >> 2][r & 3], sc, lv);
+        if (!whole) kv8_masked(a.mask, pos, key0, y);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[t][r] = mmi_fma(s[t][r], sc, lv);
-                if (!whole) s[t][r] = kv8_seen(a.mask, pos, key0 + 4 * t + r) ? s[t][r] : -INFINITY;
-                mx = fmaxf(mx, s[t][r]);
-            }
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[r]);
         mx = mmi_rows_max(mx);
-        if (mmi_any(mx > m + KV8_SLACK)) {
+        if (mmi_any(live && mx > m + KV8_SLACK)) {         // (the tile's other columns hold anything)
             const float to = fmaxf(m, mx), al = mmi_fast_exp2f(m - (to == -INFINITY ? 0.f : to));
             l *= al;
 #pragma unroll
@@ -628,34 +648,25 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
             m = to;
         }
         const float ms = (m == -INFINITY ? 0.f : m) - KV8_UP;
-        u32x4 pf[NS][2];
+        u32x4 pf[2][NS];
         float sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float e[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                e[r] = mmi_fast_exp2f(s[t][r] - ms);
-                sum += e[r];
-            }
-            uint32_t lo[NS], hi[NS];
-            kv8_split2<NS>(e[0], e[1], lo);
-            kv8_split2<NS>(e[2], e[3], hi);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                pf[n][t >> 1][2 * (t & 1)] = lo[n];
-                pf[n][t >> 1][2 * (t & 1) + 1] = hi[n];
-            }
+        for (int r = 0; r < 16; ++r) {
+            y[r] = mmi_fast_exp2f(y[r] - ms);
+            sum += y[r];
         }
-        l += sum == 0.f ? 0.f : sum * rv;                  // (the scale of a block that no column sees may be anything)
+        const float times = sum == 0.f ? 0.f : fraction;   // (the scale of a block that the column does not see may be anything)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) kv8_split8<NS>(y + 8 * u, times, pf[u]);
+        l += sum * rv;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             u32x4 lo, hi;
             C::fragments(vw[d], lo, hi);
 #pragma unroll
             for (int n = NS - 1; n >= 0; --n) {
-                acc[d] = mmi_mfma_f16_16x16x32(lo, pf[n][0], acc[d]);
-                acc[d] = mmi_mfma_f16_16x16x32(hi, pf[n][1], acc[d]);
+                acc[d] = mmi_mfma_f16_16x16x32(lo, pf[0][n], acc[d]);
+                acc[d] = mmi_mfma_f16_16x16x32(hi, pf[1][n], acc[d]);
             }
         }
     }
@@ -692,7 +703,7 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
 #pragma unroll
             for (int o = 1; o < WK; ++o) v += ob[(o * 8 + d) * 64 + lane];
             v *= inv;
-            if (c.c0 + bl >= c.ncol) continue;
+            if (!live) continue;
             const int dim = (d0 + d) * 16 + 4 * kq, head = g * a.rep + col - tok * a.rep;
             if (parts) *reinterpret_cast<f32x4*>(a.few.po + (part * 16 + bl) * a.c.vdim + dim) = v;
             else kv8_store<Tr>(a, c.s.row0 + tok, head, dim, v);
@@ -719,7 +730,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8At
 //   lane ^ 4 (lane / 32): what lets the writers, who have 16 codes of one key or dimension each, meet no bank twice
 template <int NS, int D>
 struct Kv8Tile {
-    static constexpr int QT = 1, PER = 128 * QT, KS = D / 16, DT = D / 32;
+    static constexpr int QT = 1, PER = KV8_MANY, KS = D / 16, DT = D / 32;
     static constexpr int KF = KS * 64, VF = DT * 2 * 64;                       // vectors per buffer
     static constexpr size_t smem() { return std::max({(size_t)2 * (KF + VF) * 16, (size_t)PER * D * NS * 2 + PER * 4 + KV8_ANGLES * 8, (size_t)KV8_LDS * 16}); }
 };
@@ -878,9 +889,10 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         if (busy) scores(set ^ 1, set ^ 1);
         if (busy && now && key0 <= phi) {
             const bool whole = kv8_whole(a.mask, plo, phi, key0, 32);
-            const float lv = mmi_fast_log2f(fmaxf(vsn, 0x1p-120f) + 0.f * vsn), rv = mmi_fast_exp2f(-lv);
+            float lv, rv;
+            const float fraction = kv8_fraction(vsn, lv, rv);
             u32x4 pf[QT][2][NS];
-            float mx[QT];
+            float mx[QT], y[QT][16];
             bool moved = false;
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
@@ -888,14 +900,12 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
                 const int pos = c.s.pos0 + tok[t];
                 float x = -INFINITY;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float y = mmi_fma(s[set][t][r], sc, lv);
-                    if (!whole) y = kv8_seen(a.mask, pos, key0 + 16 * hi + r) ? y : -INFINITY;
-                    s[set][t][r] = y;
-                    x = fmaxf(x, y);
-                }
+                for (int r = 0; r < 16; ++r) y[t][r] = mmi_fma(s[set][t][r], sc, lv);
+                if (!whole) kv8_masked(a.mask, pos, key0 + 16 * hi, y[t]);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x = fmaxf(x, y[t][r]);
                 mx[t] = mmi_halves_max(x);
-                moved = moved || mx[t] > m[t] + KV8_SLACK;
+                moved = moved || (w0 + 32 * t + cl < c.ncol && mx[t] > m[t] + KV8_SLACK);      // (the tile's other columns hold anything)
             }
             if (mmi_any(moved)) {
 #pragma unroll
@@ -910,15 +920,16 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
                 const float ms = (m[t] == -INFINITY ? 0.f : m[t]) - KV8_UP;
-                float sum = 0.f, e[16];
+                float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    e[r] = mmi_fast_exp2f(s[set][t][r] - ms);
-                    sum += e[r];
+                    y[t][r] = mmi_fast_exp2f(y[t][r] - ms);
+                    sum += y[t][r];
                 }
-                l[t] += sum == 0.f ? 0.f : sum * rv;
+                l[t] += sum * rv;
+                const float times = sum == 0.f ? 0.f : fraction;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) kv8_split8<NS>(e + 8 * u, 1.f, pf[t][u]);
+                for (int u = 0; u < 2; ++u) kv8_split8<NS>(y[t] + 8 * u, times, pf[t][u]);
             }
 #pragma unroll
             for (int d0 = 0; d0 < DT; d0 += 4) {

@@ -4,8 +4,9 @@
 
 // dtype of keys, values and queries: MMI_BF16 or MMI_F32 (a.k / a.v / a.x); exact: fp32 arithmetic for fp32 queries
 int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype);
-// fills in how the work is split (`cap`: pages that a sequence can have at most) and says what workspace that takes, in floats
-size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, bool f32);
+// fills in how the work is split (`cap`: pages that a sequence can have at most; `room`: floats that a workspace may have) and says what workspace
+// that takes, in floats
+size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, size_t room);
 void tlm_kv8_workspace(TlmKv8Attn& a, float* workspace);      // aligned to 16 bytes
 int tlm_kv8_attend(hipStream_t s, const TlmKv8Attn& a, int dtype, bool f32);
 

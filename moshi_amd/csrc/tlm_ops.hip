@@ -7,13 +7,13 @@
 namespace {
 
 constexpr long KV8_WORKGROUPS = 512;     // that a split of the pages aims at: 2 per CU, all at once
-constexpr long KV8_TILE_WORKGROUPS = 256;      // the same for many columns: one runs per CU
 constexpr int KV8_MAX_SPLIT = 256;       // (k_tlm_kv8_combine: a lane each)
 
 int check_cache(const mmi_kv_cache* c, TlmKv8Cache* out, const char* at) {
     auto bad = [&](int code, const char* what) { return mmi_fail(code, std::string(at) + ": " + what); };
-    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return bad(MMI_ERR_INVALID, "null cache");
+    if (!c) return bad(MMI_ERR_INVALID, "null cache");
     if (c->pages < 1 || c->pages > 0x7fffffff) return bad(MMI_ERR_SHAPE, "the cache needs between 1 and 2^31 - 1 pages");
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return bad(MMI_ERR_INVALID, "null cache");
     if (c->kv_heads < 1 || c->kv_heads > 65535) return bad(MMI_ERR_SHAPE, "key/value heads");
     if (c->dim < 16 || c->dim > 256 || c->dim % 16 || c->vdim < 16 || c->vdim > 256 || c->vdim % 16)
         return bad(MMI_ERR_UNSUPPORTED, "head sizes are multiples of 16 up to 256");
@@ -87,14 +87,20 @@ int launch_attn_d(hipStream_t s, const TlmKv8Attn& a) {
     const int d = attn_bound(a.c);
     return d == 64 ? launch_attn_c<In, Tr, NS, 64>(s, a) : (d == 128 ? launch_attn_c<In, Tr, NS, 128>(s, a) : launch_attn_c<In, Tr, NS, 256>(s, a));
 }
-// how a kernel's groups share the pages out; floats of workspace
-size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, long workgroups) {
+// how a kernel's `groups` (the ones that are likely to have columns) share the pages out; floats of workspace, at most `room`
+size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, size_t room) {
+    if (a.mask.window > 0)                             // positions plo - window + 1 .. phi, and the first ones that are kept
+        cap = std::min<long>(cap, ((long)a.mask.window + h.z.per / a.rep + 1) / TLM_PAGE + 2 + mmi_cdiv(a.mask.keep, TLM_PAGE));
+    cap = std::max(cap, 1l);
     const long units = std::max(1l, groups * a.c.kv_heads);
-    long per = std::max((cap * units + workgroups - 1) / workgroups, (cap + KV8_MAX_SPLIT - 1) / KV8_MAX_SPLIT);
+    const size_t each = (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.z.per * (a.c.vdim + 2);      // floats per split
+    long most = std::min<long>(KV8_MAX_SPLIT, (long)(room / std::max<size_t>(1, each)));
+    if (most < 2) most = 1;
+    long per = std::max((cap * units + KV8_WORKGROUPS - 1) / KV8_WORKGROUPS, (cap + most - 1) / most);
     per = std::min((per + 3) / 4 * 4, (cap + 3) / 4 * 4);      // (each of a workgroup's four waves takes every fourth page)
     h.pages = (int)per;
     h.nsplit = (int)((cap + per - 1) / per);
-    return h.nsplit > 1 ? (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.nsplit * h.z.per * (a.c.vdim + 2) : 0;
+    return h.nsplit > 1 ? each * h.nsplit : 0;
 }
 
 }  // namespace
@@ -110,22 +116,17 @@ int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype) {
     });
 }
 
-size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, bool f32) {
-    if (a.mask.window > 0) cap = std::min<long>(cap, (long)a.mask.window / TLM_PAGE + 3 + mmi_cdiv(a.mask.keep, TLM_PAGE));
-    cap = std::max(cap, 1l);
+size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, size_t room) {
     a.both = a.q.row0 != nullptr;
-    a.few.z = a.both ? Kv8Cut{0, 16, std::min(KV8_FEW / 16, mmi_cdiv(a.q.T * a.rep, 16))} : Kv8Cut{0, 16, mmi_cdiv(a.rep, 16)};
-    a.few.cols = std::min(16, a.both ? 16 : a.rep);
-    const size_t few = split_pages(a, a.few, a.both ? a.q.n : kv8_slots(a.q, a.few.z), cap, KV8_WORKGROUPS);
-    size_t many = 0;
-    if (a.both) {
-        a.many.z = Kv8Cut{a.rep, 128, 1};
-        a.many.cols = a.many.z.per;
-        many = split_pages(a, a.many, (long)a.q.T * a.rep / a.many.z.per + 1, cap, KV8_TILE_WORKGROUPS);
-    }
-    a.many.po = nullptr;
-    a.few.po = nullptr;
-    return few + many;
+    a.few.z = Kv8Cut{0, 16, a.both ? 1 : mmi_cdiv(a.rep, 16), 0};
+    a.few.cols = a.both ? KV8_FEW : std::min(16, a.rep);
+    const size_t few = split_pages(a, a.few, kv8_slots(a.q, a.few.z), cap, room);
+    if (!a.both) return few;
+    a.many.z = Kv8Cut{a.rep, KV8_MANY, 1, 0};
+    if ((long)a.q.T * a.rep / (KV8_FEW + 1) < a.q.n) a.many.z = Kv8Cut{a.rep, KV8_MANY, 0, KV8_FEW + 1};
+    a.many.cols = KV8_MANY;
+    const long full = (long)a.q.T * a.rep / KV8_MANY + 1;
+    return few + split_pages(a, a.many, full + (kv8_slots(a.q, a.many.z) - full) / 4, cap, room - few);
 }
 void tlm_kv8_workspace(TlmKv8Attn& a, float* w) {
     for (Kv8Share* h : {&a.few, &a.many}) {
@@ -175,7 +176,7 @@ extern "C" int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, i
 }
 
 namespace {
-int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t dtype, int32_t window, int32_t keep_first, TlmKv8Attn* a, size_t* floats) {
+int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first, TlmKv8Attn* a, size_t* floats) {
     memset(a, 0, sizeof(*a));
     int rc;
     if ((rc = check_cache(cache, &a->c, "mmi_kv_attend")) || (rc = check_seqs(seqs, &a->q, "mmi_kv_attend"))) return rc;
@@ -186,15 +187,15 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     a->nd = cache->vdim / 16;
     a->mask = TlmMask{window, window > 0 ? keep_first : 0, 0.f};
     if ((long)a->q.T * a->rep > 1l << 26) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^26 rows times query heads of a group");
-    *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1, dtype == MMI_F32);
+    *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1, (size_t)1 << 30);
     return MMI_OK;
 }
 }  // namespace
 
-extern "C" int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, int32_t window, int32_t keep_first) {
+extern "C" int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first) {
     TlmKv8Attn a;
     size_t floats;
-    const int rc = attn_args(cache, seqs, heads, dtype, window, keep_first, &a, &floats);
+    const int rc = attn_args(cache, seqs, heads, window, keep_first, &a, &floats);
     return rc ? rc : (int64_t)(floats * sizeof(float));
 }
 
@@ -203,7 +204,7 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
                              mmi_stream stream) {
     TlmKv8Attn a;
     size_t floats;
-    int rc = attn_args(cache, seqs, heads, dtype, window, keep_first, &a, &floats);
+    int rc = attn_args(cache, seqs, heads, window, keep_first, &a, &floats);
     if (rc) return rc;
     if (!a.q.n || !a.q.T) return MMI_OK;
     if ((rc = check_rows(q, q_row, q_head, dtype, "mmi_kv_attend")) || (rc = check_rows(out, out_row, out_head, dtype, "mmi_kv_attend"))) return rc;

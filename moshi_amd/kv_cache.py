@@ -69,7 +69,7 @@ class PagedKVCache:
         self._on = _capi.LaunchOn(self.device)
         self._where = k.get_device()
         self._need = {}
-        self._workspace(_capi.KVSeqs(), (0, 0, 0, _capi.MMI_BF16, self.kv_heads, 0, 0, True))      # (sizes that the kernels do not take are refused here)
+        self._workspace(_capi.KVSeqs(), (0, 0, 0, self.kv_heads, 0, 0, True))      # (sizes that the kernels do not take are refused here)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, dim: int, vdim: Optional[int] = None, codes: str = "int8", device: torch.device | str = "cuda", **rotation) -> "PagedKVCache":
@@ -107,10 +107,10 @@ class PagedKVCache:
         return shape[1], dtype, (t.data_ptr(), stride[0], stride[1])
 
     def _workspace(self, seqs: _capi.KVSeqs, key) -> int:
-        """Bytes that an attention of these sizes (sequences, rows, pages of a sequence, type, heads, window, first tokens, one row each?) works in."""
+        """Bytes that an attention of these sizes (sequences, rows, pages of a sequence, heads, window, first tokens, one row each?) works in."""
         need = self._need.get(key)
         if need is None:
-            need = self._lib.mmi_kv_attend_workspace(C.byref(self._desc), C.byref(seqs), *key[3:7])
+            need = self._lib.mmi_kv_attend_workspace(C.byref(self._desc), C.byref(seqs), *key[3:6])
             self._lib.check(min(0, need))
             if len(self._need) > 4096:
                 self._need.clear()
@@ -142,7 +142,7 @@ class PagedKVCache:
             if out.shape != (total, heads, self.vdim) or out.dtype != q.dtype:
                 raise AssertionError("out is [rows, heads, vdim] in the queries' type")
             op = self._rows(out, "out", heads, self.vdim)[2]
-        need = self._workspace(seqs, (seqs.n, total, seqs.table_ld, dtype, heads, window, keep_first, rows is None))
+        need = self._workspace(seqs, (seqs.n, total, seqs.table_ld, heads, window, keep_first, rows is None))
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._lib.check(self._on.call(self._lib.mmi_kv_attend, C.byref(self._desc), C.byref(seqs), dtype, heads, *qp, *op, self.dim ** -0.5 if scale is None else scale, window,
                                       keep_first, sink, work.data_ptr() if need else None, need))

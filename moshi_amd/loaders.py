@@ -203,8 +203,9 @@ def token_lm_config_from_dict(raw: dict, shapes: Optional[Dict[str, tuple]] = No
 
 
 def get_token_lm(path: str | Path, device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16, max_slots: int = 32,
-                 max_tokens: int = 65536, max_step_tokens: Optional[int] = None, load_weight: bool = True, lib=None) -> TokenLM:
-    """A token language model from a directory holding config.json and model.safetensors (load_weight=False: seeded random weights)."""
+                 max_tokens: int = 65536, max_step_tokens: Optional[int] = None, load_weight: bool = True, lib=None, kv_cache: Optional[str] = None) -> TokenLM:
+    """A token language model from a directory holding config.json and model.safetensors (load_weight=False: seeded random weights).
+    kv_cache: "int8" or "e4m3" holds grouped attention's keys and values in 8 bits."""
     path = Path(path)
     raw = json.loads((path / "config.json").read_text())
     if load_weight:
@@ -214,7 +215,7 @@ def get_token_lm(path: str | Path, device: torch.device | str = "cuda", dtype: t
         cfg = token_lm_config_from_dict(raw)
         from .weights import random_token_lm_state_dict
         state = random_token_lm_state_dict(cfg, seed=0)
-    return TokenLM(state, cfg, device=device, dtype=dtype, max_slots=max_slots, max_tokens=max_tokens, max_step_tokens=max_step_tokens, lib=lib)
+    return TokenLM(state, cfg, device=device, dtype=dtype, max_slots=max_slots, max_tokens=max_tokens, max_step_tokens=max_step_tokens, lib=lib, kv_cache=kv_cache)
 
 
 def export_quantized(src: str | Path, dst: str | Path, fmt: str = "int8", lm_kwargs: Optional[dict] = None) -> Dict[str, int]:

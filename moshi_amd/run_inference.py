@@ -158,7 +158,8 @@ def run_token_lm(args) -> None:
     pool = sum(sorted((pages(len(p) + args.max_new_tokens) for p in prompts), reverse=True)[:args.batch_size])
     step_tokens = min(args.step_tokens, pool)
     log("info", f"loading {args.checkpoint_dir}")
-    lm = loaders.get_token_lm(args.checkpoint_dir, device=args.device, dtype=dtype, max_slots=args.batch_size, max_tokens=pool, max_step_tokens=step_tokens)
+    lm = loaders.get_token_lm(args.checkpoint_dir, device=args.device, dtype=dtype, max_slots=args.batch_size, max_tokens=pool, max_step_tokens=step_tokens,
+                               kv_cache=None if args.kv_cache == "like-dtype" else args.kv_cache)
     batcher = TokenBatcher(lm, step_tokens=step_tokens, seed=args.seed)
     t0 = time.time()
     out = batcher.generate(prompts, args.max_new_tokens, temp=0.0 if args.greedy else args.temp, top_k=args.top_k, stop=args.stop_token)
@@ -191,6 +192,7 @@ def main(argv: Optional[List[str]] = None) -> None:
     tok.add_argument("--stop-token", type=int, action="append", default=[], help="end a continuation after this token (repeatable)")
     tok.add_argument("--step-tokens", type=int, default=2048, help="most tokens of one batch: prompts are cut into portions of it")
     tok.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    tok.add_argument("--kv-cache", choices=["like-dtype", "int8", "e4m3"], default="like-dtype", help="what grouped attention's keys and values are held in")
     ap.add_argument("infile", type=str)
     ap.add_argument("outfile", type=str)
     args = ap.parse_args(argv)

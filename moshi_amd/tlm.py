@@ -22,7 +22,7 @@ from .config import (ChannelDeltaConfig, DenseGLUConfig, GroupedAttentionConfig,
 Entry = Tuple[int, Sequence[int], Sequence[int]]          # slot, next tokens, wanted places among them
 
 
-def _cfg_struct(cfg: TokenLMConfig, dtype: torch.dtype):
+def _cfg_struct(cfg: TokenLMConfig, dtype: torch.dtype, kv_cache: Optional[str] = None):
     layers = (_capi.TLMLayer * len(cfg.layers))()
     for out, layer in zip(layers, cfg.layers):
         m = layer.mixer
@@ -68,6 +68,7 @@ def _cfg_struct(cfg: TokenLMConfig, dtype: torch.dtype):
         s.bigram_buckets, s.bigram_mul_prev, s.bigram_mul_cur = cfg.bigram.buckets, cfg.bigram.mul_prev, cfg.bigram.mul_cur
     s.max_positions = cfg.max_positions
     s.dtype = _capi.MMI_F32 if dtype == torch.float32 else _capi.MMI_BF16
+    s.cache = {None: 0, "int8": _capi.MMI_I8, "e4m3": _capi.MMI_F8E4M3}[kv_cache]
     return s, layers
 
 
@@ -83,14 +84,18 @@ class TokenLM:
         dtype: torch.bfloat16 (bf16 operands, fp32 accumulation, fp32 where the design wants it) or torch.float32 (all fp32).
         max_slots: live sequences.  max_tokens: tokens the cache pool holds over all of them (rounded up to pages).
         max_step_tokens: tokens of one step (activation buffers); default = the pool.
+        kv_cache: keys and values of the grouped-attention layers: None like `dtype`, "int8" or "e4m3" in 8 bits with a scale for each 16 tokens
+            and head (half of bf16's bytes, a quarter of fp32's; kv_cache.py).
     """
 
     def __init__(self, state_dict: Dict[str, torch.Tensor], config: TokenLMConfig, device: torch.device | str = "cuda",
                  dtype: torch.dtype = torch.bfloat16, max_slots: int = 32, max_tokens: int = 65536, max_step_tokens: Optional[int] = None,
-                 lib: Optional[_capi.Lib] = None):
+                 lib: Optional[_capi.Lib] = None, kv_cache: Optional[str] = None):
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype must be torch.bfloat16 or torch.float32")
-        self.config, self.dtype, self.device = config, dtype, torch.device(device)
+        if kv_cache not in (None, "int8", "e4m3"):
+            raise ValueError("kv_cache must be None, 'int8' or 'e4m3'")
+        self.config, self.dtype, self.device, self.kv_cache = config, dtype, torch.device(device), kv_cache
         if lib is None:
             if self.device.type != "cuda":
                 raise RuntimeError("moshi_amd.TokenLM runs on an MI355X (device='cuda'); there is no CPU path")
@@ -100,7 +105,7 @@ class TokenLM:
         self.vocab, self.max_slots = config.vocab, int(max_slots)
         self.max_positions = config.max_positions              # longest sequence; 0: the pool alone bounds it
         self.max_step_tokens = int(max_step_tokens or max_tokens)
-        cfg, keep_layers = _cfg_struct(config, dtype)
+        cfg, keep_layers = _cfg_struct(config, dtype, kv_cache)
         state = {k: (v if v.dtype == torch.int32 else v.to(torch.bfloat16)).to(self.device) for k, v in state_dict.items()}
         descs, keep = _capi.tensor_descs(state)
         with _capi.device_scope(self.device):

@@ -1,0 +1,85 @@
+"""The token language models' operators on the kernel simulator: the cases of tests/operator_cases.py."""
+import pytest
+
+from tests import operator_cases as oc
+from tests.test_tlm_sim import tlm_lib  # noqa: F401  (fixture)
+
+DEV = "cpu"
+
+
+@pytest.mark.parametrize("name", sorted(oc.APPENDS))
+def test_append(tlm_lib, name):  # noqa: F811
+    oc.check_append(name, DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name", ["single_tokens", "portions", "rotated_part_of_odd_sizes"])
+def test_append_unaligned(tlm_lib, name):  # noqa: F811
+    oc.check_append(name, DEV, tlm_lib, strided=True)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_append_in_any_order(tlm_lib, codes):  # noqa: F811
+    oc.check_append_order(DEV, tlm_lib, codes)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_not_finite(tlm_lib, codes):  # noqa: F811
+    oc.check_not_finite(DEV, tlm_lib, codes)
+
+
+@pytest.mark.parametrize("name", sorted(oc.ATTENDS))
+def test_attend(tlm_lib, name):  # noqa: F811
+    oc.check_attend(name, DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name", ["single_fp32", "rotated", "portions"])
+def test_attend_unaligned(tlm_lib, name):  # noqa: F811
+    oc.check_attend(name, DEV, tlm_lib, strided=True)
+
+
+def test_extreme_scores(tlm_lib):  # noqa: F811
+    oc.check_extreme_scores(DEV, tlm_lib)
+
+
+def test_refusals(tlm_lib):  # noqa: F811
+    oc.check_refusals(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name", sorted(oc.SELECTS))
+def test_select(tlm_lib, name):  # noqa: F811
+    oc.check_select(name, DEV, tlm_lib)
+
+
+def test_select_refusals(tlm_lib):  # noqa: F811
+    oc.check_select_refusals(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("beams", [1, 3, 8, 13, 32])
+def test_reorder(tlm_lib, beams):  # noqa: F811
+    oc.check_reorder(DEV, tlm_lib, beams)
+
+
+def test_reorder_refusals(tlm_lib):  # noqa: F811
+    oc.check_reorder_refusals(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("name", ["grouped_attention", "grouped_attention_own_heads", "grouped_attention_wide", "grouped_attention_keeps_more_than_it_sees", "bibapel"])
+def test_token_lm(tlm_lib, name, codes):  # noqa: F811
+    oc.check_token_lm(name, DEV, tlm_lib, oc.F32, codes)
+
+
+def test_token_lm_bf16(tlm_lib):  # noqa: F811
+    oc.check_token_lm("grouped_attention", DEV, tlm_lib, oc.BF16, "int8")
+
+
+def test_token_lm_longer_than_its_pool(tlm_lib):  # noqa: F811
+    oc.check_token_lm("two_kept_windows", DEV, tlm_lib, oc.F32, "int8", n=330, cut_sets=((130, 1),), max_slots=2, max_tokens=320)
+
+
+def test_token_lm_batch(tlm_lib):  # noqa: F811
+    oc.check_token_lm_batch(DEV, tlm_lib, oc.F32, "int8")
+
+
+def test_token_lm_refusals(tlm_lib):  # noqa: F811
+    oc.check_token_lm_refusals(DEV, tlm_lib)
