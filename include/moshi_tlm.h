@@ -83,6 +83,11 @@ int mmi_tlm_close(mmi_tlm* m, int32_t slot);
  * (device fp32 [n_want][vocab]).  MMI_ERR_BUSY, with nothing changed, when the pool has too few free pages. */
 int mmi_tlm_step(mmi_tlm* m, int32_t n_entries, const int32_t* slots, const int32_t* counts, const int32_t* tokens, int32_t n_want,
                  const int32_t* want, float* logits, mmi_stream stream);
+/* Beams: in each of `groups` groups of `beams` <= 32 open sequences (slots, host [groups][beams], each slot at most once) the sequence in place i
+ * becomes a copy of what the one in place parents[i] (host, 0 .. beams - 1) was: tokens, position, cache and recurrent state.  Full pages are
+ * shared; only the last page, where there is room in it, and the states are copied.  MMI_ERR_BUSY, with nothing changed, when the pool has too few
+ * free pages for the copies. */
+int mmi_tlm_reorder(mmi_tlm* m, int32_t groups, int32_t beams, const int32_t* slots, const int32_t* parents, mmi_stream stream);
 /* Draw one token per row of device fp32 logits [n][vocab]; row i belongs to slot slots[i] and uses temp[i] / top_k[i] (temp <= 0:
  * greedy).  out: device int32 [n]. */
 int mmi_tlm_sample(mmi_tlm* m, int32_t n, const float* logits, const int32_t* slots, const float* temp, const int32_t* top_k, uint64_t seed,

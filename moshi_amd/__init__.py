@@ -9,6 +9,9 @@ from .lm import ConditionFuser, LMGen, LMModel  # noqa: F401
 from .batcher import SessionBatcher  # noqa: F401
 from .tlm import TokenLM  # noqa: F401
 from .token_batcher import TokenBatcher  # noqa: F401
+from .kv_cache import PagedKVCache  # noqa: F401
+from .beam import BeamChoice, BeamHypothesis, beam_reorder, beam_search, beam_select  # noqa: F401
 
 __all__ = ["MimiConfig", "LMConfig", "MimiModel", "LMModel", "LMGen", "ConditionFuser", "SessionBatcher",
-           "tiny_mimi_config", "tiny_lm_config", "TokenLM", "TokenLMConfig", "TokenBatcher", "tiny_token_lm_config"]
+           "tiny_mimi_config", "tiny_lm_config", "TokenLM", "TokenLMConfig", "TokenBatcher", "tiny_token_lm_config",
+           "PagedKVCache", "BeamChoice", "BeamHypothesis", "beam_reorder", "beam_search", "beam_select"]

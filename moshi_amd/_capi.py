@@ -199,6 +199,7 @@ TLM_SIGNATURES = {
     "mmi_tlm_open": (C.c_int, [_P, C.POINTER(C.c_int32)]),
     "mmi_tlm_close": (C.c_int, [_P, C.c_int32]),
     "mmi_tlm_step": (C.c_int, [_P, C.c_int32, _P, _P, _P, C.c_int32, _P, _P, _P]),
+    "mmi_tlm_reorder": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, _P]),
     "mmi_tlm_sample": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, C.c_uint64, _P, _P]),
     "mmi_tlm_info": (C.c_int64, [_P, C.c_int32, C.c_int32]),
     "mmi_tlm_pages_needed": (C.c_int64, [_P, C.c_int32, C.c_int64]),

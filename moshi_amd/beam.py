@@ -1,18 +1,21 @@
 """Beam search on the device: the choice over beams and vocabulary (`beam_select`) and the beams' states moved to where their children are
-(`beam_reorder`); libmoshi_tlm.so, include/moshi_tlm.h.
+(`beam_reorder`); libmoshi_tlm.so, include/moshi_tlm.h.  `beam_search` runs them over a `TokenLM`.
 
     r = beam_select(logits, scores, lengths=lengths, finished=finished, eos=2, length_penalty=0.6)
     beam_reorder([state, history], r.parents)                 # row b * beams + i: what row b * beams + r.parents[b, i] was
+
+    best = beam_search(lm, prompts, beams=4, max_new_tokens=64, eos=2)[0][0].tokens
 """
 from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import Dict, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _capi
+from .tlm import TokenLM
 
 _DTYPES = {torch.bfloat16: _capi.MMI_BF16, torch.float32: _capi.MMI_F32}
 
@@ -111,3 +114,131 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, lib: Opt
             stride.append(t.stride(0) * t.element_size())
     n = len(at)
     lib.check(on.call(lib.mmi_beam_reorder, n, (C.c_void_p * n)(*at), (C.c_int64 * n)(*stride), (C.c_int64 * n)(*size), batch, beams, parents.data_ptr()))
+
+
+@dataclass
+class BeamHypothesis:
+    tokens: List[int]                    # what follows the prompt, an end token included
+    score: float                         # sum of their log probabilities
+
+
+def beam_pages(lm_pages, prompt: int, beams: int, max_new_tokens: int, page: int) -> int:
+    """Cache pages that one request's search may come to hold; lm_pages(n): pages of a sequence of n tokens.  The beams share the prompt's full pages."""
+    total = lm_pages(prompt + max_new_tokens - 1)
+    shared = min(total, prompt // page)
+    return shared + beams * (total - shared)
+
+
+@torch.no_grad()
+def beam_search(lm: TokenLM, prompts: Sequence[Sequence[int]], beams: int = 4, max_new_tokens: int = 64, eos: int = -1, length_penalty: float = 0.0,
+                step_tokens: int = 2048) -> List[List[BeamHypothesis]]:
+    """For every prompt the `beams` continuations that the search ends with, best first (by score / length ** length_penalty).  A search ends when
+    all its beams have ended with `eos` (-1: no end token), or after max_new_tokens.
+
+    As many prompts run together as the model's slots (`beams` each), its pages and `step_tokens` allow.  BufferError when not even one does.
+    """
+    prompts = [[int(t) for t in p] for p in prompts]
+    if beams < 1 or max_new_tokens < 1 or any(not p for p in prompts):
+        raise ValueError("a search needs a beam, a prompt and at least one new token")
+    if not -1 <= eos < lm.vocab:
+        raise ValueError("the end token is outside the vocabulary")
+    if any(t < 0 or t >= lm.vocab for p in prompts for t in p):
+        raise ValueError("token outside the vocabulary")
+    for p in prompts:
+        if lm.max_positions and len(p) + max_new_tokens - 1 > lm.max_positions:
+            raise ValueError(f"the request reaches position {len(p) + max_new_tokens - 1}, the model has {lm.max_positions}")
+    step_tokens = min(int(step_tokens), lm.max_step_tokens)
+    need = [beam_pages(lambda n: lm.pages_needed(-1, n), len(p), beams, max_new_tokens, lm.page_tokens) for p in prompts]
+    out: List[List[BeamHypothesis]] = []
+    while len(out) < len(prompts):
+        first, room = len(out), min(lm.free_slots, step_tokens) // beams
+        n, pages = first, lm.free_pages
+        while n < len(prompts) and n - first < room and need[n] <= pages:
+            pages -= need[n]
+            n += 1
+        if n == first:
+            raise BufferError(f"the search needs {beams} slots, {need[n]} pages and {beams} tokens a step; there are {lm.free_slots}, {lm.free_pages} and {step_tokens}")
+        out += _search(lm, prompts[first:n], beams, max_new_tokens, eos, length_penalty, step_tokens)
+    return out
+
+
+def _prefill(lm: TokenLM, prompts: List[List[int]], slots: List[int], step_tokens: int) -> torch.Tensor:
+    """Logits behind every prompt, [prompts, vocab]."""
+    logits, entries, budget = torch.empty((len(prompts), lm.vocab), dtype=_F32, device=lm.device), [], step_tokens
+    done = 0
+
+    def run():
+        nonlocal entries, budget, done
+        n = sum(len(w) for _, _, w in entries)
+        if n:
+            lm.step(entries, out=logits[done:done + n])
+        else:
+            lm.step(entries)
+        entries, budget, done = [], step_tokens, done + n
+
+    for prompt, slot in zip(prompts, slots):
+        fed = 0
+        while fed < len(prompt):
+            take = min(budget, len(prompt) - fed)
+            fed += take
+            budget -= take
+            entries.append((slot, prompt[fed - take:fed], [take - 1] if fed == len(prompt) else []))
+            if not budget:
+                run()
+    if entries:
+        run()
+    return logits
+
+
+def _search(lm: TokenLM, prompts: List[List[int]], beams: int, max_new_tokens: int, eos: int, length_penalty: float, step_tokens: int) -> List[List[BeamHypothesis]]:
+    device, opened = lm.device, []
+    result: List[List[BeamHypothesis]] = [[] for _ in prompts]
+    try:
+        for _ in range(len(prompts) * beams):
+            opened.append(lm.open())
+        slots = [opened[i:i + beams] for i in range(0, len(opened), beams)]
+        live = list(range(len(prompts)))
+        trace: List[List[Tuple[List[int], List[int]]]] = [[] for _ in prompts]      # parents and tokens of every step
+        logits = _prefill(lm, prompts, [s[0] for s in slots], step_tokens).repeat_interleave(beams, dim=0)
+        scores = torch.full((len(prompts), beams), float("-inf"), device=device)
+        scores[:, 0] = 0.0
+        lengths = torch.zeros((len(prompts), beams), dtype=_I32, device=device)
+        finished = None
+        while True:
+            r = beam_select(logits, scores, lengths, finished, eos, length_penalty, lib=lm._lib)
+            scores, lengths, finished = r.scores, r.lengths, r.finished
+            parents, tokens, size, ended = torch.stack([r.parents, r.tokens, lengths, lengths.new_zeros(lengths.shape) if finished is None else finished.int()]).tolist()
+            for i, p, t in zip(live, parents, tokens):
+                trace[i].append((p, t))
+            last = len(trace[live[0]]) == max_new_tokens
+            stay = [] if last else [j for j in range(len(live)) if not all(ended[j])]
+            if len(stay) < len(live):
+                sums = scores.tolist()
+                for j in set(range(len(live))).difference(stay):
+                    result[live[j]] = _hypotheses(trace[live[j]], sums[j], size[j])
+                    for s in slots[j]:
+                        lm.close(s)
+                        opened.remove(s)
+                if not stay:
+                    return result
+                at = torch.tensor(stay, device=device)
+                scores, lengths, finished = scores[at], lengths[at], None if finished is None else finished[at]
+                live, slots, parents, tokens = ([x[j] for j in stay] for x in (live, slots, parents, tokens))
+            lm.reorder(slots, parents)
+            logits = lm.step([(s, [t], [0]) for row, toks in zip(slots, tokens) for s, t in zip(row, toks)])
+    finally:
+        for s in opened:
+            lm.close(s)
+
+
+def _hypotheses(trace: List[Tuple[List[int], List[int]]], sums: List[float], size: List[int]) -> List[BeamHypothesis]:
+    out = []
+    for i, (score, n) in enumerate(zip(sums, size)):
+        if score == float("-inf"):
+            continue
+        back, tokens = i, []
+        for parents, toks in reversed(trace):
+            tokens.append(toks[back])
+            back = parents[back]
+        out.append(BeamHypothesis(tokens[::-1][:n], score))
+    return out

@@ -8,7 +8,7 @@
 #pragma once
 #include "tlm_common.h"
 
-constexpr int BEAM_MAX = 32, BEAM_CHUNK = 1024, BEAM_TENSORS = 48;
+constexpr int BEAM_CHUNK = 1024, BEAM_TENSORS = 48;
 
 struct TlmBeamArgs {
     const void* x; long ld;              // logits, row stride in elements

@@ -148,6 +148,8 @@ struct mmi_tlm {
     // host state
     std::vector<Slot> slots;
     std::vector<int> free_pages;
+    std::vector<int> page_refs;    // sequences that hold a page: beams share what they have in common
+    std::vector<TlmReorderTensor> page_rows, slot_rows;      // what a page, and what a slot, holds on the device
     Staging staging[4];
     int stage_at = 0;
     size_t meta_cap = 0;
@@ -617,6 +619,10 @@ int alloc_f32(mmi_tlm* m, float** p, size_t n) {
 
 int table_ld(const mmi_tlm* m) { return m->keep_pages + std::max(1, m->max_pages); }      // block-table entries per slot
 
+int64_t table_column(const mmi_tlm* m, int64_t page) {      // where a slot's row of the table names the page
+    return page < m->keep_pages ? page : m->keep_pages + (page - m->keep_pages) % std::max(1, m->max_pages);
+}
+
 int alloc_buffers(mmi_tlm* m) {
     const mmi_tlm_cfg& c = m->cfg;
     const int T = m->max_T;
@@ -750,19 +756,28 @@ int alloc_buffers(mmi_tlm* m) {
 }
 
 int alloc_state(mmi_tlm* m) {
+    auto rows = [](std::vector<TlmReorderTensor>& to, void* p, size_t total, int n) {
+        if (p) to.push_back(TlmReorderTensor{p, (int64_t)(total / n), (int64_t)(total / n)});
+    };
+    auto pages = [&](void* p, size_t total) { rows(m->page_rows, p, total, m->max_pages); };
+    auto per_slot = [&](void* p, size_t total) { rows(m->slot_rows, p, total, m->max_slots); };
+    m->page_refs.assign(m->max_pages, 0);
     for (Run& r : m->runs) {
         const Layer& L = m->layers[r.layer];
         if (L.c.mixer == MMI_TLM_MIX_MINGRU) {
             const size_t n = (size_t)m->max_slots * 2 * L.wp;
             MMI_HIP_CHECK(m->st.alloc(&r.state, n));
             MMI_HIP_CHECK(hipMemset(r.state, 0, n * sizeof(float)));
+            per_slot(r.state, n * sizeof(float));
         } else if (L.linear()) {
             const size_t n = (size_t)m->max_slots * L.c.heads * L.dim_p * L.vdim_p, nc = (size_t)m->max_slots * 2 * std::max(1, L.c.conv - 1) * std::max(1, L.conv_c);
             MMI_HIP_CHECK(m->st.alloc(&r.state, n));
             MMI_HIP_CHECK(hipMemset(r.state, 0, n * sizeof(float)));
+            per_slot(r.state, n * sizeof(float));
             if (L.conv_c) {
                 MMI_HIP_CHECK(m->st.alloc(&r.conv, nc));
                 MMI_HIP_CHECK(hipMemset(r.conv, 0, nc * sizeof(float)));
+                per_slot(r.conv, nc * sizeof(float));
             }
         } else if (L.c.mixer == MMI_TLM_MIX_ATTENTION && m->cfg.cache) {
             const size_t units = (size_t)m->max_pages * L.c.kv_heads, nk = units * TLM_PAGE * L.dim_p, nv = units * TLM_PAGE * L.vdim_p;
@@ -774,9 +789,12 @@ int alloc_state(mmi_tlm* m) {
             for (float** p : {&r.ks, &r.vs}) {
                 MMI_HIP_CHECK(m->st.alloc(p, units * KV8_PARTS));
                 MMI_HIP_CHECK(hipMemset(*p, 0, units * KV8_PARTS * sizeof(float)));
+                pages(*p, units * KV8_PARTS * sizeof(float));
             }
             r.kc = k;
             r.vc = v;
+            pages(k, nk);
+            pages(v, nv);
         } else if (L.c.mixer == MMI_TLM_MIX_ATTENTION) {
             const size_t nk = (size_t)m->max_pages * L.c.kv_heads * 4 * L.k_ks * 64, nv = (size_t)m->max_pages * L.c.kv_heads * (TLM_PAGE / m->kstep) * L.nd * 64;
             u32x4 *k = nullptr, *v = nullptr;
@@ -786,12 +804,15 @@ int alloc_state(mmi_tlm* m) {
             MMI_HIP_CHECK(hipMemset(v, 0, nv * 16));
             r.kc = k;
             r.vc = v;
+            pages(k, nk * 16);
+            pages(v, nv * 16);
         } else {
             const size_t nk = (size_t)m->max_pages * 4 * L.k_ks * 64;
             u32x4* k = nullptr;
             MMI_HIP_CHECK(m->st.alloc(&k, nk));
             MMI_HIP_CHECK(hipMemset(k, 0, nk * 16));      // masked keys of a block are multiplied by zero weights: never-written rows must be finite
             r.kc = k;
+            pages(k, nk * 16);
         }
     }
     return MMI_OK;
@@ -1895,19 +1916,22 @@ int64_t pages_for(const mmi_tlm* m, const Slot* s, int64_t n) {
     const int64_t have = s ? s->first_page + (int64_t)s->pages.size() : 0;
     return std::max<int64_t>(0, (pos + n + TLM_PAGE - 1) / TLM_PAGE - have);
 }
+void let_page_go(mmi_tlm* m, int page) {
+    if (--m->page_refs[page] == 0) m->free_pages.push_back(page);
+}
 void release_behind_window(mmi_tlm* m, Slot& s) {
     if (!m->has_attn || m->max_window <= 0) return;
     const int64_t first_seen = s.pos - m->max_window + 1;               // the oldest position the next token can see
     while (!s.pages.empty() && (s.first_page + 1) * TLM_PAGE <= first_seen) {
         if (s.first_page < m->keep_pages) s.kept.push_back(s.pages.front());
-        else m->free_pages.push_back(s.pages.front());
+        else let_page_go(m, s.pages.front());
         s.pages.erase(s.pages.begin());
         ++s.first_page;
     }
 }
 void release_slot(mmi_tlm* m, Slot& s) {
-    for (int p : s.kept) m->free_pages.push_back(p);
-    for (int p : s.pages) m->free_pages.push_back(p);
+    for (int p : s.kept) let_page_go(m, p);
+    for (int p : s.pages) let_page_go(m, p);
     s = Slot();
 }
 
@@ -2029,6 +2053,8 @@ int create_impl(mmi_tlm* m, const mmi_tensor_desc* weights, int n_weights) {
     m->slots.resize(m->max_slots);
     for (int i = m->max_pages - 1; i >= 0; --i) m->free_pages.push_back(i);
     if ((rc = alloc_state(m)) || (rc = alloc_buffers(m))) return rc;
+    m->slot_rows.push_back(TlmReorderTensor{m->last_tok, sizeof(int), sizeof(int)});
+    if (m->prev_tok) m->slot_rows.push_back(TlmReorderTensor{m->prev_tok, 2 * sizeof(int), 2 * sizeof(int)});
     m->graphs = mmi_graphs_enabled();
     m->say_forms = getenv("MMI_TLM_FORMS") != nullptr;
     if (const char* h = getenv("MMI_TLM_WIDE")) m->force_wide = std::min(256, std::max(32, atoi(h) / 32 * 32));
@@ -2206,8 +2232,8 @@ extern "C" int mmi_tlm_step(mmi_tlm* m, int32_t n_entries, const int32_t* slots,
         for (int64_t n = pages_for(m, &S, counts[e]); n > 0; --n) {
             const int page = m->free_pages.back();
             m->free_pages.pop_back();
-            const int64_t at_page = S.first_page + (int64_t)S.pages.size();
-            const int64_t idx = (int64_t)slots[e] * table_ld(m) + (at_page < m->keep_pages ? at_page : m->keep_pages + (at_page - m->keep_pages) % std::max(1, m->max_pages));
+            m->page_refs[page] = 1;
+            const int64_t idx = (int64_t)slots[e] * table_ld(m) + table_column(m, S.first_page + (int64_t)S.pages.size());
             S.pages.push_back(page);
             b[M.upd + 2 * upd] = (int)idx;
             b[M.upd + 2 * upd + 1] = page;
@@ -2353,5 +2379,96 @@ extern "C" int mmi_tlm_sample(mmi_tlm* m, int32_t n, const float* logits, const 
         MMI_CHECK_LAUNCH();
         i = k;
     }
+    return MMI_OK;
+}
+
+extern "C" int mmi_tlm_reorder(mmi_tlm* m, int32_t groups, int32_t beams, const int32_t* slots, const int32_t* parents, mmi_stream stream) {
+    if (!m || groups < 0 || beams < 1 || (groups && (!slots || !parents))) return mmi_fail(MMI_ERR_INVALID, "mmi_tlm_reorder: bad arguments");
+    if (beams > BEAM_MAX) return mmi_fail(MMI_ERR_UNSUPPORTED, "mmi_tlm_reorder: more beams than a group may have");
+    const int64_t n64 = (int64_t)groups * beams;
+    if (n64 > m->max_slots) return mmi_fail(MMI_ERR_SHAPE, "more sequences than slots");
+    const int n = (int)n64;
+    std::vector<char> seen(m->max_slots, 0);
+    bool moved = false;
+    for (int i = 0; i < n; ++i) {
+        if (slots[i] < 0 || slots[i] >= m->max_slots || !m->slots[slots[i]].live) return mmi_fail(MMI_ERR_NO_CHANNEL, "no open sequence in this slot");
+        if (seen[slots[i]]++) return mmi_fail(MMI_ERR_INVALID, "a slot appears twice");
+        if (parents[i] < 0 || parents[i] >= beams) return mmi_fail(MMI_ERR_INVALID, "a parent outside its group");
+        moved |= parents[i] != i % beams;
+    }
+    if (!moved) return MMI_OK;
+    MmiDeviceGuard guard(m->device);
+    hipStream_t s = (hipStream_t)stream;
+    Staging& st = m->staging[m->stage_at];
+    m->stage_at = (m->stage_at + 1) & 3;
+    if (st.used) MMI_HIP_CHECK(hipEventSynchronize(st.ev));
+    // Pages that are full are only read from now on: the children of a sequence share them.  The last one, if a part of it is free, is written by
+    // every child: one keeps it (the sequence itself, where it lives on), the others get copies.
+    std::vector<Slot> next(n);
+    std::vector<int> row(n, 0), copy_of(n, -1), keeper(n, -1);      // last page, the child of the group whose page it is a copy of; per old sequence its first child
+    for (int i = 0; i < n; ++i)
+        if (parents[i] == i % beams) keeper[i] = i;
+    int64_t lack = 0, columns = 0;
+    for (int i = 0; i < n; ++i) {
+        const int from = i - i % beams + parents[i];
+        const Slot& P = next[i] = m->slots[slots[from]];
+        for (int p : P.kept) ++m->page_refs[p];
+        for (int p : P.pages) ++m->page_refs[p];
+        const int64_t last = P.first_page + (int64_t)P.pages.size();
+        columns = std::max(columns, last <= table_ld(m) ? last : table_ld(m));
+        if (P.pos % TLM_PAGE == 0 || P.pages.empty()) continue;
+        if (keeper[from] < 0) keeper[from] = i;
+        copy_of[i] = keeper[from] % beams;
+        row[i] = P.pages.back();
+        if (keeper[from] != i) {
+            --m->page_refs[P.pages.back()];
+            next[i].pages.back() = -1;
+            ++lack;
+        }
+    }
+    std::vector<int> freed;
+    auto drop = [&](int p) {
+        if (--m->page_refs[p] == 0) freed.push_back(p);
+    };
+    for (int i = 0; i < n; ++i) {
+        for (int p : m->slots[slots[i]].kept) drop(p);
+        for (int p : m->slots[slots[i]].pages) drop(p);
+    }
+    if (lack > (int64_t)(m->free_pages.size() + freed.size())) {      // as it was
+        for (int i = 0; i < n; ++i) {
+            for (int p : m->slots[slots[i]].kept) ++m->page_refs[p];
+            for (int p : m->slots[slots[i]].pages) ++m->page_refs[p];
+            for (int p : next[i].kept) --m->page_refs[p];
+            for (int p : next[i].pages)
+                if (p >= 0) --m->page_refs[p];
+        }
+        return mmi_fail(MMI_ERR_BUSY, "the cache pool has too few free pages");
+    }
+    m->free_pages.insert(m->free_pages.end(), freed.begin(), freed.end());
+    int *b = st.host, updates = 0;
+    memcpy(b, slots, n * sizeof(int));
+    memcpy(b + n, parents, n * sizeof(int));
+    for (int i = 0; i < n; ++i) {
+        if (!next[i].pages.empty() && next[i].pages.back() < 0) {
+            row[i] = next[i].pages.back() = m->free_pages.back();
+            m->free_pages.pop_back();
+            m->page_refs[row[i]] = 1;
+            b[4 * n + 2 * updates] = (int)((int64_t)slots[i] * table_ld(m) + table_column(m, next[i].first_page + (int64_t)next[i].pages.size() - 1));
+            b[4 * n + 2 * updates++ + 1] = row[i];
+        }
+        b[2 * n + i] = row[i];
+        b[3 * n + i] = copy_of[i];
+    }
+    for (int i = 0; i < n; ++i) m->slots[slots[i]] = std::move(next[i]);
+    MMI_HIP_CHECK(hipMemcpyAsync(m->meta, b, (size_t)(4 * n + 2 * updates) * sizeof(int), hipMemcpyHostToDevice, s));
+    MMI_HIP_CHECK(hipEventRecord(st.ev, s));
+    st.used = true;
+    int rc = updates ? tlm_reorder(s, (int)m->page_rows.size(), m->page_rows.data(), groups, beams, m->meta + 3 * n, m->meta + 2 * n) : MMI_OK;
+    if (rc) return rc;
+    std::vector<TlmReorderTensor> rows = m->slot_rows;
+    if (columns) rows.push_back(TlmReorderTensor{m->block_table, table_ld(m) * (int64_t)sizeof(int), columns * (int64_t)sizeof(int)});
+    if ((rc = tlm_reorder(s, (int)rows.size(), rows.data(), groups, beams, m->meta + n, m->meta))) return rc;
+    if (updates) MMI_LAUNCH(k_tlm_table, mmi_cdiv(updates, 256), 256, 0, s, m->meta + 4 * n, updates, m->block_table);
+    MMI_CHECK_LAUNCH();
     return MMI_OK;
 }

@@ -89,6 +89,10 @@ struct TlmPrepArgs {
     int* prev_tok;            // [slots][2]: a step reads one copy and writes the other
     int* brow;                // out: row of the bigram table
 };
+__global__ void k_tlm_table(const int* updates, int n, int* block_table) {
+    const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
+    if (i < n) block_table[updates[2 * i]] = updates[2 * i + 1];
+}
 __global__ void k_tlm_prepare(TlmPrepArgs a) {
     const int i0 = (int)(blockIdx.x * blockDim.x + threadIdx.x), n = (int)(gridDim.x * blockDim.x);
     for (int i = i0; i < *a.n_updates; i += n) a.block_table[a.updates[2 * i]] = a.updates[2 * i + 1];

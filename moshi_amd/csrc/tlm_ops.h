@@ -11,5 +11,6 @@ void tlm_kv8_workspace(TlmKv8Attn& a, float* workspace);      // aligned to 16 b
 int tlm_kv8_attend(hipStream_t s, const TlmKv8Attn& a, int dtype, bool f32);
 
 // rows of several tensors; row r of a group of `beams` becomes a copy of what row parent[r] of it was (row: where the groups' rows are, null: in order)
+constexpr int BEAM_MAX = 32;
 struct TlmReorderTensor { void* p; int64_t stride, bytes; };
 int tlm_reorder(hipStream_t s, int n, const TlmReorderTensor* tensors, int groups, int beams, const int* parent, const int* row);

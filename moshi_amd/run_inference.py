@@ -147,6 +147,7 @@ def write_wav(path: str, pcm: np.ndarray, sample_rate: int) -> None:
 
 
 def run_token_lm(args) -> None:
+    from .beam import beam_pages, beam_search
     from .token_batcher import TokenBatcher
 
     def lines(path):
@@ -155,14 +156,21 @@ def run_token_lm(args) -> None:
     prompts = lines(args.infile)
     dtype = torch.float32 if args.dtype == "float32" else torch.bfloat16
     pages = lambda n: -(-n // 64) * 64
-    pool = sum(sorted((pages(len(p) + args.max_new_tokens) for p in prompts), reverse=True)[:args.batch_size])
+    if args.beams > 1 and len(args.stop_token) > 1:
+        raise SystemExit("--beams takes one --stop-token")
+    held = lambda p: beam_pages(lambda n: pages(n) // 64, len(p), args.beams, args.max_new_tokens + 1, 64) * 64
+    pool = sum(sorted((held(p) for p in prompts), reverse=True)[:args.batch_size])
     step_tokens = min(args.step_tokens, pool)
     log("info", f"loading {args.checkpoint_dir}")
-    lm = loaders.get_token_lm(args.checkpoint_dir, device=args.device, dtype=dtype, max_slots=args.batch_size, max_tokens=pool, max_step_tokens=step_tokens,
+    lm = loaders.get_token_lm(args.checkpoint_dir, device=args.device, dtype=dtype, max_slots=args.batch_size * args.beams, max_tokens=pool, max_step_tokens=step_tokens,
                                kv_cache=None if args.kv_cache == "like-dtype" else args.kv_cache)
-    batcher = TokenBatcher(lm, step_tokens=step_tokens, seed=args.seed)
     t0 = time.time()
-    out = batcher.generate(prompts, args.max_new_tokens, temp=0.0 if args.greedy else args.temp, top_k=args.top_k, stop=args.stop_token)
+    if args.beams > 1:
+        eos = args.stop_token[0] if args.stop_token else -1
+        out = [h[0].tokens for h in beam_search(lm, prompts, args.beams, args.max_new_tokens, eos, args.length_penalty, step_tokens)]
+    else:
+        out = TokenBatcher(lm, step_tokens=step_tokens, seed=args.seed).generate(prompts, args.max_new_tokens, temp=0.0 if args.greedy else args.temp, top_k=args.top_k,
+                                                                                 stop=args.stop_token)
     dt = time.time() - t0
     log("info", f"{len(prompts)} requests, {sum(len(p) for p in prompts)} prompt + {sum(len(o) for o in out)} new tokens in {dt:.2f}s")
     text = "".join(" ".join(str(t) for t in o) + "\n" for o in out)
@@ -192,6 +200,8 @@ def main(argv: Optional[List[str]] = None) -> None:
     tok.add_argument("--stop-token", type=int, action="append", default=[], help="end a continuation after this token (repeatable)")
     tok.add_argument("--step-tokens", type=int, default=2048, help="most tokens of one batch: prompts are cut into portions of it")
     tok.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    tok.add_argument("--beams", type=int, default=1, help="more than 1: beam search in place of sampling")
+    tok.add_argument("--length-penalty", type=float, default=0.0, help="beams are ranked by score / length ** this")
     tok.add_argument("--kv-cache", choices=["like-dtype", "int8", "e4m3"], default="like-dtype", help="what grouped attention's keys and values are held in")
     ap.add_argument("infile", type=str)
     ap.add_argument("outfile", type=str)

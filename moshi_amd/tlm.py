@@ -200,6 +200,15 @@ class TokenLM:
                                                  out.data_ptr(), _capi.stream_ptr(self.device)))
         return out
 
+    def reorder(self, slots: Sequence[Sequence[int]], parents: Sequence[Sequence[int]]) -> None:
+        """Beams: slots [groups][beams], parents [groups][beams] of places in the group; the sequence in slots[g][i] becomes a copy of what the one
+        in slots[g][parents[g][i]] was.  Full cache pages are shared.  BufferError, with nothing changed, when the pool has too few free pages."""
+        groups, beams = len(slots), len(slots[0]) if len(slots) else 1
+        if len(parents) != groups or any(len(r) != beams for r in (*slots, *parents)):
+            raise ValueError("slots and parents are [groups][beams]")
+        self._lib.check(self._lib.mmi_tlm_reorder(self._handle, groups, beams, _i32([int(s) for r in slots for s in r]), _i32([int(p) for r in parents for p in r]),
+                                                  _capi.stream_ptr(self.device)))
+
     # ---- diagnostics -----------------------------------------------------------------------------------------------
     def step_with_taps(self, entries: Sequence[Entry]) -> Tuple[torch.Tensor, torch.Tensor]:
         """`step`, and the residual stream after every layer run: fp32 [layer runs, tokens, width]."""

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from moshi_amd.beam import beam_reorder, beam_select
+from moshi_amd.beam import beam_reorder, beam_search, beam_select
 from moshi_amd.kv_cache import PagedKVCache
 
 F32, BF16 = torch.float32, torch.bfloat16
@@ -728,3 +728,175 @@ def check_token_lm_refusals(dev, lib):
         TokenLM(random_token_lm_state_dict(cfg, seed=1), cfg, device=dev, lib=lib, kv_cache="int8")
     with pytest.raises(ValueError):
         TokenLM({}, tc.MECHANISMS["grouped_attention"], device=dev, lib=lib, kv_cache="int4")
+
+
+# ---- beams --------------------------------------------------------------------------------------------------------------------
+def check_token_lm_reorder(name, dev, lib, dtype=F32, codes=None, lengths=((20, 64, 1, 130, 63), (65, 7, 90, 90, 128)), tail=70):
+    """Sequences that became copies of others, against sequences that had those tokens from the start: the same batches, so the same bits."""
+    cfg = tc.MECHANISMS[name]
+    sd = random_token_lm_state_dict(cfg, seed=5)
+    beams, parents = 5, [[[3, 1, 1, 0, 3], [2, 2, 2, 2, 2]], [[0, 0, 4, 4, 1], [4, 3, 2, 1, 0]]]
+    seqs = [[tc.tokens_of(cfg, n, seed=9 * g + i) for i, n in enumerate(row)] for g, row in enumerate(lengths)]
+    a, b = (TokenLM(sd, cfg, device=dev, dtype=dtype, lib=lib, kv_cache=codes, max_slots=11, max_tokens=64 * 60) for _ in range(2))
+    a.open()                                               # (slots need not start at the first)
+    sa, sb = ([[m.open() for _ in range(beams)] for _ in range(2)] for m in (a, b))
+    rng = np.random.default_rng(1)
+    for g in range(2):
+        for i in range(beams):
+            a.step([(sa[g][i], seqs[g][i], [])])
+    at = parents[0]
+    a.reorder(sa, at)
+    for g in range(2):
+        for i in range(beams):
+            b.step([(sb[g][i], seqs[g][at[g][i]], [])])
+    fed = [[[] for _ in range(beams)] for _ in range(2)]
+
+    def step_both():
+        toks = rng.integers(0, cfg.vocab, (2, beams)).tolist()
+        ya, yb = (m.step([(s[g][i], [toks[g][i]], [0]) for g in range(2) for i in range(beams)]) for m, s in ((a, sa), (b, sb)))
+        assert torch.equal(ya, yb)
+        for g in range(2):
+            for i in range(beams):
+                fed[g][i].append(toks[g][i])
+
+    for _ in range(tail):
+        step_both()
+    assert [[a.position(s) for s in row] for row in sa] == [[b.position(s) for s in row] for row in sb]
+    # and again: b's sequences step by step, in batches like the first ones
+    a.reorder(sa, parents[1])
+    for row in sb:
+        for s in row:
+            b.close(s)
+    sb = [[b.open() for _ in range(beams)] for _ in range(2)]
+    src = [[at[g][parents[1][g][i]] for i in range(beams)] for g in range(2)]
+    for g in range(2):
+        for i in range(beams):
+            b.step([(sb[g][i], seqs[g][src[g][i]], [])])
+    for n in range(tail):
+        b.step([(sb[g][i], [fed[g][parents[1][g][i]][n]], [0]) for g in range(2) for i in range(beams)])
+    for _ in range(3):
+        step_both()
+    a.reorder(sa, [list(range(beams))] * 2)                # nothing moves
+    step_both()
+    for m, s in ((a, sa), (b, sb)):
+        for row in s:
+            for slot in row:
+                m.close(slot)
+        assert m.free_pages == m.total_pages
+
+
+def check_token_lm_reorder_pool(dev, lib):
+    """Shared pages are counted once, given back with their last holder, and a reordering that the pool cannot hold leaves everything as it was."""
+    cfg = tc.MECHANISMS["grouped_attention_no_window"]
+    sd = random_token_lm_state_dict(cfg, seed=5)
+    lm = TokenLM(sd, cfg, device=dev, dtype=F32, lib=lib, max_slots=5, max_tokens=64 * 6)
+    s = [lm.open() for _ in range(4)]
+    toks = tc.tokens_of(cfg, 200)
+    lm.step([(s[0], toks[:130], [])])                      # two full pages and two tokens of a third
+    assert lm.free_pages == 3
+    lm.reorder([s], [[0, 0, 0, 0]])
+    assert lm.free_pages == 0 and [lm.position(x) for x in s] == [130] * 4
+    lm.reorder([s], [[1, 0, 3, 3]])                        # partly filled pages change hands: none more is needed
+    assert lm.free_pages == 0
+    with pytest.raises(BufferError):
+        lm.step([(x, toks[130:192 + 1], []) for x in s])   # (a page more each)
+    lm.close(s[1])
+    assert lm.free_pages == 1
+    s[1] = lm.open()
+    lm.step([(s[1], [1], [])])
+    before = lm.step([(s[0], [5], [0]), (s[2], [5], [0])])
+    with pytest.raises(BufferError):
+        e = lm.open()
+        lm.reorder([[s[0], e]], [[0, 0]])
+    assert lm.free_pages == 0 and lm.position(e) == 0 and lm.position(s[0]) == 131
+    y = lm.step([(s[0], [9], [0]), (s[2], [9], [0])])
+    assert torch.equal(before[0], before[1]) and torch.equal(y[0], y[1])
+    lm.close(s[0])                                         # its own page alone: the others still hold the first two
+    assert lm.free_pages == 1
+    for x in (s[1], s[2], s[3], e):
+        lm.close(x)
+    assert lm.free_pages == 6
+    for slots, parents, kind in (([[0]], [[0]], Exception), ([[0, 0]], [[0, 1]], Exception)):
+        with pytest.raises(kind):
+            lm.reorder(slots, parents)                     # no open sequence
+    s = [lm.open() for _ in range(4)]
+    for slots, parents in (([s], [[0, 1, 2, 4]]), ([s], [[0, 1, 2, -1]]), ([s[:2] + s[:2]], [[0, 0, 0, 0]]), ([s], [[0]]), ([s, s[:3]], [[0] * 4] * 2)):
+        with pytest.raises(ValueError):
+            lm.reorder(slots, parents)
+    lm.reorder([], [])
+
+
+class _Beams64:
+    """The search in 64 bits, every sequence computed anew; `gap`: the least difference of rank between what a step kept and what it left."""
+
+    def __init__(self, orc, prompt, beams, steps, eos, alpha):
+        self.gap = math.inf
+        held = [(0.0, [], False)]
+        rank = lambda c: c[0] / len(c[1]) ** alpha  # noqa: E731
+        for _ in range(steps):
+            new = []
+            for score, toks, done in held:
+                if done:
+                    new.append((score, toks, True))
+                    continue
+                p = self.log_probs(orc, prompt, toks)
+                new += [(score + p[t], toks + [t], t == eos) for t in range(len(p))]
+            new.sort(key=rank, reverse=True)
+            if len(new) > beams:
+                self.gap = min(self.gap, rank(new[beams - 1]) - rank(new[beams]))
+            held = new[:beams]
+            if all(d for _, _, d in held):
+                break
+        self.held = held
+
+    @staticmethod
+    def log_probs(orc, prompt, toks):
+        y = np.asarray(orc.logits(prompt + toks)[-1], np.float64)
+        return y - y.max() - np.log(np.exp(y - y.max()).sum())
+
+
+def check_beam_search(dev, lib, name, dtype=F32, codes=None, beams=4, steps=9, alpha=0.0, room=None, **kw):
+    cfg = tc.MECHANISMS[name]
+    sd = random_token_lm_state_dict(cfg, seed=5)
+    cuts = (16, 1)
+    orc = EightBitOracle(sd, cfg, codes, cuts) if codes else TokenLMOracle(sd, cfg)
+    prompts = [tc.tokens_of(cfg, n, seed=n) for n in (16, 16, 16)] if codes else [tc.tokens_of(cfg, n, seed=n) for n in (5, 60, 1)]
+    eos = int(np.argmax(orc.logits(prompts[0] + [int(np.argmax(orc.logits(prompts[0])[-1]))])[-1]))      # the second token of the first one's likeliest
+    lm = TokenLM(sd, cfg, device=dev, dtype=dtype, lib=lib, kv_cache=codes, **{**dict(max_slots=3 * beams, max_tokens=64 * 2 * 3 * beams), **kw})
+    got = beam_search(lm, prompts, beams, steps, eos, alpha, **({} if codes else {"step_tokens": 14}))
+    assert lm.free_pages == lm.total_pages and lm.free_slots == lm.max_slots
+    same = 0
+    for prompt, hyps in zip(prompts, got):
+        want = _Beams64(orc, prompt, beams, steps, eos, alpha)
+        # a logit is off by at most its row's RMS error times sqrt(vocab); log p by twice that (itself and the sum), a score by that per token
+        rms = math.sqrt(float(np.mean(np.square(orc.logits(prompt)))))
+        off = (tc.TOL[dtype] + (ONE_CODE[codes] if codes else 0)) * rms * math.sqrt(cfg.vocab) * 2
+        assert len(hyps) == beams
+        ranks = [h.score / len(h.tokens) ** alpha for h in hyps]
+        assert ranks == sorted(ranks, reverse=True)
+        for h in hyps:
+            assert 1 <= len(h.tokens) <= steps and eos not in h.tokens[:-1] and (len(h.tokens) == steps or h.tokens[-1] == eos)
+            p = sum(_Beams64.log_probs(orc, prompt, h.tokens[:i])[t] for i, t in enumerate(h.tokens))
+            assert abs(h.score - p) <= off * len(h.tokens)
+        if want.gap > 2 * off * steps:
+            assert sorted(h.tokens for h in hyps) == sorted(t for _, t, _ in want.held)
+            same += 1
+    return same
+
+
+def check_beam_search_of_one(dev, lib, name="mixed"):
+    """One beam is greedy decoding; more requests than fit wait for the first ones' slots and pages."""
+    from moshi_amd.token_batcher import TokenBatcher
+    cfg = tc.MECHANISMS[name]
+    lm = TokenLM(random_token_lm_state_dict(cfg, seed=5), cfg, device=dev, dtype=F32, lib=lib, max_slots=2, max_tokens=64 * 3)
+    prompts = [tc.tokens_of(cfg, n, seed=n) for n in (3, 70, 64, 9)]
+    want = TokenBatcher(lm).generate(prompts, 6)
+    assert [h[0].tokens for h in beam_search(lm, prompts, 1, 6)] == want
+    with pytest.raises(BufferError):
+        beam_search(lm, prompts, 3, 6)
+    with pytest.raises(BufferError):
+        beam_search(lm, [tc.tokens_of(cfg, 150)], 2, 6)
+    for bad in (([[]], 1, 1), ([[1]], 0, 1), ([[1]], 1, 0), ([[cfg.vocab]], 1, 1), ([[-1]], 1, 1), ([[1]], 1, 1, cfg.vocab)):
+        with pytest.raises(ValueError):
+            beam_search(lm, *bad)
+    assert beam_search(lm, [], 2, 4) == [] and lm.free_slots == 2 and lm.free_pages == lm.total_pages

@@ -177,3 +177,24 @@ def test_offsets_past_32_bits(lib):
         c.append(k, v, table, i32(0), i32(0, 200))
         out.append((c.attend(q, table, i32(0), i32(0, 200)), c.attend(q[-1:], table, i32(199))))
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("name, codes", [("mixed", None), ("bibapel", None), ("bibapel", "int8"), ("two_kept_windows", "e4m3"), ("bigram", None), ("delta_widest", None),
+                                         ("projected_passes", None)])
+@pytest.mark.parametrize("dtype", [oc.F32, oc.BF16], ids=["fp32", "bf16"])
+def test_token_lm_reorder(lib, name, codes, dtype):
+    oc.check_token_lm_reorder(name, DEV, lib, dtype, codes)
+
+
+def test_token_lm_reorder_pool(lib):
+    oc.check_token_lm_reorder_pool(DEV, lib)
+
+
+@pytest.mark.parametrize("name, codes, alpha", [("mixed", None, 0.0), ("bibapel", None, 0.7), ("grouped_attention", "int8", 1.0), ("bibapel", "e4m3", 0.0)])
+@pytest.mark.parametrize("dtype", [oc.F32, oc.BF16], ids=["fp32", "bf16"])
+def test_beam_search(lib, name, codes, alpha, dtype):
+    oc.check_beam_search(DEV, lib, name, dtype, codes, alpha=alpha)
+
+
+def test_beam_search_of_one(lib):
+    oc.check_beam_search_of_one(DEV, lib)

@@ -83,3 +83,21 @@ def test_token_lm_batch(tlm_lib):  # noqa: F811
 
 def test_token_lm_refusals(tlm_lib):  # noqa: F811
     oc.check_token_lm_refusals(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name, codes", [("mixed", None), ("bibapel", None), ("bibapel", "int8"), ("two_kept_windows", "e4m3"), ("bigram", None), ("delta", None)])
+def test_token_lm_reorder(tlm_lib, name, codes):  # noqa: F811
+    oc.check_token_lm_reorder(name, DEV, tlm_lib, codes=codes, lengths=((20, 64, 1, 70, 63), (65, 7, 30, 30, 66)), tail=6)
+
+
+def test_token_lm_reorder_pool(tlm_lib):  # noqa: F811
+    oc.check_token_lm_reorder_pool(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name, codes, alpha", [("mixed", None, 0.0), ("bibapel", None, 0.7), ("grouped_attention", "int8", 1.0)])
+def test_beam_search(tlm_lib, name, codes, alpha):  # noqa: F811
+    oc.check_beam_search(DEV, tlm_lib, name, codes=codes, alpha=alpha, beams=3, steps=5)
+
+
+def test_beam_search_of_one(tlm_lib):  # noqa: F811
+    oc.check_beam_search_of_one(DEV, tlm_lib)
