@@ -178,7 +178,6 @@ __device__ __forceinline__ Kv8Span kv8_span(const TlmKv8Seqs& q, const Kv8Cut& z
     o.row = s.row0 + o.pos - s.pos0;               // row of the block's first token (of token lo on they are the call's)
     o.page = o.none ? -1 : kv8_page(q, n_pages, kv8_table(q, e), b / KV8_PARTS);
     o.part = b % KV8_PARTS;
-    o.none = o.none || o.page < 0;
     return o;
 }
 // scale of the block after tokens with the largest magnitude `bits` (as an integer: a NaN's is above all others)
@@ -200,105 +199,169 @@ __device__ __forceinline__ unsigned kv8_bits(f32x4 x) {
     return m;
 }
 
-// One wave per block, head and side; four heads a workgroup, which form the angles of the block's tokens once.
+// Four elements as they come, to be widened behind the last load: a conversion beside each load would wait for it, 18 us for the values of a
+// block of prompts where all of it together takes 4.
+template <class In> struct Kv8In;
+template <> struct Kv8In<float> {
+    typedef f32x4 T;
+    static __device__ __forceinline__ T slow(const float* p) { return T{p[0], p[1], p[2], p[3]}; }
+    static __device__ __forceinline__ f32x4 wide(T x) { return x; }
+    static __device__ __forceinline__ float wide(float x) { return x; }
+};
+template <> struct Kv8In<uint16_t> {
+    typedef u32x2 T;
+    static __device__ __forceinline__ T slow(const uint16_t* p) { return T{p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16}; }
+    static __device__ __forceinline__ f32x4 wide(T w) {
+        return f32x4{__builtin_bit_cast(float, w[0] << 16), __builtin_bit_cast(float, w[0] & 0xffff0000u), __builtin_bit_cast(float, w[1] << 16),
+                     __builtin_bit_cast(float, w[1] & 0xffff0000u)};
+    }
+    static __device__ __forceinline__ float wide(uint16_t x) { return mmi_bf16_to_f32(x); }
+};
+// the first n of four bytes
+__device__ __forceinline__ uint32_t kv8_bytes_below(int n) { return n <= 0 ? 0u : (n >= 4 ? 0xffffffffu : (1u << (8 * n)) - 1u); }
+// pair p's angle at a position, where its dimensions find it
+__device__ __forceinline__ void kv8_put_angle(const TlmKv8Cache& c, float* cs, float* sn, int pos, int p, double freq) {
+    float co, si;
+    kv8_angle(pos, freq, co, si);
+    const int d = c.halves ? p : 2 * p, e = c.halves ? p + c.rot / 2 : d + 1;
+    cs[d] = cs[e] = co;
+    sn[d] = -si;
+    sn[e] = si;
+}
+// One wave per block, head and side; four heads a workgroup, which form the angles of the block's tokens once.  A few tokens' call is as long as its
+// chain of loads and its code's way to the CU, so no load waits for another that it does not need, nothing branches around one (lanes without a
+// token of the call read its nearest), and the common path is short.
 // grid: slots of blocks, kv heads / 4, 2 (keys, values)
 //   keys: four lanes per token, granules of 4 dimensions in turn      values: a lane per dimension, its 16 tokens side by side
-template <class In, bool E4M3>
-__global__ __launch_bounds__(256) void k_tlm_kv8_append(TlmKv8Append a) {
+template <class In, bool E4M3, int D>
+__global__ __launch_bounds__(256, D == 128 ? 4 : 2) void k_tlm_kv8_append(TlmKv8Append a) {
     typedef Kv8Code<E4M3> C;
-    MMI_SHARED float angle[KV8_BLOCK * 2 * 128];           // [token][pair][cos, sin]
+    typedef Kv8In<In> R;
+    constexpr int N = D / 16, LD = D + 16;                 // granules of a lane; floats of a token's angles (two tokens' reads: banks of their own)
+    MMI_SHARED float cs[KV8_BLOCK * LD], sn[KV8_BLOCK * LD];      // [token][dimension]: cosine; sine, with the sign that the partner takes
     const Kv8Span s = kv8_span(a.q, a.z, a.c.n_pages, (int)blockIdx.x);
-    if (s.none) return;
-    const int lane = mmi_lane(), g = (int)blockIdx.y * 4 + mmi_uniform((int)threadIdx.x >> 6), part = s.part;
-    const bool held = s.lo > 0, wide = a.wide != 0;
-    const long unit = (long)s.page * a.c.kv_heads + g;
+    if (s.none) return;                                    // (the page is looked at behind the first loads: it is on its way meanwhile)
+    const int lane = mmi_lane(), g = (int)blockIdx.y * 4 + mmi_uniform((int)threadIdx.x >> 6), gc = min(g, a.c.kv_heads - 1);
+    const bool held = s.lo > 0;
+    const long unit = (long)s.page * a.c.kv_heads + gc;
     if (blockIdx.z == 0) {
-        const int t = lane >> 2, c = lane & 3, n = a.c.dim / 16, half = a.c.rot / 2;
-        const In* row = (const In*)a.k + (long)(s.row + t) * a.k_row + (long)g * a.k_head;
-        uint32_t* out = (uint32_t*)(a.c.k + (unit * TLM_PAGE + part * KV8_BLOCK + t) * a.c.dim);
-        const bool fresh = t >= s.lo && t < s.hi && g < a.c.kv_heads;
-        f32x4 x[16], y[16];
+        const int t = lane >> 2, c = lane & 3, n = a.c.dim / 16, rot = a.c.rot, half = rot / 2;
+        const In* row = (const In*)a.k + (long)(s.row + min(max(t, s.lo), s.hi - 1)) * a.k_row + (long)gc * a.k_head;
+        typename R::T x[N], y[N];
+        auto at = [&](int i) { return 4 * (c + 4 * min(i, n - 1)); };
+        auto partner = [&](int d) { return d < half ? d + half : (d < rot ? d - half : d); };
+        if (a.wide) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n && fresh) {
-                x[i] = kv8_in4(row + 4 * (c + 4 * i), wide);
-                y[i] = kv8_partners4(a.c, row, 4 * (c + 4 * i), wide);
+            for (int i = 0; i < N; ++i) x[i] = *(const typename R::T*)(row + at(i));
+            if (rot && a.c.halves) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = *(const typename R::T*)(row + partner(at(i)));
             }
-        float* scale = a.c.ks + unit * KV8_PARTS + part, ratio;
-        const float before = held && g < a.c.kv_heads ? *scale : 0.f;
-        if (half) {
-            for (int i = (int)threadIdx.x; i < (s.hi - s.lo) * half; i += 256) {
-                const int u = s.lo + i / half, p = i % half;
-                kv8_angle(s.pos + u, a.c.freq[p], angle[(u * half + p) * 2], angle[(u * half + p) * 2 + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[i] = R::slow(row + at(i));
+                y[i] = R::slow(row + partner(at(i)));
+            }
+        }
+        if (s.page < 0) return;
+        uint32_t* out = (uint32_t*)(a.c.k + (unit * TLM_PAGE + s.part * KV8_BLOCK + t) * a.c.dim);
+        float* scale = a.c.ks + unit * KV8_PARTS + s.part, ratio;
+        const float before = held ? *scale : 0.f;
+        uint32_t old[N];
+        if (held) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) old[i] = out[at(i) / 4];
+        }
+        if (rot) {
+            const int step = 256 / half, all = (s.hi - s.lo) * half;      // (half is at most 128)
+            int u = (int)threadIdx.x / half, p = (int)threadIdx.x % half;
+            if (step * half == 256) {                                     // a thread's pair stays the same
+                const double freq = a.c.freq[p];
+                for (; u < s.hi - s.lo; u += step) kv8_put_angle(a.c, cs + (s.lo + u) * LD, sn + (s.lo + u) * LD, s.pos + s.lo + u, p, freq);
+            } else {
+                for (int i = (int)threadIdx.x; i < all; i += 256) {
+                    u = s.lo + i / half;
+                    p = i % half;
+                    kv8_put_angle(a.c, cs + u * LD, sn + u * LD, s.pos + u, p, a.c.freq[p]);
+                }
             }
             __syncthreads();
         }
+        const bool fresh = t >= s.lo && t < s.hi;
+        f32x4 z[N];
         unsigned bits = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n && fresh) {
-                x[i] = kv8_turned4(a.c, x[i], y[i], 4 * (c + 4 * i), angle + t * 2 * half);
-                bits = max(bits, kv8_bits(x[i]));
+        for (int i = 0; i < N; ++i) {
+            z[i] = R::wide(x[i]);
+            if (rot) {
+                const f32x4 o = R::wide(y[i]), w = a.c.halves ? o : f32x4{z[i][1], z[i][0], z[i][3], z[i][2]};
+                const f32x4 co = *(const f32x4*)(cs + t * LD + at(i)), si = *(const f32x4*)(sn + t * LD + at(i));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float turned = mmi_fma(w[r], si[r], z[i][r] * co[r]);
+                    z[i][r] = at(i) < rot ? turned : z[i][r];
+                }
             }
-        bits = mmi_wave_max_u32(bits);
+            bits = max(bits, kv8_bits(z[i]));
+        }
+        bits = mmi_wave_max_u32(fresh ? bits : 0u);
         if (g >= a.c.kv_heads) return;
         const float after = kv8_grown<E4M3>(before, held, bits, ratio), inv = 1.f / after;
         const bool bad = !(after == after);
         if (fresh) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < n) out[c + 4 * i] = bad ? 0u : C::pack(x[i] * inv);
+            for (int i = 0; i < N; ++i)
+                if (i < n) out[c + 4 * i] = bad ? 0u : C::pack(z[i] * inv);
         } else if (t < s.lo && ratio != 1.f) {
-            for (int i = 0; i < n; ++i) out[c + 4 * i] = bad ? 0u : C::pack(C::unpack(out[c + 4 * i]) * ratio);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < n) out[c + 4 * i] = bad ? 0u : C::pack(C::unpack(old[i]) * ratio);
         }
         if (lane == 0) *scale = after;
     } else {
-        if (g >= a.c.kv_heads) return;
-        const int n = (a.c.vdim + 63) / 64;
-        const In* v = (const In*)a.v + (long)s.row * a.v_row + (long)g * a.v_head;
-        float x[4][KV8_BLOCK];
+        const In* v = (const In*)a.v + (long)s.row * a.v_row + (long)gc * a.v_head;
+        In x[D / 64][KV8_BLOCK];
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+            for (int t = 0; t < KV8_BLOCK; ++t) x[i][t] = v[(long)min(max(t, s.lo), s.hi - 1) * a.v_row + min(lane + 64 * i, a.c.vdim - 1)];
+        if (s.page < 0 || g >= a.c.kv_heads) return;
+        const bool whole = s.lo == 0 && s.hi == KV8_BLOCK;
+        u32x4* out = (u32x4*)(a.c.v + unit * a.c.vdim * TLM_PAGE + s.part * KV8_BLOCK);
+        auto at = [&](int i) { return min(lane + 64 * i, a.c.vdim - 1) * (TLM_PAGE / 16); };
+        float* scale = a.c.vs + unit * KV8_PARTS + s.part, ratio;
+        const float before = held ? *scale : 0.f;
+        u32x4 old[D / 64];
+        if (!whole) {                                      // (the bytes behind the last token stay what they are)
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) old[i] = out[at(i)];
+        }
         unsigned bits = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = lane + 64 * i;
-            if (d < a.c.vdim)
+        for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-                for (int t = 0; t < KV8_BLOCK; ++t)
-                    if (t >= s.lo && t < s.hi) {
-                        x[i][t] = kv8_load(v + (long)t * a.v_row + d);
-                        bits = max(bits, __builtin_bit_cast(unsigned, x[i][t]) & 0x7fffffffu);
-                    }
-        }
-        float* scale = a.c.vs + unit * KV8_PARTS + part, ratio;
-        const float before = held ? *scale : 0.f;
+            for (int t = 0; t < KV8_BLOCK; ++t) bits = max(bits, __builtin_bit_cast(unsigned, R::wide(x[i][t])) & 0x7fffffffu);
         bits = mmi_wave_max_u32(bits);
         const float after = kv8_grown<E4M3>(before, held, bits, ratio), inv = 1.f / after;
-        const bool bad = !(after == after), whole = s.lo == 0 && s.hi == KV8_BLOCK;
+        const bool bad = !(after == after);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = lane + 64 * i;
-            if (i >= n || d >= a.c.vdim) continue;
-            u32x4* out = (u32x4*)(a.c.v + (unit * a.c.vdim + d) * TLM_PAGE + part * KV8_BLOCK);
-            u32x4 w = whole ? u32x4{0u, 0u, 0u, 0u} : *out;      // (the bytes behind the last token stay what they are)
+        for (int i = 0; i < D / 64; ++i) {
+            u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f32x4 y;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int t = 4 * j + r;
-                    y[r] = t >= s.lo && t < s.hi ? x[i][t] * inv : 0.f;
-                }
-                const uint32_t now = bad ? 0u : C::pack(y), was = bad ? 0u : (ratio != 1.f ? C::pack(C::unpack(w[j]) * ratio) : w[j]);
-                uint32_t m = 0, o = 0;                       // bytes of the new tokens, of the ones held
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int t = 4 * j + r;
-                    m |= t >= s.lo && t < s.hi ? 0xffu << (8 * r) : 0u;
-                    o |= t < s.lo ? 0xffu << (8 * r) : 0u;
-                }
-                w[j] = (now & m) | (was & o) | (w[j] & ~(m | o));
+                const f32x4 y = {R::wide(x[i][4 * j]), R::wide(x[i][4 * j + 1]), R::wide(x[i][4 * j + 2]), R::wide(x[i][4 * j + 3])};
+                w[j] = bad ? 0u : C::pack(y * inv);
             }
-            *out = w;
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t b = old[i][j], was = bad ? 0u : (ratio != 1.f ? C::pack(C::unpack(b) * ratio) : b);
+                    const uint32_t o = kv8_bytes_below(s.lo - 4 * j), m = kv8_bytes_below(s.hi - 4 * j) & ~o;      // tokens held, new ones
+                    w[j] = (w[j] & m) | (was & o) | (b & ~(m | o));
+                }
+            }
+            if (lane + 64 * i < a.c.vdim) out[at(i)] = w;
         }
         if (lane == 0) *scale = after;
     }
@@ -319,29 +382,46 @@ __device__ __forceinline__ void kv8_put(uint16_t* p, float v) { *p = mmi_f32_to_
 template <class Out, bool E4M3>
 __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
     typedef Kv8Code<E4M3> C;
-    Kv8Span s = kv8_span(a.q, a.z, a.c.n_pages, (int)blockIdx.x);
-    if (s.none && s.hi <= s.lo) return;
+    const Kv8Span s = kv8_span(a.q, a.z, a.c.n_pages, (int)blockIdx.x);
+    if (s.none) return;
+    const bool lost = s.page < 0;
     const int lane = mmi_lane(), g = (int)blockIdx.y;
     const long unit = (long)max(s.page, 0) * a.c.kv_heads + g;
-    const float scale = s.none ? 0.f : (blockIdx.z ? a.c.vs : a.c.ks)[unit * KV8_PARTS + s.part];
+    const float scale = lost ? 0.f : (blockIdx.z ? a.c.vs : a.c.ks)[unit * KV8_PARTS + s.part];
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     if (blockIdx.z == 0) {
         const int t = lane >> 2, c = lane & 3;
         if (t < s.lo || t >= s.hi) return;
         const uint32_t* in = (const uint32_t*)(a.c.k + (unit * TLM_PAGE + s.part * KV8_BLOCK + t) * a.c.dim);
         Out* out = (Out*)a.k + ((long)(s.row + t) * a.c.kv_heads + g) * a.c.dim;
-        for (int i = c; i < a.c.dim / 4; i += 4) kv8_put4(out + 4 * i, s.none ? zero : C::unpack(in[i]) * scale);
+        const int n = a.c.dim / 16;
+        for (int i0 = 0; i0 < n; i0 += 8) {                // (eight loads on their way at once)
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = in[c + 4 * min(i0 + i, n - 1)];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i0 + i < n) kv8_put4(out + 4 * (c + 4 * (i0 + i)), lost ? zero : C::unpack(w[i]) * scale);
+        }
     } else {
-        for (int d = lane; d < a.c.vdim; d += 64) {
-            const u32x4 w = *(const u32x4*)(a.c.v + (unit * a.c.vdim + d) * TLM_PAGE + s.part * KV8_BLOCK);
-            Out* out = (Out*)a.v + ((long)s.row * a.c.kv_heads + g) * a.c.vdim + d;
-            const long ld = (long)a.c.kv_heads * a.c.vdim;
+        const u32x4* in = (const u32x4*)(a.c.v + unit * a.c.vdim * TLM_PAGE + s.part * KV8_BLOCK);
+        const long ld = (long)a.c.kv_heads * a.c.vdim;
+        for (int d0 = lane; d0 < a.c.vdim; d0 += 128) {
+            u32x4 w[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 x = s.none ? zero : C::unpack(w[j]) * scale;
+            for (int i = 0; i < 2; ++i) w[i] = in[min(d0 + 64 * i, a.c.vdim - 1) * (TLM_PAGE / 16)];
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (4 * j + r >= s.lo && 4 * j + r < s.hi) kv8_put(out + (4 * j + r) * ld, x[r]);
+            for (int i = 0; i < 2; ++i) {
+                const int d = d0 + 64 * i;
+                if (d >= a.c.vdim) break;
+                Out* out = (Out*)a.v + ((long)s.row * a.c.kv_heads + g) * a.c.vdim + d;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 x = lost ? zero : C::unpack(w[i][j]) * scale;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (4 * j + r >= s.lo && 4 * j + r < s.hi) kv8_put(out + (4 * j + r) * ld, x[r]);
+                }
             }
         }
     }

@@ -109,8 +109,11 @@ int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype) {
     a.z = kv8_cut(a.q, 1, KV8_BLOCK, 2);               // (a portion of n rows touches at most (n + 14) / 16 + 1 blocks)
     const dim3 grid((unsigned)kv8_slots(a.q, a.z), mmi_cdiv(a.c.kv_heads, 4), 2);
     return by_codes(a.c.e4m3, [&](auto e) {
-        if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_kv8_append<float, decltype(e)::value>), grid, 256, 0, s, a);
-        else MMI_LAUNCH((k_tlm_kv8_append<uint16_t, decltype(e)::value>), grid, 256, 0, s, a);
+        const bool wide = a.c.dim > 128 || a.c.vdim > 128;
+        if (dtype == MMI_F32 && wide) MMI_LAUNCH((k_tlm_kv8_append<float, decltype(e)::value, 256>), grid, 256, 0, s, a);
+        else if (dtype == MMI_F32) MMI_LAUNCH((k_tlm_kv8_append<float, decltype(e)::value, 128>), grid, 256, 0, s, a);
+        else if (wide) MMI_LAUNCH((k_tlm_kv8_append<uint16_t, decltype(e)::value, 256>), grid, 256, 0, s, a);
+        else MMI_LAUNCH((k_tlm_kv8_append<uint16_t, decltype(e)::value, 128>), grid, 256, 0, s, a);
         MMI_CHECK_LAUNCH();
         return (int)MMI_OK;
     });
