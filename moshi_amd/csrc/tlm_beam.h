@@ -39,6 +39,15 @@ __device__ __forceinline__ f32x4 beam_load4(const uint16_t* p) {
 __device__ __forceinline__ float beam_load(const float* p) { return *p; }
 __device__ __forceinline__ float beam_load(const uint16_t* p) { return mmi_bf16_to_f32(*p); }
 
+// e^(d + low), d <= 0, as 2^(d log2 e) with the product's low part carried along: a sum's relative error stays near 2^-28, where its logarithm is
+// added to scores whose order it decides
+__device__ __forceinline__ float beam_exp(float d, float low) {
+    constexpr float L = 1.44269504f, LL = 1.92596299e-8f;
+    d = d < -200.f ? -200.f : d;                           // (zero either way; a mask's -3e38 would leave infinities)
+    const float p = L * d;
+    return mmi_fast_exp2f(mmi_fma(L, low, mmi_fma(LL, d, mmi_fma(L, d, -p)))) * mmi_fast_exp2f(p);
+}
+
 // A wave's best: the `beams`-th largest of the lanes' maxima is a bound that as many logits reach, and few more do, one or two beyond `beams` of
 // 1024 distinct ones: these are put side by side and ranked by counting who is before whom.  Where more than 64 reach it (equal logits), they are
 // taken out one at a time.  grid: chunks / 4, rows
@@ -69,15 +78,10 @@ __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
 #pragma unroll
     for (int n = 0; n < N; ++n) top = fmaxf(top, v[n]);    // (NaN is passed over here and makes the sum one)
     const float m = mmi_wave_max_f32(top);
-    // e^d as 2^(d log2 e) with the product's low part carried along: the sum's relative error stays near 2^-28, where its logarithm is added to
-    // scores whose order it decides.  Places past the vocabulary's end hold -infinity.
-    constexpr float L = 1.44269504f, LL = 1.92596299e-8f;
-    float s = 0.f;
+    float s = 0.f;                                         // (places past the vocabulary's end hold -infinity)
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        float d = v[n] - m;
-        d = d < -200.f ? -200.f : d;                       // (zero either way; a mask's -3e38 would leave infinities)
-        const float p = L * d, e = mmi_fast_exp2f(mmi_fma(LL, d, mmi_fma(L, d, -p))) * mmi_fast_exp2f(p);
+        const float e = beam_exp(v[n] - m, 0.f);
         s += v[n] == -INFINITY ? 0.f : e;
     }
     double sum = (double)s;
@@ -177,31 +181,45 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         }
     };
     ask(0);
-    for (int k = wave; k < K; k += 4) {
-        const int row = b * K + k;
-        const bool done = a.done && a.done[row];
-        const double s = (double)a.score[row];
-        double z = s;
-        if (!done) {
-            float M = -INFINITY;
-            for (int i = lane; i < a.chunks; i += 64) M = fmaxf(M, a.wm[(long)row * a.chunks + i]);
+    // two rows a wave at once, a chunk a lane; then a beam a lane: its score and its length's power, in 64 bits
+    const bool mine = tid < K, done = mine && a.done && a.done[b * K + tid];
+    const double score = mine ? (double)a.score[b * K + tid] : 0.;
+    const int len = mine && a.length ? a.length[b * K + tid] + (done ? 0 : 1) : 1;
+    for (int k = wave; k < K; k += 8) {
+        const long r0 = (long)(b * K + k) * a.chunks, r1 = (long)(b * K + min(k + 4, K - 1)) * a.chunks;
+        const int at = min(lane, a.chunks - 1);
+        const bool in = lane < a.chunks;
+        const float m0 = a.wm[r0 + at], m1 = a.wm[r1 + at];
+        const double w0 = a.ws[r0 + at], w1 = a.ws[r1 + at];
+        auto sum = [&](int k, long row, float m, double w) __attribute__((always_inline)) {
+            float M = in ? m : -INFINITY;
+            for (int i = lane + 64; i < a.chunks; i += 64) M = fmaxf(M, a.wm[row + i]);
             M = mmi_wave_max_f32(M);
-            double S = 0.;
-            for (int i = lane; i < a.chunks; i += 64) {
-                const double w = a.ws[(long)row * a.chunks + i];
-                S += w == 0. ? 0. : w * exp((double)a.wm[(long)row * a.chunks + i] - (double)M);
-            }
+            auto share = [&](float m, double w) __attribute__((always_inline)) {
+                const double d = (double)m - (double)M;
+                const float high = (float)d;
+                return w == 0. ? 0. : w * (double)beam_exp(high, (float)(d - (double)high));
+            };
+            double S = in ? share(m, w) : 0.;
+            for (int i = lane + 64; i < a.chunks; i += 64) S += share(a.wm[row + i], a.ws[row + i]);
 #pragma unroll
             for (int i = 1; i < 64; i <<= 1) S += mmi_shfl_xor(S, i);
-            z = s - ((double)M + log(S));
-        }
-        if (lane == 0) {
-            const int len = a.length ? a.length[row] + (done ? 0 : 1) : 1;
-            base[k] = z;
-            inv[k] = a.alpha == 0. ? 1. : pow((double)max(len, 1), -a.alpha);
-            kind[k] = z > -INFINITY && z < INFINITY ? (done ? 1 : 0) : 2;
-        }
+            if (lane == 0) {
+                base[k] = (double)M;
+                inv[k] = S;
+            }
+        };
+        sum(k, r0, m0, w0);
+        if (k + 4 < K) sum(k + 4, r1, m1, w1);
     }
+    __syncthreads();
+    if (mine) {
+        const double z = done ? score : score - (base[tid] + log(inv[tid]));
+        base[tid] = z;
+        inv[tid] = a.alpha == 0. ? 1. : (a.alpha == 1. ? 1. / (double)max(len, 1) : pow((double)max(len, 1), -a.alpha));
+        kind[tid] = z > -INFINITY && z < INFINITY ? (done ? 1 : 0) : 2;
+    }
+    const float one_per = 1.f / (float)per;
     x[N] = -INFINITY;
     p[N] = BEAM_NONE;
     y[N] = -INFINITY;
@@ -216,7 +234,16 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int n = n0 + tid + 256 * j, k = min((int)((unsigned)n / per), K - 1), h = n - k * (int)per;
+            if (n0 + 256 * j >= all) {                     // (one request's few candidates leave most places empty)
+                p[j] = BEAM_NONE;
+                continue;
+            }
+            const int n = n0 + tid + 256 * j;
+            int k = (int)((float)n * one_per);             // n / per (n is below 2^21: at most one off)
+            if (k * (int)per > n) --k;
+            else if ((k + 1) * (int)per <= n) ++k;
+            k = min(k, K - 1);
+            const int h = n - k * (int)per;
             int token = n < all ? p[j] : BEAM_NONE;
             double s = -INFINITY;
             if (kind[k] == 0) {
@@ -232,7 +259,8 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j <= N; ++j) top = fmaxf(top, p[j] == BEAM_NONE ? -INFINITY : (float)x[j]);
+        for (int j = 0; j <= N; ++j)
+            if (j == N || n0 + 256 * j < all) top = fmaxf(top, p[j] == BEAM_NONE ? -INFINITY : (float)x[j]);
         float bound = mmi_wave_max_f32(top);
         {
             float left = top;
@@ -249,6 +277,7 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         int count = 0;
 #pragma unroll
         for (int j = 0; j <= N; ++j) {
+            if (j < N && n0 + 256 * j >= all) continue;
             const bool in = p[j] != BEAM_NONE && (float)x[j] >= bound;
             const uint64_t at = mmi_ballot(in);
             if (!at) continue;

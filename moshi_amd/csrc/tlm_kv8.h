@@ -61,8 +61,8 @@ __device__ __forceinline__ const int* kv8_table(const TlmKv8Seqs& a, int e) { re
 // (by > 0: only entries with at least `by` units need a slot; one more for each `by` units is then enough, where that is fewer than one per entry.)
 struct Kv8Cut { int mul, per, extra, by; };            // mul 0: `extra` slots per entry
 MMI_HD int kv8_slots_before(const Kv8Cut& z, int row, int e) {
-    const long u = (long)row * z.mul;
-    return (int)(u / z.per) + (z.by ? (int)(u / z.by) : z.extra * e);
+    const unsigned u = (unsigned)row * (unsigned)z.mul;    // (below 2^31; `per` is a power of two)
+    return (int)(u >> __builtin_ctz(z.per)) + (z.by ? (int)(u / (unsigned)z.by) : z.extra * e);
 }
 __device__ __forceinline__ int kv8_slot0(const TlmKv8Seqs& a, const Kv8Cut& z, int e) { return z.mul ? kv8_slots_before(z, kv8_row0(a, e), e) : z.extra * e; }
 __device__ __forceinline__ int kv8_find(const TlmKv8Seqs& a, const Kv8Cut& z, int slot) {
@@ -1110,34 +1110,47 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
     if constexpr (!WIDE) {
         const int lane = tid & 63, G = a.c.vdim / 4, at_once = 64 / G, n = (b - slot * each) * at_once + lane / G, d = 4 * (lane % G);
         const bool on = lane / G < at_once && n < h.cols;
-        // (asked for before it is known how many splits there were)
-        const long p = part * per + (on ? n : 0);
-        float m[16], l[16];
-        f32x4 v[16];
+        const float *ml0 = h.pml + part * 2 * per, *po0 = h.po + part * per * a.c.vdim;
+        const unsigned at_ml = on ? n : 0, at_po = at_ml * a.c.vdim + d;
+        const int step = per * a.c.vdim;                   // (a split's part: addresses are a scalar and a lane's offset)
+        float m[8], l[8];
+        f32x4 v[8];
+        auto load = [&](int k0, int ns) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (k < h.nsplit) {
-                const float* ml = h.pml + (part + k) * 2 * per + (on ? n : 0);
-                m[k] = ml[0];
-                l[k] = ml[per];
-                v[k] = *(const f32x4*)(h.po + (p + (long)k * per) * a.c.vdim + d);
-            }
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < ns) {
+                    const float* ml = ml0 + (k0 + k) * 2 * per;
+                    m[k] = ml[at_ml];
+                    l[k] = (ml + per)[at_ml];
+                    v[k] = *(const f32x4*)(po0 + (k0 + k) * step + at_po);
+                }
+        };
+        if (few) load(0, h.nsplit);                        // (single tokens: asked for before it is known how many splits there were)
         const Kv8Cols c(a, h, few, slot);
         const int col = c.c0 + n, ns = max(1, (c.n + h.pages - 1) / h.pages);
         if (!on || col >= c.ncol) return;
+        if (!few) load(0, ns);                             // (of the slots that portions might need, half are empty)
         float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (k < ns) M = fmaxf(M, m[k]);
-        const float Ms = M == -INFINITY ? 0.f : M;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0;;) {
+            float top = M;
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (k < ns) {
-                const float w = exp2f(m[k] - Ms);
-                L += l[k] * w;
-                o += v[k] * w;
-            }
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < ns) top = fmaxf(top, m[k]);
+            const float Ms = top == -INFINITY ? 0.f : top, less = mmi_fast_exp2f(M - Ms);
+            L *= less;
+            o *= less;
+            M = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < ns) {
+                    const float w = mmi_fast_exp2f(m[k] - Ms);
+                    L += l[k] * w;
+                    o += v[k] * w;
+                }
+            if ((k0 += 8) >= ns) break;
+            load(k0, ns);
+        }
         const int tok = col / a.rep;
         kv8_store<Tr>(a, c.s.row0 + tok, g * a.rep + col - tok * a.rep, d, o * kv8_inverse(L, M, a.sink));
     } else {
@@ -1159,7 +1172,7 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) M = fmaxf(M, red[w][0]);
-        const float w = tid < ns ? exp2f(m - (M == -INFINITY ? 0.f : M)) : 0.f, wl = mmi_wave_sum_down(tid < ns ? l * w : 0.f);
+        const float w = tid < ns ? mmi_fast_exp2f(m - (M == -INFINITY ? 0.f : M)) : 0.f, wl = mmi_wave_sum_down(tid < ns ? l * w : 0.f);
         wt[tid] = w;
         if ((tid & 63) == 0) red[wave][1] = wl;
         __syncthreads();

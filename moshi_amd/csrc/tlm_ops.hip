@@ -7,6 +7,7 @@
 namespace {
 
 constexpr long KV8_WORKGROUPS = 512;     // that a split of the pages aims at: 2 per CU, all at once
+constexpr long KV8_TILES = 384;           // the same of k_tlm_kv8_tile, which works faster alone on a CU and writes its parts for longer (128, 256, 384, 512: 60, 46, 45, 49 us for 16 sequences with 560 tokens)
 constexpr int KV8_MAX_SPLIT = 256;       // (k_tlm_kv8_combine: a lane each)
 
 int check_cache(const mmi_kv_cache* c, TlmKv8Cache* out, const char* at) {
@@ -88,7 +89,7 @@ int launch_attn_d(hipStream_t s, const TlmKv8Attn& a) {
     return d == 64 ? launch_attn_c<In, Tr, NS, 64>(s, a) : (d == 128 ? launch_attn_c<In, Tr, NS, 128>(s, a) : launch_attn_c<In, Tr, NS, 256>(s, a));
 }
 // how a kernel's `groups` (the ones that are likely to have columns) share the pages out; floats of workspace, at most `room`
-size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, size_t room) {
+size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, size_t room, long aim, long step) {
     if (a.mask.window > 0)                             // positions plo - window + 1 .. phi, and the first ones that are kept
         cap = std::min<long>(cap, ((long)a.mask.window + h.z.per / a.rep + 1) / TLM_PAGE + 2 + mmi_cdiv(a.mask.keep, TLM_PAGE));
     cap = std::max(cap, 1l);
@@ -96,8 +97,8 @@ size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, size
     const size_t each = (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.z.per * (a.c.vdim + 2);      // floats per split
     long most = std::min<long>(KV8_MAX_SPLIT, (long)(room / std::max<size_t>(1, each)));
     if (most < 2) most = 1;
-    long per = std::max((cap * units + KV8_WORKGROUPS - 1) / KV8_WORKGROUPS, (cap + most - 1) / most);
-    per = std::min((per + 3) / 4 * 4, (cap + 3) / 4 * 4);      // (each of a workgroup's four waves takes every fourth page)
+    long per = std::max((cap * units + aim - 1) / aim, (cap + most - 1) / most);
+    per = std::min((per + step - 1) / step * step, (cap + step - 1) / step * step);
     h.pages = (int)per;
     h.nsplit = (int)((cap + per - 1) / per);
     return h.nsplit > 1 ? each * h.nsplit : 0;
@@ -123,13 +124,13 @@ size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, size_t room) {
     a.both = a.q.row0 != nullptr;
     a.few.z = Kv8Cut{0, 16, a.both ? 1 : mmi_cdiv(a.rep, 16), 0};
     a.few.cols = a.both ? KV8_FEW : std::min(16, a.rep);
-    const size_t few = split_pages(a, a.few, kv8_slots(a.q, a.few.z), cap, room);
+    const size_t few = split_pages(a, a.few, kv8_slots(a.q, a.few.z), cap, room, KV8_WORKGROUPS, 4);      // (each of a workgroup's four waves takes every fourth page)
     if (!a.both) return few;
     a.many.z = Kv8Cut{a.rep, KV8_MANY, 1, 0};
     if ((long)a.q.T * a.rep / (KV8_FEW + 1) < a.q.n) a.many.z = Kv8Cut{a.rep, KV8_MANY, 0, KV8_FEW + 1};
     a.many.cols = KV8_MANY;
     const long full = (long)a.q.T * a.rep / KV8_MANY + 1;
-    return few + split_pages(a, a.many, full + (kv8_slots(a.q, a.many.z) - full) / 4, cap, room - few);
+    return few + split_pages(a, a.many, full + (kv8_slots(a.q, a.many.z) - full) / 4, cap, room - few, KV8_TILES, 1);
 }
 void tlm_kv8_workspace(TlmKv8Attn& a, float* w) {
     for (Kv8Share* h : {&a.few, &a.many}) {
@@ -184,6 +185,7 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     int rc;
     if ((rc = check_cache(cache, &a->c, "mmi_kv_attend")) || (rc = check_seqs(seqs, &a->q, "mmi_kv_attend"))) return rc;
     if (heads < 1 || heads % cache->kv_heads || heads / cache->kv_heads > 1024) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: query heads are a multiple of the key/value heads, at most 1024 times");
+    if ((int64_t)seqs->rows * (heads / cache->kv_heads) > 0x7fffffff) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^31 - 1 rows of a group's heads");
     if (window < 0 || keep_first < 0) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: negative window");
     a->heads = heads;
     a->rep = heads / cache->kv_heads;
