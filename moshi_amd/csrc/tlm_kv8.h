@@ -445,6 +445,7 @@ struct Kv8Share {                        // one kernel's part of a call
     int pages, nsplit;                   // pages per split; splits that a group can need
     float* po;                           // nsplit > 1: [group slot][kv head][split][z.per columns][vdim] un-normalised sums
     float* pml;                          // [group slot][kv head][split][2][z.per]: running maximum, sum of weights
+    int* what;                           // [group slot][4]: its columns, the splits that were needed, first row and column of its sequence
 };
 struct TlmKv8Attn {
     TlmKv8Cache c;
@@ -496,6 +497,11 @@ struct Kv8Pages {
         return mmi_from_lane(held, i - from);
     }
 };
+// for the kernel that joins the splits, which would have to look for it in every wave (of 64 sequences with 4 rows each, 20 us for slots without a column)
+__device__ __forceinline__ void kv8_tell(const Kv8Share& h, const Kv8Cols& c, int slot, int g, int split) {
+    if (h.nsplit > 1 && g == 0 && split == 0 && threadIdx.x == 0)
+        *(u32x4*)(h.what + 4 * slot) = u32x4{(unsigned)max(0, c.ncol - c.c0), (unsigned)max(1, (c.n + h.pages - 1) / h.pages), (unsigned)c.s.row0, (unsigned)c.c0};
+}
 // a value scale = fraction 2^exponent (at least 2^-120; a NaN's fraction is one), and 2^-exponent
 __device__ __forceinline__ float kv8_fraction(float scale, float& exponent, float& back) {
     const float v = scale < 0x1p-120f ? 0x1p-120f : scale;
@@ -640,6 +646,7 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     constexpr int NP = D / 64, ND = D / 16, WK = 4;
     const int lane = (int)threadIdx.x & 63, wave = mmi_uniform((int)threadIdx.x >> 6), bl = lane & 15, kq = lane >> 4;
     const Kv8Cols c(a, a.few, true, slot);
+    kv8_tell(a.few, c, slot, g, split);
     const int i0 = split * a.few.pages, i1 = min(c.n, i0 + a.few.pages);
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
     const int col = min(c.c0 + bl, c.ncol - 1), tok = col / a.rep, pos = c.s.pos0 + tok;
@@ -821,6 +828,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
     constexpr int QT = Z::QT, KS = Z::KS, DT = Z::DT, KU = D > 128 ? 2 : 1;      // units of 16 codes per thread and side
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = mmi_uniform(tid >> 6), cl = lane & 31, hi = lane >> 5;
     const Kv8Cols c(a, a.many, false, slot);
+    kv8_tell(a.many, c, slot, g, split);
     const int i0 = 2 * split * a.many.pages;
     int i1 = min(2 * c.n, i0 + 2 * a.many.pages);
     if (i1 == 2 * c.n && c.n > 0 && c.page(c.n - 1) * TLM_PAGE + 32 > c.phi) --i1;      // (the last page's second half lies ahead of every column)
@@ -1107,6 +1115,7 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
     const Kv8Share& h = few ? a.few : a.many;
     const int b = at - (few ? 0 : first_many), each = kv8_joined(h.cols, a.c.vdim, WIDE), slot = b / each, per = h.z.per, g = (int)blockIdx.y;
     const long part = ((long)slot * a.c.kv_heads + g) * h.nsplit;
+    const int cols = mmi_load_const(h.what + 4 * slot), ns = mmi_load_const(h.what + 4 * slot + 1), row0 = mmi_load_const(h.what + 4 * slot + 2), c0 = mmi_load_const(h.what + 4 * slot + 3);
     if constexpr (!WIDE) {
         const int lane = tid & 63, G = a.c.vdim / 4, at_once = 64 / G, n = (b - slot * each) * at_once + lane / G, d = 4 * (lane % G);
         const bool on = lane / G < at_once && n < h.cols;
@@ -1126,9 +1135,8 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
                 }
         };
         if (few) load(0, h.nsplit);                        // (single tokens: asked for before it is known how many splits there were)
-        const Kv8Cols c(a, h, few, slot);
-        const int col = c.c0 + n, ns = max(1, (c.n + h.pages - 1) / h.pages);
-        if (!on || col >= c.ncol) return;
+        const int col = c0 + n;
+        if (!on || n >= cols) return;
         if (!few) load(0, ns);                             // (of the slots that portions might need, half are empty)
         float M = -INFINITY, L = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -1152,14 +1160,13 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
             load(k0, ns);
         }
         const int tok = col / a.rep;
-        kv8_store<Tr>(a, c.s.row0 + tok, g * a.rep + col - tok * a.rep, d, o * kv8_inverse(L, M, a.sink));
+        kv8_store<Tr>(a, row0 + tok, g * a.rep + col - tok * a.rep, d, o * kv8_inverse(L, M, a.sink));
     } else {
         MMI_SHARED float wt[256], red[4][2];
         MMI_SHARED __attribute__((aligned(16))) f32x4 sum[256];
         const int n = b - slot * each;
-        const Kv8Cols c(a, h, few, slot);
-        const int col = c.c0 + n, ns = max(1, (c.n + h.pages - 1) / h.pages);      // (at most 256)
-        if (col >= c.ncol) return;
+        const int col = c0 + n;                            // (ns: at most 256)
+        if (n >= cols) return;
         const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
         float m = -INFINITY, l = 0.f;
         if (tid < ns) {
@@ -1190,7 +1197,7 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
             if (k == 0 && d < a.c.vdim) {
 #pragma unroll
                 for (int i = 1; i < 16; ++i) v += sum[16 * i + q];
-                kv8_store<Tr>(a, c.s.row0 + tok, head, d, v * inv);
+                kv8_store<Tr>(a, row0 + tok, head, d, v * inv);
             }
         }
     }

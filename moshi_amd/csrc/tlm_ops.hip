@@ -95,13 +95,14 @@ size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, size
     cap = std::max(cap, 1l);
     const long units = std::max(1l, groups * a.c.kv_heads);
     const size_t each = (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.z.per * (a.c.vdim + 2);      // floats per split
-    long most = std::min<long>(KV8_MAX_SPLIT, (long)(room / std::max<size_t>(1, each)));
+    const size_t what = 4 * (size_t)kv8_slots(a.q, h.z);
+    long most = room > what ? std::min<long>(KV8_MAX_SPLIT, (long)((room - what) / std::max<size_t>(1, each))) : 1;
     if (most < 2) most = 1;
     long per = std::max((cap * units + aim - 1) / aim, (cap + most - 1) / most);
     per = std::min((per + step - 1) / step * step, (cap + step - 1) / step * step);
     h.pages = (int)per;
     h.nsplit = (int)((cap + per - 1) / per);
-    return h.nsplit > 1 ? each * h.nsplit : 0;
+    return h.nsplit > 1 ? each * h.nsplit + what : 0;
 }
 
 }  // namespace
@@ -139,6 +140,8 @@ void tlm_kv8_workspace(TlmKv8Attn& a, float* w) {
         h->po = w;
         h->pml = w + parts * a.c.vdim;
         w += parts * (a.c.vdim + 2);
+        h->what = (int*)w;
+        w += 4 * kv8_slots(a.q, h->z);
     }
 }
 
