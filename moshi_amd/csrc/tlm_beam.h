@@ -50,7 +50,7 @@ __device__ __forceinline__ float beam_exp(float d, float low) {
 
 // A wave's best: the `beams`-th largest of the lanes' maxima is a bound that as many logits reach, and few more do, one or two beyond `beams` of
 // 1024 distinct ones: these are put side by side and ranked by counting who is before whom.  Where more than 64 reach it (equal logits), they are
-// taken out one at a time.  grid: chunks / 4, rows
+// taken out one at a time.  Reads the logits once: 128 rows of 65521 fp32 13 us, 2.5 TB/s, 4 rows of 32000 5.3 us.  grid: chunks / 4, rows
 template <class In>
 __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
     constexpr int N = BEAM_CHUNK / 64;                     // logits per lane, in runs of four
@@ -156,7 +156,9 @@ __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
 
 // A workgroup per request: 4096 of its candidates at a time in registers, 16 a lane, beside the best found so far.  As in the rows, a bound that
 // `beams` lanes of one wave reach leaves few to be ranked by counting; ranks rounded to 32 bits keep their order, which is all a bound needs.  A
-// candidate's place is beam * V + token.  (One at a time, a maximum over the workgroup for each: 25 us for 8 beams, 16 requests.)
+// candidate's place is beam * V + token.  Latency from end to end, chunks' sums, their logarithms,
+// candidates, bound, ranks: 6.8 us for 4 beams of 32000, 14.5 us for 16 requests with 8 beams of 65521.  (Candidates taken one at a time, a maximum over the
+// workgroup for each: 25 us there.)
 __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
     constexpr int N = 16;
     MMI_SHARED double base[BEAM_MAX], inv[BEAM_MAX], bx[2][4], kx[2][BEAM_MAX];      // base: score - log sum exp; inv: 1 / length^alpha; kx: the best, in order
@@ -359,7 +361,8 @@ struct TlmReorder {
 };
 // A lane owns a unit of the request's rows: it has read all of it before it writes any, so rows may change places.  Rows that stay are not written,
 // and in their place a row that some other one needs is asked for again: a load behind a branch would wait for the one before it (315 us
-// instead of 195 for 64 rows of 13 MB).
+// instead of 188 for 64 rows of 13 MB, with random parents 1.2 GB: 6.6 TB/s, above a large copy's 4.9, since a row that two children
+// take is read once).  Four rows of 3.4 MB: 5.5 us, a launch and one round trip.  Instances by the beams, since their registers are a lane's.
 template <class U, int K>
 __device__ __forceinline__ void beam_move(const TlmReorder::T& t, const int (&from)[K], const int (&to)[K], unsigned moved, unsigned u) {
     U v[K];

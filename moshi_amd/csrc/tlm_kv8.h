@@ -169,10 +169,10 @@ struct Kv8Span { int page, part, lo, hi, row, pos; bool none; };
 __device__ __forceinline__ Kv8Span kv8_span(const TlmKv8Seqs& q, const Kv8Cut& z, int n_pages, int slot) {
     const int e = kv8_find(q, z, slot);
     const TlmKv8Seq s = kv8_seq(q, e);
-    const int b = s.pos0 / KV8_BLOCK + slot - kv8_slot0(q, z, e);      // block of the sequence
+    const int i = slot - kv8_slot0(q, z, e), b = s.pos0 / KV8_BLOCK + i;      // block of the sequence
     Kv8Span o;
     o.pos = b * KV8_BLOCK;
-    o.none = s.len < 1 || o.pos >= s.pos0 + s.len;
+    o.none = s.len < 1 || i < 0 || o.pos >= s.pos0 + s.len;      // (i < 0: row starts that do not ascend)
     o.lo = max(s.pos0 - o.pos, 0);
     o.hi = min(s.pos0 + s.len - o.pos, KV8_BLOCK);
     o.row = s.row0 + o.pos - s.pos0;               // row of the block's first token (of token lo on they are the call's)
@@ -233,6 +233,8 @@ __device__ __forceinline__ void kv8_put_angle(const TlmKv8Cache& c, float* cs, f
 // token of the call read its nearest), and the common path is short.
 // grid: slots of blocks, kv heads / 4, 2 (keys, values)
 //   keys: four lanes per token, granules of 4 dimensions in turn      values: a lane per dimension, its 16 tokens side by side
+// Measured (8 heads of 128, bf16): 3.6k tokens in three portions 13 us for 25 MB, the rest latency; one token 5.8 us, 64 tokens 7.0 us, of which an
+// empty launch is 1.4.  Heads of up to 128 dimensions have an instance of their own (68 registers; as the one for 256, 117 and half the waves on a CU).
 template <class In, bool E4M3, int D>
 __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void k_tlm_kv8_append(TlmKv8Append a) {
     typedef Kv8Code<E4M3> C;
@@ -378,6 +380,7 @@ __device__ __forceinline__ void kv8_put4(float* p, f32x4 v) { TlmF32::store4(p, 
 __device__ __forceinline__ void kv8_put4(uint16_t* p, f32x4 v) { TlmBf16::store4(p, v); }
 __device__ __forceinline__ void kv8_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void kv8_put(uint16_t* p, float v) { *p = mmi_f32_to_bf16(v); }
+// Eight loads a lane on their way, then stores: 3.6k tokens of 8 heads of 128 in bf16 11 us for 25 MB, 64 tokens 7 us (positions, page, codes: a chain).
 // grid: slots of blocks, kv heads, 2
 template <class Out, bool E4M3>
 __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
@@ -434,7 +437,9 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
 // it by 2^6.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both operands come in two parts, 22 bits, good to 2^-24.
 // (bf16 operands left 1.8 times the error of the result's rounding.)  Sums, maxima and the denominator, which has the weights before they were
 // rounded, are fp32.
-constexpr int KV8_FEW = 16;              // sequences with up to so many columns, one tile, are the few's where a call may bring longer ones
+// Sequences with up to so many columns, one tile, are the few's where a call may bring longer ones: 64 sequences with 4 rows of 4 heads, 2000 keys each,
+// take 52 us there and 101 us as the many's; 2 with 20 000 keys, 27 and 46 us.  (A second tile would read every key again.)
+constexpr int KV8_FEW = 16;
 constexpr int KV8_MANY = 128;            // columns of a workgroup of the many's
 constexpr float KV8_UP = 8.f, KV8_SLACK = 6.f;      // log2: of what weights are carried times, of what they may outgrow it by (fp16 ends at 2^16)
 constexpr int KV8_ANGLES = 2048;         // pairs of a cosine and a sine in LDS
@@ -471,6 +476,7 @@ struct Kv8Cols {
         c0 = (slot - kv8_slot0(a.q, h.z, e)) * per;
         ncol = s.len * a.rep;
         plo = phi = n = n0 = b0 = 0;
+        if (c0 < 0) c0 = ncol = 0;                         // (row starts that do not ascend)
         if (a.both && (ncol <= KV8_FEW) != few) ncol = 0;
         if (c0 >= ncol) return;
         plo = s.pos0 + c0 / a.rep;
@@ -478,8 +484,9 @@ struct Kv8Cols {
         const int w = a.mask.window;
         b0 = w > 0 && plo - w + 1 > 0 ? (plo - w + 1) / TLM_PAGE : 0;
         n0 = w > 0 ? min(b0, (a.mask.keep + TLM_PAGE - 1) / TLM_PAGE) : 0;
+        if (!a.q.ring) n0 = min(n0, a.q.pages.ld);
         n = n0 + phi / TLM_PAGE + 1 - b0;
-        if (!a.q.ring) n = min(n, n0 + max(a.q.pages.ld - b0, 0));
+        if (!a.q.ring) n = min(n, n0 + max(a.q.pages.ld - b0, 0));      // (so that the splits, as many as a sequence of `ld` pages needs, are enough)
     }
     __device__ __forceinline__ int page(int i) const { return i < n0 ? i : b0 + i - n0; }
 };
@@ -637,7 +644,8 @@ __device__ __forceinline__ float kv8_inverse(float L, float M, int sink) {
 }
 
 // Few columns: four waves share one tile of 16 columns, each takes every fourth of its pages straight from the cache - the page after it is
-// asked for before the products of this one - and their sums meet in LDS.
+// asked for before the products of this one - and their sums meet in LDS.  Bound by the codes' way from memory: 100 003 keys of 8 heads of 128
+// 41.5 us at 4.9 TB/s, as fast as a large copy; 64 sequences of 800 to 4096 keys 77 us at 4.2 TB/s, the longest ones' end is not full.
 // LDS: the queries and their angles, then (the same memory) the waves' sums
 constexpr int KV8_LDS = 4 * 8 * 64;                        // vectors of four floats: 8 waves' worth of 8 x 16 dimensions; queries of 256 in two parts and angles take 2048 too
 template <class In, class Tr, int NS, int D, bool E4M3>
@@ -809,6 +817,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8At
     tlm_kv8_attn<In, Tr, NS, D, E4M3>(a, ob, ml, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
 }
 
+// 128 columns and not 256: with two tiles a wave, accumulators leave one workgroup on a CU and moves between register files (422 us instead of 227).
+// A prompt of 4001 tokens, 32 heads of 128 over 8: 218 us, 601 TFLOP/s, half of what a large bf16 product reaches here; bound by the vector work between
+// the products (exponentials, masks, the conversion of codes and weights).
 // Many columns: four waves x QT tiles of 32 columns of one sequence and kv head walk the same keys, 32 at a time.  Codes become operand
 // fragments on their way into LDS, once for all waves; 32 x 32 products read an operand half as often as 16 x 16 ones.  The scores of step
 // i + 1 are formed beside the softmax of step i; keys lie two steps ahead of their use and values one, one barrier a step.
@@ -1103,8 +1114,10 @@ __global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(Tlm
     }
 }
 
-// The splits of one column -> output.  grid: columns of all slots (first the few's, then the many's), kv heads.
-// Up to 16 splits (WIDE false): a wave for every 64 / (vdim / 4) columns, four dimensions a lane, all partial sums asked for at once.  More: a
+// The splits of one column -> output.  A chain of two round trips behind a launch: 3.9 us for 5 sequences (the wide one: 5.0), 5.6 us for 56 splits of
+// one (the other: 8.6), 7.8 us for 16 sequences with 560 tokens (the wide one: 46).
+//  grid: columns of all slots (first the few's, then the many's), kv heads.
+// Up to 16 splits (WIDE false): a wave for every 64 / (vdim / 4) columns, four dimensions a lane, eight partial sums asked for at once.  More: a
 // workgroup per column, 16 groups of lanes take every 16th split, and their sums meet in LDS.
 MMI_HD int kv8_joined(int cols, int vdim, bool wide) { return wide ? cols : (cols + 256 / vdim - 1) / (256 / vdim); }      // waves (wide: workgroups) per slot
 template <class Tr, bool WIDE>

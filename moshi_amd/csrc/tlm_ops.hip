@@ -69,7 +69,7 @@ int launch_attn(hipStream_t s, const TlmKv8Attn& a) {
     } else {
         MMI_LAUNCH((k_tlm_kv8_attn<In, Tr, NS, D, E4M3>), dim3((unsigned)kv8_slots(a.q, a.few.z), a.c.kv_heads, a.few.nsplit), 256, 0, s, a);
     }
-    const bool wide = std::max(a.few.nsplit, a.both ? a.many.nsplit : 1) > 16;
+    const bool wide = std::max(a.few.nsplit, a.both ? a.many.nsplit : 1) > 16;      // (both sides measured: k_tlm_kv8_combine)
     auto joined = [&](const Kv8Share& h) { return h.nsplit > 1 ? (int)kv8_slots(a.q, h.z) * kv8_joined(h.cols, a.c.vdim, wide) : 0; };
     const int few = joined(a.few), all = few + (a.both ? joined(a.many) : 0);
     if (all && wide) MMI_LAUNCH((k_tlm_kv8_combine<Tr, true>), dim3(all, a.c.kv_heads), 256, 0, s, a, few, all);
@@ -188,7 +188,6 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     int rc;
     if ((rc = check_cache(cache, &a->c, "mmi_kv_attend")) || (rc = check_seqs(seqs, &a->q, "mmi_kv_attend"))) return rc;
     if (heads < 1 || heads % cache->kv_heads || heads / cache->kv_heads > 1024) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: query heads are a multiple of the key/value heads, at most 1024 times");
-    if ((int64_t)seqs->rows * (heads / cache->kv_heads) > 0x7fffffff) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^31 - 1 rows of a group's heads");
     if (window < 0 || keep_first < 0) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: negative window");
     a->heads = heads;
     a->rep = heads / cache->kv_heads;
@@ -196,6 +195,10 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     a->mask = TlmMask{window, window > 0 ? keep_first : 0, 0.f};
     if ((long)a->q.T * a->rep > 1l << 26) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^26 rows times query heads of a group");
     *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1, (size_t)1 << 30);
+    long groups = 0;
+    for (const Kv8Share* h : {&a->few, &a->many})
+        if (h->nsplit) groups += kv8_slots(a->q, h->z) * (long)cache->kv_heads * h->nsplit;
+    if (groups > 1l << 23) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: too many sequences, rows and heads for one call");      // (2^31 lanes a launch)
     return MMI_OK;
 }
 }  // namespace

@@ -167,7 +167,7 @@ def run_token_lm(args) -> None:
     t0 = time.time()
     if args.beams > 1:
         eos = args.stop_token[0] if args.stop_token else -1
-        out = [h[0].tokens for h in beam_search(lm, prompts, args.beams, args.max_new_tokens, eos, args.length_penalty, step_tokens)]
+        out = [h[0].tokens if h else [] for h in beam_search(lm, prompts, args.beams, args.max_new_tokens, eos, args.length_penalty, step_tokens)]
     else:
         out = TokenBatcher(lm, step_tokens=step_tokens, seed=args.seed).generate(prompts, args.max_new_tokens, temp=0.0 if args.greedy else args.temp, top_k=args.top_k,
                                                                                  stop=args.stop_token)

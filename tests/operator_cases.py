@@ -900,3 +900,49 @@ def check_beam_search_of_one(dev, lib, name="mixed"):
         with pytest.raises(ValueError):
             beam_search(lm, *bad)
     assert beam_search(lm, [], 2, 4) == [] and lm.free_slots == 2 and lm.free_pages == lm.total_pages
+
+
+# ---- calls that the documentation allows, at its edges ----------------------------------------------------------------------------
+def _filled(dev, lib, pages, tokens, codes="int8", dim=32):
+    """A cache of one head with one sequence's tokens in pages 0, 1, ..; the values it holds, in 64 bits."""
+    g = torch.Generator().manual_seed(4)
+    cache = PagedKVCache.empty(pages, 1, dim, codes=codes, device=dev, lib=lib)
+    k, v = [torch.randn((tokens, 1, dim), generator=g).to(dev) for _ in range(2)]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+    cache.append(k, v, table, i32(0), i32(0, tokens))
+    held = [x[:, 0].double().cpu() for x in cache.read(table, i32(0), i32(0, tokens), tokens=tokens)]
+    return cache, table, held, i32, g
+
+
+def check_position_past_the_table(dev, lib, codes="int8"):
+    """Far behind the last page that the table names, the kept first tokens (more of them than it names) are all there is to see."""
+    cache, table, (k, v), i32, g = _filled(dev, lib, 8, 512, codes)
+    for n in (1, 20):
+        q = torch.randn((n, 2, 32), generator=g).to(dev)
+        for keep in (2000, 100):
+            got = cache.attend(q, table, i32(10000), None if n == 1 else i32(0, n), window=64, keep_first=keep)
+            s = torch.einsum("rhd,td->rht", q.double().cpu(), k[:keep]) * 32 ** -0.5
+            want = torch.softmax(s, dim=-1) @ v[:keep]
+            # operands of 22 bits, sums in 32: as for the other fp32 cases
+            assert torch.allclose(got.double().cpu(), want, rtol=2.0 ** -16, atol=2.0 ** -18), (n, keep)
+        assert not cache.attend(q, table, i32(10000), None if n == 1 else i32(0, n), window=64).any()
+
+
+def check_rows_in_no_order(dev, lib):
+    """Row starts that do not ascend are no sequences; whatever becomes of those rows, the memory beside the tensors stays as it is."""
+    cache, table, _, i32, g = _filled(dev, lib, 8, 300)
+    tables = table.expand(4, 8).contiguous()
+    for rows in ((0, 40, 10, 60, 25), (60, 0, 60, 0, 60), (50, 40, 30, 20, 10), (-5, 70, 1 << 30, -(1 << 30), 3)):
+        q = torch.full((60 + 128, 2, 32), 7.0, device=dev)
+        out = torch.full((60 + 128, 2, 32), 7.0, device=dev)
+        q[64:124] = torch.randn((60, 2, 32), generator=g).to(dev)
+        cache.attend(q[64:124], tables, i32(100, 200, 299, 0), i32(*rows), out=out[64:124])
+        assert (out[:64] == 7).all() and (out[124:] == 7).all(), rows
+        before = [t.clone() for t in (cache.k_scale, cache.v_scale)]
+        big = torch.full((60 + 128, 1, 32), 1e30, device=dev)                         # (what lies beside the rows would show in a scale)
+        big[64:124] = 0.01
+        cache.append(big[64:124], big[64:124], tables, i32(100, 200, 299, 0), i32(*rows))
+        assert max(float(t.max()) for t in (cache.k_scale, cache.v_scale)) <= max(float(t.max()) for t in before), rows
+        kv = cache.read(tables, i32(100, 200, 299, 0), i32(*rows), tokens=60)
+        assert kv[0].shape == (60, 1, 32)

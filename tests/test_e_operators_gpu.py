@@ -198,3 +198,12 @@ def test_beam_search(lib, name, codes, alpha, dtype):
 
 def test_beam_search_of_one(lib):
     oc.check_beam_search_of_one(DEV, lib)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_position_past_the_table(lib, codes):
+    oc.check_position_past_the_table(DEV, lib, codes)
+
+
+def test_rows_in_no_order(lib):
+    oc.check_rows_in_no_order(DEV, lib)

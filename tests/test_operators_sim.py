@@ -101,3 +101,12 @@ def test_beam_search(tlm_lib, name, codes, alpha):  # noqa: F811
 
 def test_beam_search_of_one(tlm_lib):  # noqa: F811
     oc.check_beam_search_of_one(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_position_past_the_table(tlm_lib, codes):  # noqa: F811
+    oc.check_position_past_the_table(DEV, tlm_lib, codes)
+
+
+def test_rows_in_no_order(tlm_lib):  # noqa: F811
+    oc.check_rows_in_no_order(DEV, tlm_lib)
