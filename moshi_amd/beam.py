@@ -8,7 +8,7 @@
 """
 from __future__ import annotations
 
-import ctypes as C
+from array import array
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -78,13 +78,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
         if len(_need) > 4096:
             _need.clear()
         _need[batch, beams, vocab] = need
-    parents, tokens, grown = torch.empty((3, batch, beams), dtype=_I32, device=device).unbind()
-    r = BeamChoice(torch.empty(shape, dtype=_F32, device=device), parents, tokens, torch.empty(shape, dtype=_BOOL, device=device) if eos >= 0 else None,
-                   None if lengths is None else grown)
-    work = torch.empty(need, dtype=torch.uint8, device=device)
+    like = torch.empty_like                                # (a third of what `empty` with its arguments takes)
+    parents, tokens = like(scores, dtype=_I32), like(scores, dtype=_I32)
+    r = BeamChoice(like(scores), parents, tokens, like(scores, dtype=_BOOL) if eos >= 0 else None, None if lengths is None else like(lengths))
+    work = scores.new_empty(need, dtype=torch.uint8)
     lib.check(on.call(lib.mmi_beam_select, batch, beams, vocab, dtype, logits.data_ptr(), row, scores.data_ptr(), None if lengths is None else lengths.data_ptr(),
                       None if finished is None else finished.data_ptr(), eos, length_penalty, r.scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-                      None if eos < 0 else r.finished.data_ptr(), None if lengths is None else grown.data_ptr(), work.data_ptr(), need))
+                      None if eos < 0 else r.finished.data_ptr(), None if lengths is None else r.lengths.data_ptr(), work.data_ptr(), need))
     return r
 
 
@@ -112,8 +112,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, lib: Opt
             if not t[:1].is_contiguous():
                 raise ValueError("a state's rows are contiguous, on the parents' device")
             stride.append(t.stride(0) * t.element_size())
-    n = len(at)
-    lib.check(on.call(lib.mmi_beam_reorder, n, (C.c_void_p * n)(*at), (C.c_int64 * n)(*stride), (C.c_int64 * n)(*size), batch, beams, parents.data_ptr()))
+    lists = [array("q", x) for x in (at, stride, size)]
+    lib.check(on.call(lib.mmi_beam_reorder, len(at), *[x.buffer_info()[0] for x in lists], batch, beams, parents.data_ptr()))
 
 
 @dataclass

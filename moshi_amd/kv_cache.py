@@ -136,14 +136,14 @@ class PagedKVCache:
         total = q.shape[0]
         seqs = self._seqs(table, positions, rows, total)
         if out is None:
-            out = torch.empty((total, heads, self.vdim), dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q) if self.vdim == self.dim and q.is_contiguous() else q.new_empty((total, heads, self.vdim))
             op = (out.data_ptr(), heads * self.vdim, self.vdim)
         else:
             if out.shape != (total, heads, self.vdim) or out.dtype != q.dtype:
                 raise AssertionError("out is [rows, heads, vdim] in the queries' type")
             op = self._rows(out, "out", heads, self.vdim)[2]
         need = self._workspace(seqs, (seqs.n, total, seqs.table_ld, heads, window, keep_first, rows is None))
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        work = q.new_empty(need, dtype=torch.uint8) if need else None
         self._lib.check(self._on.call(self._lib.mmi_kv_attend, C.byref(self._desc), C.byref(seqs), dtype, heads, *qp, *op, self.dim ** -0.5 if scale is None else scale, window,
                                       keep_first, sink, work.data_ptr() if need else None, need))
         return out
@@ -158,7 +158,7 @@ class PagedKVCache:
         if dtype not in _DTYPES:
             raise ValueError("dtype must be torch.bfloat16 or torch.float32")
         seqs = self._seqs(table, positions, rows, total)
-        k = torch.empty((total, self.kv_heads, self.dim), dtype=dtype, device=self.device)
-        v = torch.empty((total, self.kv_heads, self.vdim), dtype=dtype, device=self.device)
+        k = self.k_scale.new_empty((total, self.kv_heads, self.dim), dtype=dtype)
+        v = torch.empty_like(k) if self.vdim == self.dim else k.new_empty((total, self.kv_heads, self.vdim))
         self._lib.check(self._on.call(self._lib.mmi_kv_read, C.byref(self._desc), C.byref(seqs), _DTYPES[dtype], k.data_ptr(), v.data_ptr()))
         return k, v
