@@ -818,7 +818,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8At
 }
 
 // 128 columns and not 256: with two tiles a wave, accumulators leave one workgroup on a CU and moves between register files (422 us instead of 227).
-// A prompt of 4001 tokens, 32 heads of 128 over 8: 218 us, 601 TFLOP/s, half of what a large bf16 product reaches here; bound by the vector work between
+// A prompt of 4001 tokens, 32 heads of 128 over 8: 215 us, 610 TFLOP/s, half of what a large bf16 product reaches here; bound by the vector work between
 // the products (exponentials, masks, the conversion of codes and weights).
 // Many columns: four waves x QT tiles of 32 columns of one sequence and kv head walk the same keys, 32 at a time.  Codes become operand
 // fragments on their way into LDS, once for all waves; 32 x 32 products read an operand half as often as 16 x 16 ones.  The scores of step
