@@ -8,7 +8,7 @@
 #pragma once
 #include "tlm_common.h"
 
-constexpr int BEAM_CHUNK = 1024, BEAM_TENSORS = 48;
+constexpr int BEAM_CHUNK = 1024, BEAM_TENSORS = 48, BEAM_LISTS = 1024;
 
 struct TlmBeamArgs {
     const void* x; long ld;              // logits, row stride in elements
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
     MMI_SHARED int kind[BEAM_MAX], bi[2][4], kp[2][BEAM_MAX];                        // kind 0: a row of logits; 1: finished; 2: no candidate with a chance
     MMI_SHARED float ks[2][BEAM_MAX], wb[4], cs[4][64];
     MMI_SHARED double cx[4][64];
-    MMI_SHARED int cp[4][64], cn[4];
+    MMI_SHARED int cp[4][64], cn[4], pick[BEAM_LISTS];
     const int b = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.beams;
     // candidate n of the request: entry n % K of chunk n / K % chunks of beam n / K / chunks
     const unsigned per = (unsigned)a.chunks * (unsigned)K;
@@ -174,15 +174,41 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
     double x[N + 1];
     int p[N + 1];
     float y[N + 1];
+    int total = all;                                       // candidates that are looked at
+    bool some = false;                                     // they are those of the lists in pick
+    const float one_k = 1.f / (float)K, one_per = 1.f / (float)per;
+    auto quotient = [](int n, int d, float one) __attribute__((always_inline)) {      // n / d (n is below 2^21: at most one off)
+        int k = (int)((float)n * one);
+        if (k * d > n) --k;
+        else if ((k + 1) * d <= n) ++k;
+        return k;
+    };
+    auto place = [&](int n) __attribute__((always_inline)) {
+        if (!some) return n;
+        const int l = quotient(n, K, one_k);
+        return pick[l] * K + n - l * K;
+    };
     auto ask = [&](int n0) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int n = min(n0 + tid + 256 * j, all - 1);
+            if (j && n0 + 256 * j >= total) break;
+            const int n = place(min(n0 + tid + 256 * j, total - 1));
             p[j] = a.wi[first + n];
             y[j] = a.wx[first + n];
         }
     };
-    ask(0);
+    // the largest value that `beams` lanes of the wave reach (-infinity: there is none)
+    auto reached = [&](float top) __attribute__((always_inline)) {
+        float bound = mmi_wave_max_f32(top), left = top;
+        for (int found = 0;;) {
+            found += __builtin_popcountll(mmi_ballot(left == bound));
+            if (found >= K || bound == -INFINITY) break;
+            if (left == bound) left = -INFINITY;
+            bound = mmi_wave_max_f32(left);
+        }
+        return bound;
+    };
+    if (all <= 256 * N) ask(0);
     // two rows a wave at once, a chunk a lane; then a beam a lane: its score and its length's power, in 64 bits
     const bool mine = tid < K, done = mine && a.done && a.done[b * K + tid];
     const double score = mine ? (double)a.score[b * K + tid] : 0.;
@@ -221,12 +247,53 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         inv[tid] = a.alpha == 0. ? 1. : (a.alpha == 1. ? 1. / (double)max(len, 1) : pow((double)max(len, 1), -a.alpha));
         kind[tid] = z > -INFINITY && z < INFINITY ? (done ? 1 : 0) : 2;
     }
-    const float one_per = 1.f / (float)per;
+    float least = -INFINITY;                               // as many candidates as there are beams reach it
+    if (all > 256 * N) {
+        // Lists are in order, so the first ones of each tell which lists can have a candidate at all: those whose first reaches a bound that as many
+        // firsts reach.
+        const int lists = K * a.chunks;
+        const float one_chunk = 1.f / (float)a.chunks;
+        auto head = [&](int i) __attribute__((always_inline)) {
+            const int k = quotient(i, a.chunks, one_chunk);
+            double s = -INFINITY;
+            if (kind[k] == 0) s = base[k] + (double)a.wx[first + (long)i * K];
+            else if (kind[k] == 1 && i == k * a.chunks) s = base[k];
+            return (float)(s * inv[k]);
+        };
+        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int i = tid; i < lists; i += 256) top = fmaxf(top, head(i));
+        const float bound = reached(top);
+        if (lane == 0) wb[wave] = bound;
+        __syncthreads();
+        least = fmaxf(fmaxf(wb[0], wb[1]), fmaxf(wb[2], wb[3]));
+        if (least > -INFINITY) {
+            int count = 0;
+            for (int i0 = 0; i0 < lists; i0 += 256) count += __builtin_popcountll(mmi_ballot(i0 + tid < lists && head(min(i0 + tid, lists - 1)) >= least));
+            if (lane == 0) cn[wave] = count;
+            __syncthreads();
+            if (cn[0] + cn[1] + cn[2] + cn[3] <= BEAM_LISTS) {
+                int at = 0;
+                for (int w = 0; w < wave; ++w) at += cn[w];
+                for (int i0 = 0; i0 < lists; i0 += 256) {
+                    const bool in = i0 + tid < lists && head(min(i0 + tid, lists - 1)) >= least;
+                    const uint64_t who = mmi_ballot(in);
+                    if (in) pick[at + mmi_below(who)] = i0 + tid;
+                    at += __builtin_popcountll(who);
+                }
+                some = true;
+                total = (cn[0] + cn[1] + cn[2] + cn[3]) * K;
+            }
+            __syncthreads();
+        }
+        ask(0);
+    }
     x[N] = -INFINITY;
     p[N] = BEAM_NONE;
     y[N] = -INFINITY;
     int set = 0;
-    for (int n0 = 0; n0 < all; n0 += 256 * N, set ^= 1) {
+    for (int n0 = 0; n0 < total; n0 += 256 * N, set ^= 1) {
         if (n0) ask(n0);
         __syncthreads();
         if (n0 && tid < K) {                               // (place BEAM_NONE: there was none)
@@ -236,23 +303,22 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            if (n0 + 256 * j >= all) {                     // (one request's few candidates leave most places empty)
+            if (n0 + 256 * j >= total) {                   // (one request's few candidates leave most places empty)
                 p[j] = BEAM_NONE;
                 continue;
             }
-            const int n = n0 + tid + 256 * j;
-            int k = (int)((float)n * one_per);             // n / per (n is below 2^21: at most one off)
-            if (k * (int)per > n) --k;
-            else if ((k + 1) * (int)per <= n) ++k;
+            const bool there = n0 + tid + 256 * j < total;
+            const int n = place(min(n0 + tid + 256 * j, total - 1));
+            int k = quotient(n, (int)per, one_per);
             k = min(k, K - 1);
             const int h = n - k * (int)per;
-            int token = n < all ? p[j] : BEAM_NONE;
+            int token = there ? p[j] : BEAM_NONE;
             double s = -INFINITY;
             if (kind[k] == 0) {
                 if (token != BEAM_NONE) s = base[k] + (double)y[j];
             } else {                                       // no logits to choose from: the end token, then what else there is, in order, as the first entries
                 token = kind[k] == 2 ? h : (h == 0 ? a.eos : (h - 1 < a.eos ? h - 1 : h));
-                if (h >= K || n >= all || token >= a.V) token = BEAM_NONE;
+                if (h >= K || !there || token >= a.V) token = BEAM_NONE;
                 if (kind[k] == 1 && h == 0) s = base[k];
             }
             x[j] = s * inv[k];
@@ -262,24 +328,15 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j <= N; ++j)
-            if (j == N || n0 + 256 * j < all) top = fmaxf(top, p[j] == BEAM_NONE ? -INFINITY : (float)x[j]);
-        float bound = mmi_wave_max_f32(top);
-        {
-            float left = top;
-            for (int found = 0;;) {
-                found += __builtin_popcountll(mmi_ballot(left == bound));
-                if (found >= K || bound == -INFINITY) break;
-                if (left == bound) left = -INFINITY;
-                bound = mmi_wave_max_f32(left);
-            }
-        }
+            if (j == N || n0 + 256 * j < total) top = fmaxf(top, p[j] == BEAM_NONE ? -INFINITY : (float)x[j]);
+        float bound = reached(top);
         if (lane == 0) wb[wave] = bound;
         __syncthreads();
-        bound = fmaxf(fmaxf(wb[0], wb[1]), fmaxf(wb[2], wb[3]));
+        bound = fmaxf(fmaxf(fmaxf(wb[0], wb[1]), fmaxf(wb[2], wb[3])), least);
         int count = 0;
 #pragma unroll
         for (int j = 0; j <= N; ++j) {
-            if (j < N && n0 + 256 * j >= all) continue;
+            if (j < N && n0 + 256 * j >= total) continue;
             const bool in = p[j] != BEAM_NONE && (float)x[j] >= bound;
             const uint64_t at = mmi_ballot(in);
             if (!at) continue;

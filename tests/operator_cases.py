@@ -533,6 +533,16 @@ SELECTS = {
     "masked_altogether": dict(batch=2, beams=3, vocab=1100, masked=-math.inf, left=0),
     "not_finite": dict(batch=2, beams=4, vocab=1200, spoil=True),
     "strided": dict(batch=2, beams=3, vocab=513, pad=6),
+    # more candidates than are ranked at once
+    "many": dict(batch=2, beams=32, vocab=9000),
+    "many_finished": dict(batch=1, beams=20, vocab=12100, finished=0.4, penalty=0.8),
+    "many_bf16_ties": dict(batch=1, beams=24, vocab=10007, dtype=BF16, coarse=True),
+    "many_start": dict(batch=1, beams=32, vocab=5000, start=True),
+    "many_equal": dict(batch=1, beams=16, vocab=17000, equal=True),
+    "many_equal_lists": dict(batch=1, beams=32, vocab=33 * 1024, equal=True),
+    "many_masked_all_but_two": dict(batch=1, beams=24, vocab=9000, masked=-math.inf, left=2),
+    "many_masked_lowest": dict(batch=1, beams=24, vocab=9000, masked=-3.4028234663852886e38),
+    "many_not_finite": dict(batch=1, beams=24, vocab=9000, spoil=True),
 }
 
 
