@@ -9,6 +9,9 @@
 #include "tlm_common.h"
 
 constexpr int BEAM_CHUNK = 1024, BEAM_TENSORS = 48, BEAM_LISTS = 1024;
+// More candidates than this: their lists' first ones are looked at before the rest (2048 candidates of one request take 10.6 us with it and 10.1 us without,
+// 4096 of 16 requests 12.7 and 15.5 us, 32768 of 2 requests 35 and 216 us).
+constexpr int BEAM_FIRSTS = 2048;
 
 struct TlmBeamArgs {
     const void* x; long ld;              // logits, row stride in elements
@@ -157,7 +160,7 @@ __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
 // A workgroup per request: 4096 of its candidates at a time in registers, 16 a lane, beside the best found so far.  As in the rows, a bound that
 // `beams` lanes of one wave reach leaves few to be ranked by counting; ranks rounded to 32 bits keep their order, which is all a bound needs.  A
 // candidate's place is beam * V + token.  Latency from end to end, chunks' sums, their logarithms,
-// candidates, bound, ranks: 6.8 us for 4 beams of 32000, 14.5 us for 16 requests with 8 beams of 65521.  (Candidates taken one at a time, a maximum over the
+// candidates, bound, ranks: 6.8 us for 4 beams of 32000, 12.7 us for 16 requests with 8 beams of 65521.  (Candidates taken one at a time, a maximum over the
 // workgroup for each: 25 us there.)
 __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
     constexpr int N = 16;
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         }
         return bound;
     };
-    if (all <= 256 * N) ask(0);
+    if (all <= BEAM_FIRSTS) ask(0);
     // two rows a wave at once, a chunk a lane; then a beam a lane: its score and its length's power, in 64 bits
     const bool mine = tid < K, done = mine && a.done && a.done[b * K + tid];
     const double score = mine ? (double)a.score[b * K + tid] : 0.;
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
         kind[tid] = z > -INFINITY && z < INFINITY ? (done ? 1 : 0) : 2;
     }
     float least = -INFINITY;                               // as many candidates as there are beams reach it
-    if (all > 256 * N) {
+    if (all > BEAM_FIRSTS) {
         // Lists are in order, so the first ones of each tell which lists can have a candidate at all: those whose first reaches a bound that as many
         // firsts reach.
         const int lists = K * a.chunks;
