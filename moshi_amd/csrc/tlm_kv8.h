@@ -432,11 +432,13 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
 
 // ---- attention -----------------------------------------------------------------------------------------------------------
 // Numerics, both kernels.  Operands are fp16, 11 bits: codes are exact in it, queries are first brought to [2^14, 2^15) by a power of two of
-// their own, softmax weights are carried times the value scale of their block, relative to a running reference of score + exponent of that scale:
-// so the largest lie between 2^8 and 2^15 however blocks' scales differ, and the reference, with the sums, moves only where a maximum has outgrown
-// it by 2^6.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both operands come in two parts, 22 bits, good to 2^-24.
-// (bf16 operands left 1.8 times the error of the result's rounding.)  Sums, maxima and the denominator, which has the weights before they were
-// rounded, are fp32.
+// their own, softmax weights are carried times the value scale of their block.  Two running references, powers of two both (moving one rounds
+// nothing): r of the scores, which weights and their sum are relative to, and r + off of score + exponent of the value scale, which weights times
+// scale are relative to.  So what the products take lies between 2^7 and 2^15 at its largest, however blocks' scales differ, and the denominator does not
+// know of the scales: blocks of zeros, whose scale is 2^-107, neither let it overflow nor are lost from it beside values of 2^20.  References, with
+// the sums, move only where a maximum has outgrown one by 2^6.  One fp16 rounding (2^-12) is below a bf16 result's own; for fp32 queries both
+// operands come in two parts, 22 bits, good to 2^-24.  (bf16 operands left 1.8 times the error of the result's rounding.)  Sums, maxima and the
+// denominator, which has the weights before they were rounded, are fp32.
 // Sequences with up to so many columns, one tile, are the few's where a call may bring longer ones: 64 sequences with 4 rows of 4 heads, 2000 keys each,
 // take 52 us there and 101 us as the many's; 2 with 20 000 keys, 27 and 46 us.  (A second tile would read every key again.)
 constexpr int KV8_FEW = 16;
@@ -449,7 +451,7 @@ struct Kv8Share {                        // one kernel's part of a call
     int cols;                            // columns that a slot can have: z.per, or fewer where no group has more
     int pages, nsplit;                   // pages per split; splits that a group can need
     float* po;                           // nsplit > 1: [group slot][kv head][split][z.per columns][vdim] un-normalised sums
-    float* pml;                          // [group slot][kv head][split][2][z.per]: running maximum, sum of weights
+    float* pml;                          // [group slot][kv head][split][3][z.per]: references (Kv8Refs: r, off) and sum of weights
     int* what;                           // [group slot][4]: its columns, the splits that were needed, first row and column of its sequence
 };
 struct TlmKv8Attn {
@@ -509,14 +511,35 @@ __device__ __forceinline__ void kv8_tell(const Kv8Share& h, const Kv8Cols& c, in
     if (h.nsplit > 1 && g == 0 && split == 0 && threadIdx.x == 0)
         *(u32x4*)(h.what + 4 * slot) = u32x4{(unsigned)max(0, c.ncol - c.c0), (unsigned)max(1, (c.n + h.pages - 1) / h.pages), (unsigned)c.s.row0, (unsigned)c.c0};
 }
-// a value scale = fraction 2^exponent (at least 2^-120; a NaN's fraction is one), and 2^-exponent
-__device__ __forceinline__ float kv8_fraction(float scale, float& exponent, float& back) {
-    const float v = scale < 0x1p-120f ? 0x1p-120f : scale;
-    const int e = min((int)(__builtin_bit_cast(unsigned, v) >> 23 & 255u) - 127, 126);
-    exponent = (float)e;
-    back = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
-    return v * back;
-}
+// 2^x, x whole (a NaN, where nothing has been seen yet: zero)
+__device__ __forceinline__ float kv8_two(float x) { return __builtin_ldexpf(1.f, (int)fminf(fmaxf(x, -200.f), 200.f)); }
+// exponent of a value scale, at least -100: what lies below fits into the weights' 2^7 and more
+__device__ __forceinline__ float kv8_exponent(float scale) { return (float)min(max((int)(__builtin_bit_cast(unsigned, scale) >> 23 & 255u) - 127, -100), 126); }
+// A column's references: r = ceil(maximum of the scores) when it was moved last, off the same of score - r + exponent of the value scale.
+struct Kv8Refs {
+    float r = -INFINITY, off = -INFINITY;
+    float up = 0.f;                      // 2^(KV8_UP - off): weights times value scale times this are the product's operand
+    // does a lane's maximum `top` of scores in a block of exponent e outgrow one of them?
+    __device__ __forceinline__ bool outgrown(float top, float e) const { return top > r + KV8_SLACK || top - r + e > off + KV8_SLACK; }
+    // moved to the column's maxima (max over its lanes: `across`); factors of the sum of weights and of the weighted sums
+    template <class F>
+    __device__ __forceinline__ void move(float top, float e, F across, float& fewer, float& less) {
+        const float to = fmaxf(r, ceilf(across(top))), step = to - r;
+        const float held = off - step, out = fmaxf(held, ceilf(across(top - (to == -INFINITY ? 0.f : to) + e)));
+        fewer = kv8_two(-step);
+        less = kv8_two(held - out);
+        r = to;
+        off = out;
+        up = kv8_two(KV8_UP - off);
+    }
+    __device__ __forceinline__ float base() const { return r == -INFINITY ? 0.f : r; }
+    // what a block's weights are multiplied by: its scale and `up` (where that is beyond fp32, all of its weights are below 2^-100 of the largest); a block
+    // that the column does not see may have any scale
+    __device__ __forceinline__ float times(float scale, float top) const {
+        const float x = scale * up;
+        return top == -INFINITY ? 0.f : (fabsf(x) > 0x1p126f && fabsf(scale) < INFINITY ? 0x1p126f : x);
+    }
+};
 // scores of keys key0 .. key0 + 15 for a query at `pos`, -infinity where it does not see them
 __device__ __forceinline__ void kv8_masked(const TlmMask& m, int pos, int key0, float (&y)[16]) {
     const int behind = m.window > 0 ? pos - m.window : -1;      // the last position that a window has passed
@@ -637,11 +660,13 @@ __device__ __forceinline__ void kv8_store(const TlmKv8Attn& a, int row, int head
     typedef typename Tr::elem E;
     Tr::store4((E*)a.out + (a.out_ks ? tlm_index<Tr>(row, head * 16 * a.nd + d, a.out_ks) : row * a.out_row + head * a.out_head + d), v);
 }
-// 1 / denominator of weights that were summed relative to 2^(M - KV8_UP); nothing seen: zero
-__device__ __forceinline__ float kv8_inverse(float L, float M, int sink) {
-    const float sum = sink ? L + exp2f(KV8_UP - M) : L;
-    return sum == 0.f ? 0.f : 1.f / sum;
+// 1 / denominator of weights that were summed relative to 2^r; nothing seen: zero
+__device__ __forceinline__ float kv8_inverse(float L, float r, int sink) {
+    const float sum = sink ? L + exp2f(-r) : L;
+    return r == -INFINITY && sum == sum ? 0.f : 1.f / sum;
 }
+// weighted sums -> outputs (two factors: at the scales' ends either alone is in range)
+__device__ __forceinline__ f32x4 kv8_result(f32x4 v, float inverse, float off) { return v * inverse * kv8_two(off - KV8_UP); }
 
 // Few columns: four waves share one tile of 16 columns, each takes every fourth of its pages straight from the cache - the page after it is
 // asked for before the products of this one - and their sums meet in LDS.  Bound by the codes' way from memory: 100 003 keys of 8 heads of 128
@@ -700,12 +725,12 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     f32x4 acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    Kv8Refs ref;
+    float l = 0.f;
     for (int i = i0 + wave; i < i1; i += WK) {
         const int key0 = nb * TLM_PAGE + 16 * kq;
         const bool now = have, whole = kv8_whole(a.mask, c.plo, c.phi, nb * TLM_PAGE, TLM_PAGE);
-        float lv, rv;
-        const float sc = ks * back, fraction = kv8_fraction(vs, lv, rv);
+        const float sc = ks * back, vsn = vs;
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -730,30 +755,29 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         // (scalars: an element of a vector written behind a branch has come out as its neighbour where the vector was kept in accumulation registers)
         float y[16], mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] = mmi_fma(s[r >> 2][r & 3], sc, lv);
+        for (int r = 0; r < 16; ++r) y[r] = s[r >> 2][r & 3] * sc;
         if (!whole) kv8_masked(a.mask, pos, key0, y);
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[r]);
-        mx = mmi_rows_max(mx);
-        if (mmi_any(live && mx > m + KV8_SLACK)) {         // (the tile's other columns hold anything)
-            const float to = fmaxf(m, mx), al = mmi_fast_exp2f(m - (to == -INFINITY ? 0.f : to));
-            l *= al;
+        const float ev = kv8_exponent(vsn);
+        if (mmi_any(live && ref.outgrown(mx, ev))) {       // (the tile's other columns hold anything)
+            float fewer, less;
+            ref.move(mx, ev, [](float x) { return mmi_rows_max(x); }, fewer, less);
+            l *= fewer;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) acc[d] *= al;
-            m = to;
+            for (int d = 0; d < ND; ++d) acc[d] *= less;
         }
-        const float ms = (m == -INFINITY ? 0.f : m) - KV8_UP;
+        const float base = ref.base(), times = ref.times(vsn, mx);
         u32x4 pf[2][NS];
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            y[r] = mmi_fast_exp2f(y[r] - ms);
+            y[r] = mmi_fast_exp2f(y[r] - base);
             sum += y[r];
         }
-        const float times = sum == 0.f ? 0.f : fraction;   // (the scale of a block that the column does not see may be anything)
+        l += sum;
 #pragma unroll
         for (int u = 0; u < 2; ++u) kv8_split8<NS>(y + 8 * u, times, pf[u]);
-        l += sum * rv;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             u32x4 lo, hi;
@@ -768,19 +792,22 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     l += mmi_shfl_xor(l, 16);
     l += mmi_shfl_xor(l, 32);
     if (kq == 0) {
-        ml[0][wave][bl] = m;
-        ml[1][wave][bl] = l;
+        ml[0][wave][bl] = ref.r;
+        ml[1][wave][bl] = ref.off;
+        ml[2][wave][bl] = l;
     }
     __syncthreads();
-    float M = -INFINITY, L = 0.f;
+    float R = -INFINITY, O = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int v = 0; v < WK; ++v) M = fmaxf(M, ml[0][v][bl]);
-    const float Ms = M == -INFINITY ? 0.f : M;
+    for (int v = 0; v < WK; ++v) R = fmaxf(R, ml[0][v][bl]);
 #pragma unroll
-    for (int v = 0; v < WK; ++v) L += ml[1][v][bl] * exp2f(ml[0][v][bl] - Ms);
-    const float f = exp2f(m - Ms);
+    for (int v = 0; v < WK; ++v) {
+        O = fmaxf(O, ml[1][v][bl] + (ml[0][v][bl] - R));
+        L += ml[2][v][bl] * kv8_two(ml[0][v][bl] - R);
+    }
+    const float f = kv8_two(ref.off + (ref.r - R) - O);
     const bool parts = a.few.nsplit > 1;
-    const float inv = parts ? 1.f : kv8_inverse(L, M, a.sink);
+    const float inv = kv8_inverse(L, R, a.sink);
     const long part = ((long)slot * a.c.kv_heads + g) * a.few.nsplit + split;
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += 8) {
@@ -797,23 +824,24 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
             f32x4 v = ob[d * 64 + lane];
 #pragma unroll
             for (int o = 1; o < WK; ++o) v += ob[(o * 8 + d) * 64 + lane];
-            v *= inv;
             if (!live) continue;
+            if (!parts) v = kv8_result(v, inv, O);
             const int dim = (d0 + d) * 16 + 4 * kq, head = g * a.rep + col - tok * a.rep;
             if (parts) *reinterpret_cast<f32x4*>(a.few.po + (part * 16 + bl) * a.c.vdim + dim) = v;
             else kv8_store<Tr>(a, c.s.row0 + tok, head, dim, v);
         }
     }
     if (parts && wave == 0 && kq == 0) {
-        a.few.pml[part * 32 + bl] = M;
-        a.few.pml[part * 32 + 16 + bl] = L;
+        a.few.pml[part * 48 + bl] = R;
+        a.few.pml[part * 48 + 16 + bl] = O;
+        a.few.pml[part * 48 + 32 + bl] = L;
     }
 }
 // grid: slots of tiles, kv heads, splits
 template <class In, class Tr, int NS, int D, bool E4M3>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8Attn a) {
     MMI_SHARED __attribute__((aligned(16))) f32x4 ob[KV8_LDS];
-    MMI_SHARED float ml[2][4][16];
+    MMI_SHARED float ml[3][4][16];
     tlm_kv8_attn<In, Tr, NS, D, E4M3>(a, ob, ml, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
 }
 
@@ -944,10 +972,10 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         vs = a.c.vs[n];
     };
     f32x16 acc[QT][DT];
-    float m[QT], l[QT];
+    Kv8Refs ref[QT];
+    float l[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        m[t] = -INFINITY;
         l[t] = 0.f;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -988,8 +1016,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         if (busy) scores(set ^ 1, set ^ 1);
         if (busy && now && key0 <= phi) {
             const bool whole = kv8_whole(a.mask, plo, phi, key0, 32);
-            float lv, rv;
-            const float fraction = kv8_fraction(vsn, lv, rv);
+            const float ev = kv8_exponent(vsn);
             u32x4 pf[QT][2][NS];
             float mx[QT], y[QT][16];
             bool moved = false;
@@ -999,34 +1026,33 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
                 const int pos = c.s.pos0 + tok[t];
                 float x = -INFINITY;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) y[t][r] = mmi_fma(s[set][t][r], sc, lv);
+                for (int r = 0; r < 16; ++r) y[t][r] = s[set][t][r] * sc;
                 if (!whole) kv8_masked(a.mask, pos, key0 + 16 * hi, y[t]);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x = fmaxf(x, y[t][r]);
-                mx[t] = mmi_halves_max(x);
-                moved = moved || (w0 + 32 * t + cl < c.ncol && mx[t] > m[t] + KV8_SLACK);      // (the tile's other columns hold anything)
+                mx[t] = x;
+                moved = moved || (w0 + 32 * t + cl < c.ncol && ref[t].outgrown(x, ev));      // (the tile's other columns hold anything)
             }
             if (mmi_any(moved)) {
 #pragma unroll
                 for (int t = 0; t < QT; ++t) {
-                    const float to = fmaxf(m[t], mx[t]), al = mmi_fast_exp2f(m[t] - (to == -INFINITY ? 0.f : to));
-                    l[t] *= al;
+                    float fewer, less;
+                    ref[t].move(mx[t], ev, [](float x) { return mmi_halves_max(x); }, fewer, less);
+                    l[t] *= fewer;
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[t][d] *= al;
-                    m[t] = to;
+                    for (int d = 0; d < DT; ++d) acc[t][d] *= less;
                 }
             }
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float ms = (m[t] == -INFINITY ? 0.f : m[t]) - KV8_UP;
+                const float base = ref[t].base(), times = ref[t].times(vsn, mx[t]);
                 float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    y[t][r] = mmi_fast_exp2f(y[t][r] - ms);
+                    y[t][r] = mmi_fast_exp2f(y[t][r] - base);
                     sum += y[t][r];
                 }
-                l[t] += sum * rv;
-                const float times = sum == 0.f ? 0.f : fraction;
+                l[t] += sum;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) kv8_split8<NS>(y[t] + 8 * u, times, pf[t][u]);
             }
@@ -1078,21 +1104,22 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int n = wave * 32 * QT + 32 * t + cl;        // column of the group
-        const float L = mmi_halves_sum(l[t]), inv = parts ? 1.f : kv8_inverse(L, m[t], a.sink);
+        const float L = mmi_halves_sum(l[t]), inv = kv8_inverse(L, ref[t].r, a.sink);
         if (c.c0 + n >= c.ncol) continue;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int dim = 32 * d + 8 * r + 4 * hi;
-                const f32x4 v = f32x4{acc[t][d][4 * r], acc[t][d][4 * r + 1], acc[t][d][4 * r + 2], acc[t][d][4 * r + 3]} * inv;
+                const f32x4 v = f32x4{acc[t][d][4 * r], acc[t][d][4 * r + 1], acc[t][d][4 * r + 2], acc[t][d][4 * r + 3]};
                 if (dim >= a.c.vdim) continue;
                 if (parts) *reinterpret_cast<f32x4*>(a.many.po + (part * Z::PER + n) * a.c.vdim + dim) = v;
-                else kv8_store<Tr>(a, c.s.row0 + tok[t], head[t], dim, v);
+                else kv8_store<Tr>(a, c.s.row0 + tok[t], head[t], dim, kv8_result(v, inv, ref[t].off));
             }
         if (parts && hi == 0) {
-            a.many.pml[part * 2 * Z::PER + n] = m[t];
-            a.many.pml[part * 2 * Z::PER + Z::PER + n] = L;
+            a.many.pml[part * 3 * Z::PER + n] = ref[t].r;
+            a.many.pml[part * 3 * Z::PER + Z::PER + n] = ref[t].off;
+            a.many.pml[part * 3 * Z::PER + 2 * Z::PER + n] = L;
         }
     }
 }
@@ -1101,7 +1128,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 template <class In, class Tr, int NS, int D, bool E4M3>
 __global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(TlmKv8Attn a, int many, int few_slots) {
     MMI_DYN_SHARED(u32x4, lds);
-    MMI_SHARED float ml[2][4][16];
+    MMI_SHARED float ml[3][4][16];
     const int G = a.c.kv_heads;
     int b = (int)blockIdx.x;
     if (b < many) {
@@ -1132,18 +1159,19 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
     if constexpr (!WIDE) {
         const int lane = tid & 63, G = a.c.vdim / 4, at_once = 64 / G, n = (b - slot * each) * at_once + lane / G, d = 4 * (lane % G);
         const bool on = lane / G < at_once && n < h.cols;
-        const float *ml0 = h.pml + part * 2 * per, *po0 = h.po + part * per * a.c.vdim;
+        const float *ml0 = h.pml + part * 3 * per, *po0 = h.po + part * per * a.c.vdim;
         const unsigned at_ml = on ? n : 0, at_po = at_ml * a.c.vdim + d;
         const int step = per * a.c.vdim;                   // (a split's part: addresses are a scalar and a lane's offset)
-        float m[8], l[8];
+        float m[8], e[8], l[8];
         f32x4 v[8];
         auto load = [&](int k0, int ns) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (k0 + k < ns) {
-                    const float* ml = ml0 + (k0 + k) * 2 * per;
+                    const float* ml = ml0 + (k0 + k) * 3 * per;
                     m[k] = ml[at_ml];
-                    l[k] = (ml + per)[at_ml];
+                    e[k] = (ml + per)[at_ml];
+                    l[k] = (ml + 2 * per)[at_ml];
                     v[k] = *(const f32x4*)(po0 + (k0 + k) * step + at_po);
                 }
         };
@@ -1151,52 +1179,65 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
         const int col = c0 + n;
         if (!on || n >= cols) return;
         if (!few) load(0, ns);                             // (of the slots that portions might need, half are empty)
-        float M = -INFINITY, L = 0.f;
+        float R = -INFINITY, O = -INFINITY, L = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         for (int k0 = 0;;) {
-            float top = M;
+            float r = R;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (k0 + k < ns) top = fmaxf(top, m[k]);
-            const float Ms = top == -INFINITY ? 0.f : top, less = mmi_fast_exp2f(M - Ms);
-            L *= less;
-            o *= less;
-            M = top;
+                if (k0 + k < ns) r = fmaxf(r, m[k]);
+            const float held = O + (R - r);
+            float off = held;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < ns) off = fmaxf(off, e[k] + (m[k] - r));
+            L *= kv8_two(R - r);
+            o *= kv8_two(held - off);
+            R = r;
+            O = off;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (k0 + k < ns) {
-                    const float w = mmi_fast_exp2f(m[k] - Ms);
-                    L += l[k] * w;
-                    o += v[k] * w;
+                    L += l[k] * kv8_two(m[k] - r);
+                    o += v[k] * kv8_two(e[k] + (m[k] - r) - off);
                 }
             if ((k0 += 8) >= ns) break;
             load(k0, ns);
         }
         const int tok = col / a.rep;
-        kv8_store<Tr>(a, row0 + tok, g * a.rep + col - tok * a.rep, d, o * kv8_inverse(L, M, a.sink));
+        kv8_store<Tr>(a, row0 + tok, g * a.rep + col - tok * a.rep, d, kv8_result(o, kv8_inverse(L, R, a.sink), O));
     } else {
-        MMI_SHARED float wt[256], red[4][2];
+        MMI_SHARED float wt[256], red[4][3];
         MMI_SHARED __attribute__((aligned(16))) f32x4 sum[256];
         const int n = b - slot * each;
         const int col = c0 + n;                            // (ns: at most 256)
         if (n >= cols) return;
         const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, e = -INFINITY, l = 0.f;
         if (tid < ns) {
-            m = h.pml[(part + tid) * 2 * per + n];
-            l = h.pml[(part + tid) * 2 * per + per + n];
+            const float* ml = h.pml + (part + tid) * 3 * per + n;
+            m = ml[0];
+            e = ml[per];
+            l = ml[2 * per];
         }
         const float wm = mmi_wave_max_f32(m);
         if ((tid & 63) == 0) red[wave][0] = wm;
         __syncthreads();
-        float M = -INFINITY;
+        float R = -INFINITY, O = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, red[w][0]);
-        const float w = tid < ns ? mmi_fast_exp2f(m - (M == -INFINITY ? 0.f : M)) : 0.f, wl = mmi_wave_sum_down(tid < ns ? l * w : 0.f);
-        wt[tid] = w;
-        if ((tid & 63) == 0) red[wave][1] = wl;
+        for (int w = 0; w < 4; ++w) R = fmaxf(R, red[w][0]);
+        e += m - R;                                        // (nothing seen: -infinity or a NaN, which maxima pass over)
+        const float we = mmi_wave_max_f32(e), wl = mmi_wave_sum_down(tid < ns ? l * kv8_two(m - R) : 0.f);
+        if ((tid & 63) == 0) {
+            red[wave][1] = wl;
+            red[wave][2] = we;
+        }
         __syncthreads();
-        const float inv = kv8_inverse((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]), M, a.sink);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) O = fmaxf(O, red[w][2]);
+        wt[tid] = kv8_two(e - O);
+        __syncthreads();
+        const float inv = kv8_inverse((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]), R, a.sink);
         const int q = tid & 15, k = tid >> 4;
         for (int d0 = 0; d0 < a.c.vdim; d0 += 64) {
             const int d = d0 + 4 * q;
@@ -1210,7 +1251,7 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
             if (k == 0 && d < a.c.vdim) {
 #pragma unroll
                 for (int i = 1; i < 16; ++i) v += sum[16 * i + q];
-                kv8_store<Tr>(a, row0 + tok, head, d, v * inv);
+                kv8_store<Tr>(a, row0 + tok, head, d, kv8_result(v, inv, O));
             }
         }
     }

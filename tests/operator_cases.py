@@ -956,3 +956,66 @@ def check_rows_in_no_order(dev, lib):
         assert max(float(t.max()) for t in (cache.k_scale, cache.v_scale)) <= max(float(t.max()) for t in before), rows
         kv = cache.read(tables, i32(100, 200, 299, 0), i32(*rows), tokens=60)
         assert kv[0].shape == (60, 1, 32)
+
+
+# ---- value scales of a sequence's blocks far apart -------------------------------------------------------------------------------------
+def _ramp(first, last):
+    return lambda t: 2.0 ** (first + (last - first) * t)
+
+
+# mags: of the values, levels: scores (natural logarithms), both functions of the place 0 .. 1 in the sequence; nothing: pages that the caller's own scales say
+# hold zeros; negative: pages whose scales are negative
+FAR = {
+    "zeros_in_a_page": dict(c=Case([40], [24], kv_heads=1, rep=2, dim=32, vdim=32), mags=lambda t: 0.0 if t < 0.5 else 1.0, levels=lambda t: 5.0 if t < 0.5 else 0.0),
+    "zeros_first": dict(c=Case([639], [1], single=True, kv_heads=1, rep=2, dim=32, vdim=32), mags=lambda t: 0.0 if t < 0.5 else 1.0, levels=lambda t: 3.0 if t < 0.5 else 0.0),
+    "zeros_last": dict(c=Case([600], [40], kv_heads=1, rep=2, dim=32, vdim=32, codes="e4m3", dtype=F32), mags=lambda t: 1.0 if t < 0.5 else 0.0, levels=lambda t: 0.0 if t < 0.5 else 6.0),
+    "zeros_alone": dict(c=Case([90], [40], kv_heads=1, rep=2, dim=32, vdim=32), mags=lambda t: 0.0, levels=lambda t: 0.0),
+    "scale_of_zero": dict(c=Case([127], [1], single=True, kv_heads=2, rep=2, dim=32, vdim=32), mags=lambda t: 1.0, levels=lambda t: 1.0 if t < 0.5 else 0.0, nothing=(0,)),
+    "scale_of_zero_portion": dict(c=Case([100], [60], kv_heads=2, rep=2, dim=32, vdim=48, codes="e4m3"), mags=lambda t: 1.0, levels=lambda t: 2.0 if t < 0.4 else 0.0, nothing=(0, 2)),
+    "scale_of_zero_fp32_sink": dict(c=Case([300], [1], single=True, kv_heads=1, rep=3, dim=32, vdim=32, dtype=F32, sink=True), mags=lambda t: 1.0, levels=lambda t: 0.0, nothing=(1, 3)),
+    "large_behind_likelier_zeros": dict(c=Case([639], [1], single=True, kv_heads=1, rep=2, dim=32, vdim=32, dtype=F32), mags=lambda t: 0.0 if t < 0.5 else 2.0 ** 20,
+                                        levels=lambda t: 9.0 if t < 0.5 else 0.0),
+    "large_behind_likelier_zeros_portion": dict(c=Case([600], [40], kv_heads=1, rep=2, dim=32, vdim=32, dtype=F32, codes="e4m3"), mags=lambda t: 0.0 if t < 0.5 else 2.0 ** 40,
+                                                levels=lambda t: 9.0 if t < 0.5 else 0.0),
+    "growing": dict(c=Case([1299], [1], single=True, kv_heads=1, rep=2, dim=32, vdim=32, dtype=F32), mags=_ramp(-110, 110), levels=lambda t: 0.0),
+    "growing_portion": dict(c=Case([1270], [30], kv_heads=1, rep=2, dim=32, vdim=32, sink=True), mags=_ramp(-110, 110), levels=lambda t: 0.0),
+    "shrinking": dict(c=Case([1299], [1], single=True, kv_heads=1, rep=2, dim=32, vdim=32, dtype=F32, codes="e4m3"), mags=_ramp(110, -110), levels=lambda t: 0.0),
+    "shrinking_against_scores": dict(c=Case([1270], [30], kv_heads=1, rep=2, dim=32, vdim=32, dtype=F32), mags=_ramp(60, -60), levels=lambda t: 70 * t),
+    "negative_scales": dict(c=Case([200], [1], single=True, kv_heads=2, rep=2, dim=32, vdim=32), mags=lambda t: 1.0, levels=lambda t: 0.0, negative=(0, 2)),
+    "negative_scales_portion": dict(c=Case([200], [30], kv_heads=2, rep=2, dim=32, vdim=32, codes="e4m3", dtype=F32), mags=lambda t: 4.0, levels=lambda t: t, negative=(1,)),
+}
+# pages that are not split, so that a sum runs over many of them (long on the simulator)
+FAR_LARGE = {
+    "zeros_below_unsplit": dict(c=Case([620], [20], kv_heads=400, rep=1, dim=16, vdim=16), mags=lambda t: 0.0 if t < 0.8 else 1.0,
+                                levels=lambda t: 5.6 * math.log(2) if 0.1 <= t < 0.8 else 0.0),
+    "large_behind_likelier_zeros_unsplit": dict(c=Case([620], [20], kv_heads=400, rep=1, dim=16, vdim=16), mags=lambda t: 0.0 if t < 0.5 else 2.0 ** 60, levels=lambda t: 8.0 if t < 0.5 else 0.0),
+}
+
+
+def check_blocks_far_apart(name, dev, lib):
+    """Blocks of zeros, of values 2^220 apart, of scales of zero or below it: no sum overflows and none is lost, whichever kernel, split or not."""
+    o = {**FAR, **FAR_LARGE}[name]
+    c, g = o["c"], torch.Generator().manual_seed(len(name))
+    cache, q, _, _, args = build(c, dev, lib, fill=False)
+    n = c.past[0] + c.rows[0]
+    at = torch.arange(n) / n
+    mags, levels = [torch.tensor([o[f](float(t)) for t in at], dtype=torch.float64).float() for f in ("mags", "levels")]
+    keys = 0.1 * torch.randn((n, c.kv_heads, c.dim), generator=g)
+    keys[..., 0] = levels[:, None]
+    vals = torch.randn((n, c.kv_heads, c.vdim), generator=g) * mags[:, None, None]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cache.append(keys.to(dev), vals.to(dev), args[0], i32(0), i32(0, n))
+    table = args[0][0].tolist()
+    for i in o.get("nothing", ()):
+        cache.v_scale[table[i]] = 0.0
+    for i in o.get("negative", ()):
+        cache.v_scale[table[i]] *= -1.0
+    q = torch.randn(q.shape, generator=g) * 0.1
+    q[..., 0] = c.dim ** 0.5                               # (times the softmax's factor: one)
+    q = q.to(c.dtype).to(dev)
+    got = cache.attend(q, *args, sink=c.sink).cpu().double()
+    want, size, top = attend64(c, cache, q, args)
+    h = 2.0 ** -12 if c.dtype == BF16 else 2.0 ** -23      # (check_attend)
+    off = 2 * size * (h + c.dim * 2.0 ** -24) + h + 2.0 ** -20
+    limit = off[:, None, None].double() * top + want.abs() * (torch.finfo(c.dtype).eps / 2)
+    assert got.isfinite().all() and ((got - want).abs() <= limit).all(), float(((got - want).abs() / limit).max())

@@ -207,3 +207,8 @@ def test_position_past_the_table(lib, codes):
 
 def test_rows_in_no_order(lib):
     oc.check_rows_in_no_order(DEV, lib)
+
+
+@pytest.mark.parametrize("name", sorted(oc.FAR | oc.FAR_LARGE))
+def test_blocks_far_apart(lib, name):
+    oc.check_blocks_far_apart(name, DEV, lib)

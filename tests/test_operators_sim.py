@@ -110,3 +110,8 @@ def test_position_past_the_table(tlm_lib, codes):  # noqa: F811
 
 def test_rows_in_no_order(tlm_lib):  # noqa: F811
     oc.check_rows_in_no_order(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name", sorted(oc.FAR))
+def test_blocks_far_apart(tlm_lib, name):  # noqa: F811
+    oc.check_blocks_far_apart(name, DEV, tlm_lib)
