@@ -157,7 +157,7 @@ int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dt
 /* Beam search                                                                                */
 /* ------------------------------------------------------------------------------------------ */
 /* Of every request's beams x vocab candidates the `beams` best.  Candidate (beam, token): score + log softmax(logits)[token], ranked by
- * score / length^length_penalty, length counting the token; equal ranks go to the lower beam, then the lower token.  A finished beam has one
+ * score / length^length_penalty (-16 .. 16), length counting the token; equal ranks go to the lower beam, then the lower token.  A finished beam has one
  * candidate, `eos` at the score and the length it has.  Rows with a NaN, and beams of score -infinity, rank last.  Device memory all of it:
  * logits bf16 or fp32 [batch * beams][vocab], `row` elements apart; score, out_* [batch][beams]; length (NULL: no penalty), finished (NULL:
  * none is) and the outputs of either kind may be NULL.  At most 32 beams. */

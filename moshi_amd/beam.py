@@ -55,7 +55,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
             (all but one at a request's start).
         lengths: int32 [requests, beams], tokens so far; needed for a length penalty.
         finished: bool [requests, beams]; a finished beam has one candidate, `eos` at the score and length it has.
-        length_penalty: candidates are ranked by score / length ** length_penalty.
+        length_penalty: candidates are ranked by score / length ** length_penalty; between -16 and 16.
     Equal ranks go to the lower beam, then the lower token.  At most 32 beams.
     """
     device, shape = logits.device, scores.shape
@@ -140,6 +140,8 @@ def beam_search(lm: TokenLM, prompts: Sequence[Sequence[int]], beams: int = 4, m
     prompts = [[int(t) for t in p] for p in prompts]
     if beams < 1 or max_new_tokens < 1 or any(not p for p in prompts):
         raise ValueError("a search needs a beam, a prompt and at least one new token")
+    if not abs(length_penalty) <= 16:
+        raise ValueError("a length penalty is between -16 and 16")
     if not -1 <= eos < lm.vocab:
         raise ValueError("the end token is outside the vocabulary")
     if any(t < 0 or t >= lm.vocab for p in prompts for t in p):

@@ -26,6 +26,9 @@ struct TlmBeamArgs {
     float* out_score; int* out_parent; int* out_token; uint8_t* out_done; int* out_length;
 };
 constexpr int BEAM_NONE = 0x7fffffff;
+// Largest length penalty.  Lengths are below 2^31, so 1 / length^alpha lies between 2^-496 and 2^496: a finite score's rank is finite, and -infinity
+// stays one.  (An infinity times zero would be a NaN, before and behind nobody: fewer candidates than beams.)
+constexpr float BEAM_PENALTY = 16.f;
 
 // before in the order: the larger value, the lower index where they are equal
 template <class T>

@@ -270,7 +270,8 @@ extern "C" int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int3
     if ((rc = check_rows(logits, row, 0, dtype, "mmi_beam_select"))) return rc;
     if (!score || !out_score || !out_parent || !out_token) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: null tensor");
     if (finished && (eos < 0 || eos >= vocab)) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: finished beams need an end token of the vocabulary");
-    if (!(length_penalty - length_penalty == 0.f) || (length_penalty != 0.f && !length)) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: a length penalty is finite and needs lengths");
+    if (!(fabsf(length_penalty) <= BEAM_PENALTY)) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: a length penalty is between -16 and 16");
+    if (length_penalty != 0.f && !length) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: a length penalty needs lengths");
     const BeamSpace z = beam_space(batch * beams, beams, vocab);
     if (!workspace || workspace_bytes < (int64_t)z.total || (uintptr_t)workspace % 16) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_select: the workspace is too small (mmi_beam_select_workspace) or not aligned to 16 bytes");
     char* w = (char*)workspace;

@@ -201,7 +201,7 @@ def main(argv: Optional[List[str]] = None) -> None:
     tok.add_argument("--step-tokens", type=int, default=2048, help="most tokens of one batch: prompts are cut into portions of it")
     tok.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     tok.add_argument("--beams", type=int, default=1, help="more than 1: beam search in place of sampling")
-    tok.add_argument("--length-penalty", type=float, default=0.0, help="beams are ranked by score / length ** this")
+    tok.add_argument("--length-penalty", type=float, default=0.0, help="beams are ranked by score / length ** this (-16 .. 16)")
     tok.add_argument("--kv-cache", choices=["like-dtype", "int8", "e4m3"], default="like-dtype", help="what grouped attention's keys and values are held in")
     ap.add_argument("infile", type=str)
     ap.add_argument("outfile", type=str)

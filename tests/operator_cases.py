@@ -1019,3 +1019,31 @@ def check_blocks_far_apart(name, dev, lib):
     off = 2 * size * (h + c.dim * 2.0 ** -24) + h + 2.0 ** -20
     limit = off[:, None, None].double() * top + want.abs() * (torch.finfo(c.dtype).eps / 2)
     assert got.isfinite().all() and ((got - want).abs() <= limit).all(), float(((got - want).abs() / limit).max())
+
+
+def check_select_penalties(dev, lib):
+    """Length penalties at the ends of what is taken, with beams at -infinity and few candidates that are not: as in 64 bits.  Beyond: refused."""
+    g = torch.Generator().manual_seed(2)
+    B, K, V = 3, 4, 700
+    for bad in (16.001, -16.001, 110.0, 300.0, -300.0, math.inf, -math.inf, math.nan):
+        with pytest.raises(ValueError, match="penalty"):
+            beam_select(torch.zeros((K, V), device=dev), torch.zeros((1, K), device=dev), torch.ones((1, K), dtype=torch.int32, device=dev), length_penalty=bad, lib=lib)
+    for penalty in (16.0, -16.0, 1.0):
+        for longest in (30, 2 ** 31 - 2):
+            x = torch.full((B * K, V), -math.inf)
+            x[:, :3] = torch.randn((B * K, 3), generator=g)
+            x[2 * K:] = torch.randn((K, V), generator=g)
+            x[4:6] = -math.inf
+            scores = -20 * torch.rand((B, K), generator=g)
+            scores[0, 1:] = -math.inf                          # three candidates for four places
+            scores[2, 2] = 0.0
+            lengths = torch.randint(longest // 2, longest, (B, K), generator=g, dtype=torch.int32)
+            finished = torch.zeros((B, K), dtype=torch.bool)
+            finished[1, 2:], finished[2, :2] = True, True
+            scores[1, 3] = -math.inf
+            want = select64(x, scores, lengths, finished, 2, penalty)
+            r = beam_select(x.to(dev), scores.to(dev), lengths.to(dev), finished.to(dev), eos=2, length_penalty=penalty, lib=lib)
+            got = [t.cpu().numpy() for t in (r.scores, r.parents, r.tokens, r.finished, r.lengths)]
+            assert all(np.array_equal(a, b) for a, b in zip(got[1:], want[1:])), (penalty, longest, got, want)
+            fin = np.isfinite(want[0])
+            assert np.array_equal(np.isfinite(got[0]), fin) and (np.abs(got[0] - want[0])[fin] <= np.abs(want[0])[fin] * 2.0 ** -24 + 2.0 ** -22).all()

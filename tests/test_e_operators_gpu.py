@@ -212,3 +212,7 @@ def test_rows_in_no_order(lib):
 @pytest.mark.parametrize("name", sorted(oc.FAR | oc.FAR_LARGE))
 def test_blocks_far_apart(lib, name):
     oc.check_blocks_far_apart(name, DEV, lib)
+
+
+def test_select_penalties(lib):
+    oc.check_select_penalties(DEV, lib)

@@ -115,3 +115,7 @@ def test_rows_in_no_order(tlm_lib):  # noqa: F811
 @pytest.mark.parametrize("name", sorted(oc.FAR))
 def test_blocks_far_apart(tlm_lib, name):  # noqa: F811
     oc.check_blocks_far_apart(name, DEV, tlm_lib)
+
+
+def test_select_penalties(tlm_lib):  # noqa: F811
+    oc.check_select_penalties(DEV, tlm_lib)
