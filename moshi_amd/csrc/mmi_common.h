@@ -7,6 +7,7 @@
 #include <stdlib.h>
 #include <string.h>
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <vector>
 #include <functional>
@@ -58,6 +59,18 @@ int mmi_fail(int code, const std::string& msg);
         if (e_ != hipSuccess)                                                                        \
             return mmi_fail(MMI_ERR_HIP, std::string("kernel launch: ") + hipGetErrorString(e_));    \
     } while (0)
+
+// More than 64 KiB of dynamic LDS for a kernel: an attribute of the kernel on one device, asked for once on each (`asked`: a bit per device, the
+// kernel's own).  Threads whose first launches meet may both ask
+inline int mmi_allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& asked) {
+    int device = 0;
+    MMI_HIP_CHECK(hipGetDevice(&device));
+    const uint64_t bit = 1ull << (device & 63);
+    if (asked.load() & bit) return MMI_OK;
+    MMI_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    asked |= bit;
+    return MMI_OK;
+}
 
 // A handle binds to the HIP device that was current when it was created; every ABI entry switches the calling thread to that
 // device for the duration of the call and restores the caller's (so `device='cuda:1'` works without the caller having made

@@ -909,8 +909,8 @@ int launch_tile(hipStream_t s, const TlmJobs& J, bool say) {
     if (say) fprintf(stderr, "tile %dx%d stages %d of %d, %d workgroups\n", 16 * FN * WN, 16 * FM * WM, ST, KK, grid);
     static_assert(smem * OCC <= 160 * 1024, "LDS of a CU");
     if (smem > 64 * 1024) {
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_gemm_tile<Tr, FN, FM, WN, WM, ST, OCC, KK>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        MMI_HIP_CHECK(attr);
+        static std::atomic<uint64_t> asked{0};
+        if (const int rc = mmi_allow_lds(reinterpret_cast<const void*>(&k_tlm_gemm_tile<Tr, FN, FM, WN, WM, ST, OCC, KK>), (int)smem, asked)) return rc;
     }
     MMI_LAUNCH((k_tlm_gemm_tile<Tr, FN, FM, WN, WM, ST, OCC, KK>), grid, 256, smem, s, J);
     MMI_CHECK_LAUNCH();
@@ -1084,8 +1084,8 @@ int launch_wide(hipStream_t s, const Plan& p, TlmJobs& J, bool say) {
     for (int i = 0; i < J.n; ++i) grid += 8 * mmi_cdiv(J.j[i].blocks, 8);
     if (say) fprintf(stderr, "wide 256x%d, %d workgroups\n", J.height, grid);
     static_assert(TlmWide::smem() <= 160 * 1024, "LDS of a CU");
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_gemm_wide<TlmBf16>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)TlmWide::smem());
-    MMI_HIP_CHECK(attr);
+    static std::atomic<uint64_t> asked{0};
+    if (const int rc = mmi_allow_lds(reinterpret_cast<const void*>(&k_tlm_gemm_wide<TlmBf16>), (int)TlmWide::smem(), asked)) return rc;
     MMI_LAUNCH((k_tlm_gemm_wide<TlmBf16>), grid, 512, TlmWide::smem(), s, J);
     MMI_CHECK_LAUNCH();
     return MMI_OK;
@@ -1148,8 +1148,8 @@ int launch_attn_t(hipStream_t s, const TlmAttnArgs& a, bool tiled) {
             constexpr size_t smem = TlmAttnTile<Tr, ND, RK>::smem();
             static_assert(smem <= 160 * 1024, "LDS of a CU");
             if (smem > 64 * 1024) {
-                static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_attn_tile<Tr, ND, RK>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-                MMI_HIP_CHECK(attr);
+                static std::atomic<uint64_t> asked{0};
+                if (const int rc = mmi_allow_lds(reinterpret_cast<const void*>(&k_tlm_attn_tile<Tr, ND, RK>), (int)smem, asked)) return rc;
             }
             MMI_LAUNCH((k_tlm_attn_tile<Tr, ND, RK>), a.n_tiles, 256, smem, s, a);
             MMI_CHECK_LAUNCH();
@@ -1168,8 +1168,8 @@ int launch_gqa_tile(hipStream_t s, const TlmGqaArgs& u, const TlmGqaArgs& t) {
     constexpr size_t smem = TlmGqaTile<Tr, D>::smem();
     static_assert(smem <= 160 * 1024, "LDS of a CU");
     if (smem > 64 * 1024) {
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_gqa_tile<Tr, D, BESIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        MMI_HIP_CHECK(attr);
+        static std::atomic<uint64_t> asked{0};
+        if (const int rc = mmi_allow_lds(reinterpret_cast<const void*>(&k_tlm_gqa_tile<Tr, D, BESIDE>), (int)smem, asked)) return rc;
     }
     MMI_LAUNCH((k_tlm_gqa_tile<Tr, D, BESIDE>), u.kv_heads * (u.n_tiles + (BESIDE ? t.n_tiles * t.nsplit : 0)), 256, smem, s, u, t);
     return MMI_OK;
@@ -1570,8 +1570,8 @@ int launch_state_step(hipStream_t s, const TlmLinArgs& a, int n) {
 template <class Tr, int NP, bool BESIDE>
 int launch_chunk_delta_t(hipStream_t s, const TlmLinArgs& a, int n_chunk, int n_small) {
     const size_t smem = tlm_chunk_delta_smem();
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_chunk_delta<Tr, NP, BESIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    MMI_HIP_CHECK(attr);
+    static std::atomic<uint64_t> asked{0};
+    if (const int rc = mmi_allow_lds(reinterpret_cast<const void*>(&k_tlm_chunk_delta<Tr, NP, BESIDE>), (int)smem, asked)) return rc;
     MMI_LAUNCH((k_tlm_chunk_delta<Tr, NP, BESIDE>), (n_chunk + n_small) * a.heads, 512, smem, s, a, n_chunk, n_small, tlm_step_groups(a.vdim_p));
     MMI_CHECK_LAUNCH();
     return MMI_OK;

@@ -61,8 +61,8 @@ int launch_attn(hipStream_t s, const TlmKv8Attn& a) {
         constexpr size_t smem = Kv8Tile<NS, D>::smem();
         static_assert(smem <= 160 * 1024, "LDS of a CU");
         if (smem > 64 * 1024) {
-            static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            MMI_HIP_CHECK(attr);
+            static std::atomic<uint64_t> asked{0};
+            if (const int rc = mmi_allow_lds(reinterpret_cast<const void*>(&k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), (int)smem, asked)) return rc;
         }
         const int slots = (int)kv8_slots(a.q, a.few.z), many = (int)kv8_slots(a.q, a.many.z) * a.c.kv_heads * a.many.nsplit;
         MMI_LAUNCH((k_tlm_kv8_tile<In, Tr, NS, D, E4M3>), (unsigned)many + (unsigned)slots * a.c.kv_heads * a.few.nsplit, 256, smem, s, a, many, slots);

@@ -119,3 +119,24 @@ def test_blocks_far_apart(tlm_lib, name):  # noqa: F811
 
 def test_select_penalties(tlm_lib):  # noqa: F811
     oc.check_select_penalties(DEV, tlm_lib)
+
+
+def test_large_lds_is_asked_for_on_every_device(tlm_lib):  # noqa: F811
+    """How much LDS a kernel may have is an attribute of the kernel on ONE device: the operators, and the engine's kernels, ask again on another."""
+    c, dll, asked = oc.ATTENDS["portions_fp32"], tlm_lib.cdll, []
+    cfg = oc.tc.MECHANISMS["delta"]
+    sd = oc.random_token_lm_state_dict(cfg, seed=5)
+    for device in (51, 52, 51):
+        dll.hipsim_set_device(device)
+        try:
+            cache, q, k, v, args = oc.build(c, DEV, tlm_lib)
+            cache.append(k, v, *args)
+            before = dll.hipsim_attributes(device)
+            cache.attend(q, *args)
+            both = dll.hipsim_attributes(device)
+            lm = oc.TokenLM(sd, cfg, device=DEV, dtype=oc.F32, lib=tlm_lib, max_slots=2, max_tokens=256)
+            lm.step([(lm.open(), oc.tc.tokens_of(cfg, 80), [79])])
+        finally:
+            dll.hipsim_set_device(0)
+        asked.append((both - before, dll.hipsim_attributes(device)))
+    assert asked[0][0] == 1 and asked[0][1] > 1 and asked[1] == asked[0] and asked[2] == (0, asked[0][1]), asked
