@@ -37,6 +37,7 @@ constexpr int TLM_PAGE = 64;         // tokens per cache page
 
 // which keys a position sees, and the factor of the scores (times log2(e)): the last `window` ones (0: all), and the first `keep`
 struct TlmMask { int window, keep; float scale; };
+constexpr int TLM_KEEP = 0x7fffff00;      // more first positions than there can be; rounded up to pages it has 31 bits still
 // pages of a sequence: the block table's first `keep` entries are for the pages that no window releases, the others are a ring
 struct TlmPages { const int* table; int ld, keep; };
 __device__ __forceinline__ int tlm_page(const TlmPages& p, const int* row, int i) { return mmi_load_const(row + (i < p.keep ? i : p.keep + (i - p.keep) % (p.ld - p.keep))); }

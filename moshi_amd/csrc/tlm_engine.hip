@@ -1989,6 +1989,7 @@ int create_impl(mmi_tlm* m, const mmi_tensor_desc* weights, int n_weights) {
         m->layers.emplace_back();
         Layer& L = m->layers.back();
         L.c = c.layers[i];
+        L.c.keep_first = std::min(L.c.keep_first, TLM_KEEP);
         const std::string p = "l" + std::to_string(i);
         if ((rc = ld.vec(p + ".norm1", c.width, m->ld, &L.norm)) || (c.norms == 2 && L.c.mlp != MMI_TLM_MLP_NONE && (rc = ld.vec(p + ".norm2", c.width, m->ld, &L.norm2))) ||
             (c.layer_scales && (rc = ld.vec(p + ".ls1", c.width, m->ld, &L.ls1))))
@@ -2036,7 +2037,7 @@ int create_impl(mmi_tlm* m, const mmi_tensor_desc* weights, int n_weights) {
         }
     }
     if (unlimited) m->max_window = 0;
-    if (m->max_window > 0) m->keep_pages = mmi_cdiv(keep, TLM_PAGE);
+    if (m->max_window > 0) m->keep_pages = std::min(mmi_cdiv(keep, TLM_PAGE), m->max_pages);      // (where the pool has no more, none is ever released)
     const int times = c.loop_stop > c.loop_start ? c.loop_times : 1;
     const int start = c.loop_stop > c.loop_start ? c.loop_start : c.n_layers, stop = c.loop_stop > c.loop_start ? c.loop_stop : c.n_layers;
     auto run = [&](int layer, bool add, int pass) {
@@ -2283,7 +2284,7 @@ extern "C" int mmi_tlm_step(mmi_tlm* m, int32_t n_entries, const int32_t* slots,
             b[M.crow + row] = m->has_attn ? S.page(pos / TLM_PAGE) * TLM_PAGE + (int)(pos % TLM_PAGE) : 0;
         }
         int64_t span = S.pos + counts[e];
-        if (m->max_window > 0) span = std::min<int64_t>(span, m->max_window + counts[e] + m->keep_pages * TLM_PAGE);
+        if (m->max_window > 0) span = std::min<int64_t>(span, m->max_window + counts[e] + (int64_t)m->keep_pages * TLM_PAGE);
         blocks = std::max(blocks, span / 32 + 1);
         if (m->cfg.cache)
             while ((int64_t)1 << sh.span < (S.pos + counts[e] - 1) / TLM_PAGE + 1) ++sh.span;

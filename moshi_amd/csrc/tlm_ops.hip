@@ -192,7 +192,7 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     a->heads = heads;
     a->rep = heads / cache->kv_heads;
     a->nd = cache->vdim / 16;
-    a->mask = TlmMask{window, window > 0 ? keep_first : 0, 0.f};
+    a->mask = TlmMask{window, window > 0 ? std::min(keep_first, TLM_KEEP) : 0, 0.f};
     if ((long)a->q.T * a->rep > 1l << 26) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^26 rows times query heads of a group");
     *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1, (size_t)1 << 30);
     long groups = 0;

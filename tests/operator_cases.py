@@ -1047,3 +1047,27 @@ def check_select_penalties(dev, lib):
             assert all(np.array_equal(a, b) for a, b in zip(got[1:], want[1:])), (penalty, longest, got, want)
             fin = np.isfinite(want[0])
             assert np.array_equal(np.isfinite(got[0]), fin) and (np.abs(got[0] - want[0])[fin] <= np.abs(want[0])[fin] * 2.0 ** -24 + 2.0 ** -22).all()
+
+
+def check_keeps_everything(dev, lib, codes="int8"):
+    """A window that keeps more first positions than there can be, and one longer than any sequence, hide nothing."""
+    cache, table, _, i32, g = _filled(dev, lib, 8, 500, codes)
+    for n in (1, 20):
+        q = torch.randn((n, 2, 32), generator=g).to(dev)
+        args = (q, table, i32(500 - n), None if n == 1 else i32(0, n))
+        want = cache.attend(*args)
+        assert want.any()
+        for window, keep in ((10, 2 ** 31 - 64), (10, 2 ** 31 - 63), (1, 2 ** 31 - 1), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
+            # the same keys in the same order, whatever the splits: sums in another order at most
+            assert torch.allclose(cache.attend(*args, window=window, keep_first=keep), want, rtol=2.0 ** -16, atol=2.0 ** -18), (n, window, keep)
+
+
+def check_token_lm_keeps_everything(dev, lib, codes):
+    from dataclasses import replace
+    cfg = tc.MECHANISMS["grouped_attention_no_window"]
+    sd, toks, out = random_token_lm_state_dict(cfg, seed=5), tc.tokens_of(cfg, 150), []
+    for window, keep in ((0, 0), (9, 2 ** 31 - 1), (9, 2 ** 31 - 63), (2 ** 31 - 1, 2 ** 31 - 1)):
+        layers = [replace(x, mixer=replace(x.mixer, window=window, keep_first=keep)) if isinstance(x.mixer, GroupedAttentionConfig) else x for x in cfg.layers]
+        lm = TokenLM(sd, replace(cfg, layers=layers), device=dev, dtype=F32, lib=lib, kv_cache=codes, max_slots=2, max_tokens=256)
+        out.append(tc.run_cut(lm, toks, [100, 1]))
+        assert tc.rel(out[-1], out[0]) < 1e-5, (window, keep)      # fp32 sums in another order

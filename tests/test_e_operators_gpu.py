@@ -216,3 +216,13 @@ def test_blocks_far_apart(lib, name):
 
 def test_select_penalties(lib):
     oc.check_select_penalties(DEV, lib)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_keeps_everything(lib, codes):
+    oc.check_keeps_everything(DEV, lib, codes)
+
+
+@pytest.mark.parametrize("codes", [None, "int8", "e4m3"])
+def test_token_lm_keeps_everything(lib, codes):
+    oc.check_token_lm_keeps_everything(DEV, lib, codes)

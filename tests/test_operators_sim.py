@@ -140,3 +140,13 @@ def test_large_lds_is_asked_for_on_every_device(tlm_lib):  # noqa: F811
             dll.hipsim_set_device(0)
         asked.append((both - before, dll.hipsim_attributes(device)))
     assert asked[0][0] == 1 and asked[0][1] > 1 and asked[1] == asked[0] and asked[2] == (0, asked[0][1]), asked
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_keeps_everything(tlm_lib, codes):  # noqa: F811
+    oc.check_keeps_everything(DEV, tlm_lib, codes)
+
+
+@pytest.mark.parametrize("codes", [None, "int8", "e4m3"])
+def test_token_lm_keeps_everything(tlm_lib, codes):  # noqa: F811
+    oc.check_token_lm_keeps_everything(DEV, tlm_lib, codes)
