@@ -142,15 +142,18 @@ typedef struct mmi_kv_seqs {
  * that two sequences of a call write to are different ones. */
 int mmi_kv_append(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                   int64_t v_head, mmi_stream stream);
-/* What the cache holds for those rows: k [rows][kv_heads][dim], v [rows][kv_heads][vdim]; zeros where there is no page. */
+/* What the cache holds for those rows: k [rows][kv_heads][dim], v [rows][kv_heads][vdim]; zeros where there is no page, and in rows that no sequence
+ * brings (one that is passed over brings none). */
 int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, void* k, void* v, mmi_stream stream);
 /* out = softmax(scale q k^T) v over the positions up to a row's own; window > 0: the last `window` of them and the first `keep_first`;
- * sink: one is added to the softmax's denominator.  Query head h reads key/value head h / (heads / kv_heads).  Sums are
- * fp32; bf16 queries and the weights beside them are fp16 operands, fp32 ones two fp16 parts each (22 bits).  A row that sees nothing gets zeros.  workspace: device memory of mmi_kv_attend_workspace bytes (a negative
- * status in its place where the arguments are refused), one per call in flight. */
+ * MMI_KV_SINK: one is added to the softmax's denominator; MMI_KV_ZERO_REST: rows that no sequence brings (one that is passed over brings none)
+ * become zeros, where they otherwise stay as they were.  Query head h reads key/value head h / (heads / kv_heads).  Sums are
+ * fp32; bf16 queries and the weights beside them are fp16 operands, fp32 ones two fp16 parts each (22 bits).  A row that sees nothing gets zeros.
+ * workspace: device memory of mmi_kv_attend_workspace bytes (a negative status in its place where the arguments are refused), one per call in flight. */
+enum { MMI_KV_SINK = 1, MMI_KV_ZERO_REST = 2 };
 int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first);
 int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
-                  int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t sink, void* workspace, int64_t workspace_bytes,
+                  int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t flags, void* workspace, int64_t workspace_bytes,
                   mmi_stream stream);
 
 /* ------------------------------------------------------------------------------------------ */

@@ -109,6 +109,7 @@ TLM_MIX_LATENT_ATTENTION, TLM_MIX_MINGRU, TLM_MIX_ATTENTION, TLM_MIX_CHANNEL_DEL
 TLM_MLP_NONE, TLM_MLP_MOE, TLM_MLP_DENSE = 0, 1, 2
 TLM_ACT_RELU2, TLM_ACT_CLAMPED_SWIGLU, TLM_ROUTE_TOKEN_TABLE = 1, 2, 1
 TLM_LOOP_ADD, TLM_LOOP_PROJECT = 0, 1
+MMI_KV_SINK, MMI_KV_ZERO_REST = 1, 2
 (TLM_PAGE_TOKENS, TLM_TOTAL_PAGES, TLM_FREE_PAGES, TLM_FREE_SLOTS, TLM_POSITION, TLM_HELD_PAGES, TLM_WEIGHT_BYTES, TLM_LAYER_RUNS,
  TLM_GRAPHS) = range(9)
 

@@ -48,6 +48,13 @@ __device__ __forceinline__ TlmKv8Seq kv8_seq(const TlmKv8Seqs& a, int e) {
     s.pos0 = mmi_uniform(pos0);
     return s;
 }
+// Rows that no sequence brings: those before the first sequence, and those from the sequence's end to the next one's start (all of its own, if it is
+// passed over) or to the tensors'.  f(first, end)
+template <class F>
+__device__ __forceinline__ void kv8_rest(const TlmKv8Seqs& a, const TlmKv8Seq& s, F f) {
+    if (s.e == 0) f(0, s.row0);
+    f(s.row0 + s.len, s.e == a.n - 1 ? a.T : mmi_uniform(kv8_row0(a, s.e + 1)));
+}
 // page number of the sequence's tokens 64 i .. 64 i + 63; -1: there is none
 __device__ __forceinline__ int kv8_page(const TlmKv8Seqs& a, int n_pages, const int* row, int i) {
     if (!a.ring && i >= a.pages.ld) return -1;
@@ -165,12 +172,14 @@ struct TlmKv8Append {
 };
 
 // a block of an entry: tokens lo .. hi - 1 of its 16 are new, the ones before are held already
-struct Kv8Span { int page, part, lo, hi, row, pos; bool none; };
+struct Kv8Span { TlmKv8Seq s; int page, part, lo, hi, row, pos; bool none, first; };
 __device__ __forceinline__ Kv8Span kv8_span(const TlmKv8Seqs& q, const Kv8Cut& z, int n_pages, int slot) {
     const int e = kv8_find(q, z, slot);
     const TlmKv8Seq s = kv8_seq(q, e);
     const int i = slot - kv8_slot0(q, z, e), b = s.pos0 / KV8_BLOCK + i;      // block of the sequence
     Kv8Span o;
+    o.s = s;
+    o.first = i == 0;
     o.pos = b * KV8_BLOCK;
     o.none = s.len < 1 || i < 0 || o.pos >= s.pos0 + s.len;      // (i < 0: row starts that do not ascend)
     o.lo = max(s.pos0 - o.pos, 0);
@@ -374,7 +383,7 @@ struct TlmKv8Read {
     TlmKv8Cache c;
     TlmKv8Seqs q;
     Kv8Cut z;
-    void *k, *v;                         // [rows][kv heads][dim], [rows][kv heads][vdim]; tokens without a page: zeros
+    void *k, *v;                         // [rows][kv heads][dim], [rows][kv heads][vdim]; tokens without a page, rows without a sequence: zeros
 };
 __device__ __forceinline__ void kv8_put4(float* p, f32x4 v) { TlmF32::store4(p, v); }
 __device__ __forceinline__ void kv8_put4(uint16_t* p, f32x4 v) { TlmBf16::store4(p, v); }
@@ -386,9 +395,16 @@ template <class Out, bool E4M3>
 __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
     typedef Kv8Code<E4M3> C;
     const Kv8Span s = kv8_span(a.q, a.z, a.c.n_pages, (int)blockIdx.x);
+    const int lane = mmi_lane(), g = (int)blockIdx.y;
+    if (s.first) {
+        const int n = blockIdx.z ? a.c.vdim : a.c.dim;
+        kv8_rest(a.q, s.s, [&](int first, int end) __attribute__((always_inline)) {
+            for (int row = first; row < end; ++row)
+                for (int d = 4 * lane; d < n; d += 256) kv8_put4((Out*)(blockIdx.z ? a.v : a.k) + ((long)row * a.c.kv_heads + g) * n + d, f32x4{0.f, 0.f, 0.f, 0.f});
+        });
+    }
     if (s.none) return;
     const bool lost = s.page < 0;
-    const int lane = mmi_lane(), g = (int)blockIdx.y;
     const long unit = (long)max(s.page, 0) * a.c.kv_heads + g;
     const float scale = lost ? 0.f : (blockIdx.z ? a.c.vs : a.c.ks)[unit * KV8_PARTS + s.part];
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -464,6 +480,7 @@ struct TlmKv8Attn {
     int heads, rep, nd;                  // rep: query heads per key/value head; nd: vdim / 16
     TlmMask mask;                        // scale: log2 e times the softmax's
     int sink;                            // one is added to the denominator
+    int rest;                            // rows that no sequence brings become zeros (few's, which has a slot for every sequence)
     int both;                            // sequences of more than KV8_FEW columns are `many`'s; otherwise all are `few`'s
     Kv8Share few, many;
 };
@@ -680,6 +697,12 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     const int lane = (int)threadIdx.x & 63, wave = mmi_uniform((int)threadIdx.x >> 6), bl = lane & 15, kq = lane >> 4;
     const Kv8Cols c(a, a.few, true, slot);
     kv8_tell(a.few, c, slot, g, split);
+    if (a.rest && split == 0 && c.c0 == 0)
+        kv8_rest(a.q, c.s, [&](int first, int end) __attribute__((always_inline)) {
+            const int n = a.c.vdim / 4 * a.rep;
+            for (int row = first; row < end; ++row)
+                for (int i = (int)threadIdx.x; i < n; i += 256) kv8_store<Tr>(a, row, g * a.rep + i / (a.c.vdim / 4), i % (a.c.vdim / 4) * 4, f32x4{0.f, 0.f, 0.f, 0.f});
+        });
     const int i0 = split * a.few.pages, i1 = min(c.n, i0 + a.few.pages);
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
     const int col = min(c.c0 + bl, c.ncol - 1), tok = col / a.rep, pos = c.s.pos0 + tok;

@@ -211,7 +211,7 @@ extern "C" int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_
 }
 
 extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
-                             int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t sink, void* workspace, int64_t workspace_bytes,
+                             int64_t out_row, int64_t out_head, float scale, int32_t window, int32_t keep_first, int32_t flags, void* workspace, int64_t workspace_bytes,
                              mmi_stream stream) {
     TlmKv8Attn a;
     size_t floats;
@@ -220,6 +220,7 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
     if (!a.q.n || !a.q.T) return MMI_OK;
     if ((rc = check_rows(q, q_row, q_head, dtype, "mmi_kv_attend")) || (rc = check_rows(out, out_row, out_head, dtype, "mmi_kv_attend"))) return rc;
     if (!aligned4(out, out_row, out_head, dtype)) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: four elements of the output must be aligned");
+    if (flags & ~(MMI_KV_SINK | MMI_KV_ZERO_REST)) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: unknown flags");
     if (!(scale == scale) || scale - scale != 0.f) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: the scale is not finite");
     if (floats && (!workspace || workspace_bytes < (int64_t)(floats * sizeof(float)) || (uintptr_t)workspace % 16))
         return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: the workspace is too small (mmi_kv_attend_workspace) or not aligned to 16 bytes");
@@ -231,7 +232,8 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
     a.out_row = out_row;
     a.out_head = out_head;
     a.mask.scale = scale * 1.44269504088896340736f;
-    a.sink = sink;
+    a.sink = flags & MMI_KV_SINK;
+    a.rest = flags & MMI_KV_ZERO_REST;
     tlm_kv8_workspace(a, (float*)workspace);
     return tlm_kv8_attend((hipStream_t)stream, a, dtype, dtype == MMI_F32);
 }

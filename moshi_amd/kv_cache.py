@@ -8,7 +8,8 @@ include/moshi_tlm.h).
 Which page holds what is the caller's: `table` [sequences, pages of a sequence] int32 names them, `positions` [sequences] int32 says where the
 sequence's first row of this call stands, and `rows` [sequences + 1] int32 where its rows lie in the tensors (None: one row each, a decoding
 step).  All three are device tensors and are read when the kernels run, so a captured graph replays with what they hold then.  A page
-number outside the cache stands for no page: rows that belong there are not written, and nothing is seen of it.
+number outside the cache stands for no page: rows that belong there are not written, and nothing is seen of it.  A sequence at a negative
+position is passed over: an unused place of a batch.
 """
 from __future__ import annotations
 
@@ -131,13 +132,18 @@ class PagedKVCache:
                keep_first: int = 0, sink: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of queries [rows, heads, dim] over the positions up to their own, those rows' keys having been appended: [rows, heads, vdim]
         in the queries' type.  scale: default dim ** -0.5.  window > 0: the last `window` positions and the first `keep_first`.  sink: one is
-        added to the softmax's denominator.  Rows that see nothing are zeros; rows behind the last sequence are left as they were."""
+        added to the softmax's denominator.  Rows that see nothing are zeros.  Rows that no sequence brings - behind the last one, or of one that
+        is passed over - are zeros too in a new tensor, and left as they were in `out`."""
         heads, dtype, qp = self._rows(q, "q", None, self.dim)
         total = q.shape[0]
         seqs = self._seqs(table, positions, rows, total)
+        flags = _capi.MMI_KV_SINK if sink else 0
         if out is None:
+            flags |= _capi.MMI_KV_ZERO_REST
             out = torch.empty_like(q) if self.vdim == self.dim and q.is_contiguous() else q.new_empty((total, heads, self.vdim))
             op = (out.data_ptr(), heads * self.vdim, self.vdim)
+            if not seqs.n:
+                out.zero_()
         else:
             if out.shape != (total, heads, self.vdim) or out.dtype != q.dtype:
                 raise AssertionError("out is [rows, heads, vdim] in the queries' type")
@@ -145,13 +151,13 @@ class PagedKVCache:
         need = self._workspace(seqs, (seqs.n, total, seqs.table_ld, heads, window, keep_first, rows is None))
         work = q.new_empty(need, dtype=torch.uint8) if need else None
         self._lib.check(self._on.call(self._lib.mmi_kv_attend, C.byref(self._desc), C.byref(seqs), dtype, heads, *qp, *op, self.dim ** -0.5 if scale is None else scale, window,
-                                      keep_first, sink, work.data_ptr() if need else None, need))
+                                      keep_first, flags, work.data_ptr() if need else None, need))
         return out
 
     def read(self, table: torch.Tensor, positions: torch.Tensor, rows: Optional[torch.Tensor] = None, tokens: Optional[int] = None,
              dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values the cache holds for those positions (keys as they were rotated): [tokens, kv_heads, dim] and [tokens, kv_heads, vdim];
-        zeros where there is no page.  tokens: rows[-1] (without `rows`: one for each sequence)."""
+        zeros where there is no page, and in rows that no sequence brings.  tokens: rows[-1] (without `rows`: one for each sequence)."""
         if rows is not None and tokens is None:
             raise ValueError("tokens is needed beside rows")
         total = positions.shape[0] if rows is None else int(tokens)
@@ -160,5 +166,7 @@ class PagedKVCache:
         seqs = self._seqs(table, positions, rows, total)
         k = self.k_scale.new_empty((total, self.kv_heads, self.dim), dtype=dtype)
         v = torch.empty_like(k) if self.vdim == self.dim else k.new_empty((total, self.kv_heads, self.vdim))
+        if not seqs.n:
+            return k.zero_(), v.zero_()
         self._lib.check(self._on.call(self._lib.mmi_kv_read, C.byref(self._desc), C.byref(seqs), _DTYPES[dtype], k.data_ptr(), v.data_ptr()))
         return k, v

@@ -1071,3 +1071,67 @@ def check_token_lm_keeps_everything(dev, lib, codes):
         lm = TokenLM(sd, replace(cfg, layers=layers), device=dev, dtype=F32, lib=lib, kv_cache=codes, max_slots=2, max_tokens=256)
         out.append(tc.run_cut(lm, toks, [100, 1]))
         assert tc.rel(out[-1], out[0]) < 1e-5, (window, keep)      # fp32 sums in another order
+
+
+from contextlib import contextmanager  # noqa: E402
+
+
+@contextmanager
+def _new_memory_is_nan():
+    """torch.empty and its like give NaN (the largest integers), not what the memory happens to hold."""
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    try:
+        yield
+    finally:
+        torch.use_deterministic_algorithms(False)
+
+
+# `first`: rows before the first sequence; a negative past: passed over, with as many rows as it brings
+RESTS = {
+    "single_tokens": (Case([-1, 4, -7, 70, -2], [1] * 5, single=True, rep=20, kv_heads=1), 0),
+    "single_tokens_fp32": (Case([-1, -3], [1] * 2, single=True, dtype=F32, codes="e4m3", vdim=48), 0),
+    "behind": (Case([5, 12], [2, 20], extra_rows=5, rep=4), 0),
+    "before_and_behind": (Case([70, 3], [30, 1], extra_rows=3, dtype=F32, dim=32, vdim=80), 4),
+    "portions_passed_over": (Case([-1, 40, -64, 9, -5], [18, 3, 1, 25, 7], extra_rows=2, rep=3, codes="e4m3"), 1),
+    "all_passed_over": (Case([-1, -1], [18, 3], extra_rows=2), 3),
+}
+
+
+def check_rest(name, dev, lib):
+    """Rows that no sequence brings: zeros in new tensors, in `out` as they were; the others the same either way."""
+    c, first = RESTS[name]
+    c = Case(**{**c.__dict__, "extra_rows": c.extra_rows + first})
+    cache, q, k, v, args = build(c, dev, lib)
+    if not c.single:
+        args = (args[0], args[1], args[2] + first)
+    cache.append(k, v, *args)
+    brought = torch.zeros(c.total, dtype=torch.bool)
+    for e, p, n, row in sequences(c):
+        brought[row + first:row + first + n] = p >= 0
+    held = torch.full((c.total, c.kv_heads * c.rep, c.vdim), 7.0, dtype=c.dtype, device=dev)
+    cache.attend(q, *args, out=held)
+    with _new_memory_is_nan():
+        fresh = cache.attend(q, *args)
+        got = cache.read(*args, tokens=c.total, dtype=c.dtype)
+    held, fresh, got = held.cpu(), fresh.cpu(), [t.cpu() for t in got]
+    assert (held[~brought] == 7).all() and (fresh[~brought] == 0).all() and torch.equal(held[brought], fresh[brought]) and fresh[brought].isfinite().all()
+    for t in got:
+        assert (t[~brought] == 0).all() and t[brought].isfinite().all() and (t[brought] != 0).flatten(1).any(dim=1).all()
+    with _new_memory_is_nan():                                # no sequence at all
+        none = (args[0][:0], args[1][:0], torch.zeros(1, dtype=torch.int32, device=dev))
+        assert not cache.attend(q, *none).any() and not any(t.any() for t in cache.read(*none, tokens=c.total))
+    held = torch.full_like(fresh, 7.0).to(dev)
+    assert (cache.attend(q, *none, out=held) == 7).all()
+
+
+def check_flags(dev, lib):
+    import ctypes as C
+    from moshi_amd import _capi
+    cache, table, _, i32, g = _filled(dev, lib, 2, 70)
+    pos, q = i32(69), torch.randn((1, 2, 32), generator=g).to(dev)
+    s, out = _capi.KVSeqs(1, 1, None, pos.data_ptr(), table.data_ptr(), 2), torch.zeros_like(q)
+    for flags, status in ((0, 0), (1, 0), (2, 0), (3, 0), (4, _capi.MMI_ERR_INVALID), (-1, _capi.MMI_ERR_INVALID)):
+        need = lib.mmi_kv_attend_workspace(C.byref(cache._desc), C.byref(s), 2, 0, 0)
+        work = torch.empty(max(1, need), dtype=torch.uint8, device=dev)
+        assert lib.mmi_kv_attend(C.byref(cache._desc), C.byref(s), _capi.MMI_F32, 2, q.data_ptr(), 64, 32, out.data_ptr(), 64, 32, 0.1, 0, 0, flags, work.data_ptr(), need,
+                                 _capi.stream_ptr(out.device)) == status

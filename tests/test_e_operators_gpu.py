@@ -226,3 +226,12 @@ def test_keeps_everything(lib, codes):
 @pytest.mark.parametrize("codes", [None, "int8", "e4m3"])
 def test_token_lm_keeps_everything(lib, codes):
     oc.check_token_lm_keeps_everything(DEV, lib, codes)
+
+
+@pytest.mark.parametrize("name", sorted(oc.RESTS))
+def test_rows_that_no_sequence_brings(lib, name):
+    oc.check_rest(name, DEV, lib)
+
+
+def test_flags(lib):
+    oc.check_flags(DEV, lib)

@@ -150,3 +150,12 @@ def test_keeps_everything(tlm_lib, codes):  # noqa: F811
 @pytest.mark.parametrize("codes", [None, "int8", "e4m3"])
 def test_token_lm_keeps_everything(tlm_lib, codes):  # noqa: F811
     oc.check_token_lm_keeps_everything(DEV, tlm_lib, codes)
+
+
+@pytest.mark.parametrize("name", sorted(oc.RESTS))
+def test_rows_that_no_sequence_brings(tlm_lib, name):  # noqa: F811
+    oc.check_rest(name, DEV, tlm_lib)
+
+
+def test_flags(tlm_lib):  # noqa: F811
+    oc.check_flags(DEV, tlm_lib)
