@@ -169,7 +169,9 @@ int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int32_t dtype, 
                     const uint8_t* finished, int32_t eos, float length_penalty, float* out_score, int32_t* out_parent, int32_t* out_token, uint8_t* out_finished,
                     int32_t* out_length, void* workspace, int64_t workspace_bytes, mmi_stream stream);
 /* Row b * beams + i of every tensor (host arrays: device pointers, bytes from row to row, bytes of a row) becomes a copy of what row
- * b * beams + parents[b][i] was; in place.  parents: device int32 [batch][beams]; one outside the request leaves its row alone. */
+ * b * beams + parents[b][i] was; in place.  parents: device int32 [batch][beams]; one outside the request leaves its row alone.  At most 2^16
+ * tensors, which share no memory with one another or with the parents: their ranges are apart, or they are as far from row to row and their rows apart
+ * (views of one buffer).  Ranges that overlap with other distances are refused. */
 int mmi_beam_reorder(int32_t n, void* const* tensors, const int64_t* strides, const int64_t* row_bytes, int32_t batch, int32_t beams, const int32_t* parents,
                      mmi_stream stream);
 

@@ -90,7 +90,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
 
 def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, lib: Optional[_capi.Lib] = None) -> None:
     """In place, for every tensor [requests * beams, ...] of any type: row b * beams + i becomes a copy of what row b * beams + parents[b, i] was.
-    parents: int32 [requests, beams]; one outside the request leaves its row alone.  A row's elements lie together; no two tensors share memory."""
+    parents: int32 [requests, beams]; one outside the request leaves its row alone.  A row's elements lie together; no two tensors share memory,
+    with the parents among them (views of one buffer's rows, as far apart from row to row, may lie between one another)."""
     lib, on = _place(parents.device, lib)
     if parents.dim() != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
         raise ValueError("parents is a contiguous int32 tensor [requests, beams]")

@@ -338,20 +338,55 @@ int tlm_reorder(hipStream_t s, int n, const TlmReorderTensor* tensors, int group
     return MMI_OK;
 }
 
+namespace {
+// Does a byte of one tensor's rows belong to another's, or to the parents?  Tensors whose ranges overlap may be views of one buffer, a row of theirs
+// being a part of its row: with strides that are equal they share nothing where the parts, modulo the stride, are apart.
+bool rows_share_memory(std::vector<TlmReorderTensor> t, int rows, const TlmReorderTensor& parents) {
+    auto end = [&](const TlmReorderTensor& x) { return (uintptr_t)x.p + (uintptr_t)x.stride * (uintptr_t)(rows - 1) + (uintptr_t)x.bytes; };
+    t.erase(std::remove_if(t.begin(), t.end(), [](const TlmReorderTensor& x) { return x.bytes == 0; }), t.end());
+    for (const TlmReorderTensor& x : t) {                  // (the parents' first byte behind x's start: in or behind its row k)
+        const uintptr_t a = (uintptr_t)parents.p, b = a + (uintptr_t)parents.bytes, p = (uintptr_t)x.p;
+        if (b <= p || a >= end(x)) continue;
+        const uintptr_t k = a < p ? 0 : std::min<uintptr_t>((a - p) / (uintptr_t)x.stride, (uintptr_t)rows - 1), row = p + k * (uintptr_t)x.stride;
+        if (a < row + (uintptr_t)x.bytes || (k + 1 < (uintptr_t)rows && b > row + (uintptr_t)x.stride)) return true;
+    }
+    std::sort(t.begin(), t.end(), [](const TlmReorderTensor& x, const TlmReorderTensor& y) { return (uintptr_t)x.p < (uintptr_t)y.p; });
+    for (size_t i = 0; i < t.size();) {                    // a cluster: ranges that overlap one another in a chain
+        size_t j = i + 1;
+        for (uintptr_t to = end(t[i]); j < t.size() && (uintptr_t)t[j].p < to; ++j) to = std::max(to, end(t[j]));
+        if (j > i + 1) {
+            const uintptr_t stride = (uintptr_t)t[i].stride, from = (uintptr_t)t[i].p;
+            std::vector<std::pair<uintptr_t, uintptr_t>> part;
+            for (size_t k = i; k < j; ++k) {
+                if ((uintptr_t)t[k].stride != stride) return true;
+                const uintptr_t at = ((uintptr_t)t[k].p - from) % stride;
+                part.push_back({at, at + (uintptr_t)t[k].bytes});
+            }
+            std::sort(part.begin(), part.end());
+            for (size_t k = 1; k < part.size(); ++k)
+                if (part[k].first < part[k - 1].second) return true;
+            if (part.back().second > stride + part[0].first) return true;
+        }
+        i = j;
+    }
+    return false;
+}
+}  // namespace
+
 extern "C" int mmi_beam_reorder(int32_t n, void* const* tensors, const int64_t* strides, const int64_t* row_bytes, int32_t batch, int32_t beams, const int32_t* parents,
                                 mmi_stream stream) {
     int rc = check_beams(batch, beams, 1, "mmi_beam_reorder");
     if (rc || !batch || !n) return rc;
     if (n < 0 || !tensors || !strides || !row_bytes || !parents) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: null argument");
+    if (n > 1 << 16) return mmi_fail(MMI_ERR_SHAPE, "mmi_beam_reorder: at most 2^16 tensors");
+    const int rows = batch * beams;
     std::vector<TlmReorderTensor> t((size_t)n);
     for (int i = 0; i < n; ++i) {
         if (!tensors[i] || row_bytes[i] < 0 || strides[i] < row_bytes[i]) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: rows are apart and not null");
+        if (strides[i] > (int64_t)1 << 46) return mmi_fail(MMI_ERR_SHAPE, "mmi_beam_reorder: rows are too far apart");      // (65535 of them within 2^62)
         t[i] = TlmReorderTensor{tensors[i], strides[i], row_bytes[i]};
     }
-    std::vector<std::pair<uintptr_t, uintptr_t>> span;     // (a tensor given twice would be read and written by two workgroups)
-    for (const TlmReorderTensor& x : t) span.push_back({(uintptr_t)x.p, (uintptr_t)x.p + (uintptr_t)x.stride * (uintptr_t)(batch * beams - 1) + (uintptr_t)x.bytes});
-    std::sort(span.begin(), span.end());
-    for (int i = 1; i < n; ++i)
-        if (span[i].first < span[i - 1].second) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: two tensors share memory");
+    // (a tensor given twice would be read and written by two workgroups, parents among the rows read by some behind others' writes)
+    if (rows_share_memory(t, rows, TlmReorderTensor{(void*)parents, 4ll * rows, 4ll * rows})) return mmi_fail(MMI_ERR_INVALID, "mmi_beam_reorder: two tensors share memory");
     return tlm_reorder((hipStream_t)stream, n, t.data(), batch, beams, parents, nullptr);
 }

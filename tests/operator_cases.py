@@ -1135,3 +1135,47 @@ def check_flags(dev, lib):
         work = torch.empty(max(1, need), dtype=torch.uint8, device=dev)
         assert lib.mmi_kv_attend(C.byref(cache._desc), C.byref(s), _capi.MMI_F32, 2, q.data_ptr(), 64, 32, out.data_ptr(), 64, 32, 0.1, 0, 0, flags, work.data_ptr(), need,
                                  _capi.stream_ptr(out.device)) == status
+
+
+def check_reorder_views(dev, lib):
+    """Views of one buffer whose rows lie between one another's move like tensors of their own; views that share a byte, and parents among the rows, are refused."""
+    g = torch.Generator().manual_seed(6)
+    parents = torch.tensor([[2, 0, 1, 1], [3, 3, 0, 2]], dtype=torch.int32)
+    at = parents.long().flatten() + torch.tensor([0] * 4 + [4] * 4)
+    kv = torch.randn((8, 2, 3, 8), generator=g)
+    mine = kv.clone().to(dev)
+    beam_reorder([mine[:, 0], mine[:, 1]], parents.to(dev), lib=lib)
+    assert torch.equal(mine.cpu(), kv[at])
+    wide = torch.randint(0, 200, (8, 100), generator=g, dtype=torch.uint8)
+    mine, more = wide.clone().to(dev), kv.clone().to(dev)
+    beam_reorder([mine[:, 60:], more, mine[:, :7], mine[:, 7:20], mine[:, 33:34]], parents.to(dev), lib=lib)
+    want = wide.clone()
+    for part in (slice(60, 100), slice(0, 20), slice(33, 34)):
+        want[:, part] = wide[at][:, part]
+    assert torch.equal(mine.cpu(), want) and torch.equal(more.cpu(), kv[at])
+    # a buffer of rows that a second one begins inside, whole rows later: apart only where the parts are
+    flat = torch.zeros(480, dtype=torch.int32, device=dev)
+    rows = lambda first, n, step=40: torch.as_strided(flat, (8, n), (step, 1), first)  # noqa: E731
+    beam_reorder([rows(0, 10), rows(90, 10), rows(20, 10)], parents.to(dev), lib=lib)
+    for views in ([rows(0, 10), rows(9, 5)], [rows(0, 10), rows(85, 10)], [rows(0, 10), rows(115, 10)], [rows(0, 10), rows(35, 6)], [rows(0, 10), rows(20, 10), rows(25, 3)],
+                  [rows(0, 10), rows(20, 4, 41)], [rows(5, 10), rows(0, 6)]):
+        before = flat.clone()
+        with pytest.raises(ValueError, match="share"):
+            beam_reorder(views, parents.to(dev), lib=lib)
+        assert torch.equal(before, flat)
+    p = flat[40 * 3 + 12:40 * 3 + 20].view(2, 4)               # parents between rows: nobody's
+    p.copy_(parents)
+    beam_reorder([rows(0, 12), rows(20, 20)], p, lib=lib)
+    assert torch.equal(p.cpu(), parents)
+    for views in ([rows(0, 13)], [rows(19, 4)], [flat[:320].view(8, 40)], [rows(20, 10), rows(12, 1)]):
+        with pytest.raises(ValueError, match="share"):
+            beam_reorder(views, p, lib=lib)
+    # rows without a byte share nothing; one row of one tensor may have any distance to its next
+    beam_reorder([flat[:80].view(8, 10), flat[:80].view(8, 10)[:, :0]], parents.to(dev), lib=lib)
+    # more tensors than the entry takes: refused before any of them is looked at
+    import ctypes as C
+    from moshi_amd import _capi
+    place = _capi.LaunchOn(torch.device(dev, 0) if dev == "cuda" else torch.device(dev))
+    one = (C.c_int64 * 1)(flat.data_ptr())
+    assert place.call(lib.mmi_beam_reorder, (1 << 16) + 1, one, one, one, 2, 4, p.data_ptr()) == _capi.MMI_ERR_SHAPE
+    assert place.call(lib.mmi_beam_reorder, 1, one, (C.c_int64 * 1)(1 << 60), (C.c_int64 * 1)(4), 2, 4, p.data_ptr()) == _capi.MMI_ERR_SHAPE

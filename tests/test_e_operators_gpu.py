@@ -235,3 +235,7 @@ def test_rows_that_no_sequence_brings(lib, name):
 
 def test_flags(lib):
     oc.check_flags(DEV, lib)
+
+
+def test_reorder_views(lib):
+    oc.check_reorder_views(DEV, lib)

@@ -159,3 +159,7 @@ def test_rows_that_no_sequence_brings(tlm_lib, name):  # noqa: F811
 
 def test_flags(tlm_lib):  # noqa: F811
     oc.check_flags(DEV, tlm_lib)
+
+
+def test_reorder_views(tlm_lib):  # noqa: F811
+    oc.check_reorder_views(DEV, tlm_lib)
