@@ -39,6 +39,11 @@ int check_rows(const void* p, int64_t row, int64_t head, int dtype, const char* 
     if (dtype != MMI_BF16 && dtype != MMI_F32) return mmi_fail(MMI_ERR_UNSUPPORTED, std::string(at) + ": bf16 or fp32");
     return MMI_OK;
 }
+// do the heads of rows (n elements each) lie apart, heads within rows or rows within heads?
+bool rows_apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t n) {
+    auto fits = [n](int64_t few, int64_t narrow, int64_t many, int64_t wide) { return (few == 1 || narrow >= n) && (many == 1 || (__int128)wide >= (__int128)(few - 1) * narrow + n); };
+    return fits(heads, head, rows, row) || fits(rows, row, heads, head);
+}
 // can four elements be loaded at once?
 bool aligned4(const void* p, int64_t row, int64_t head, int dtype) { return (uintptr_t)p % (dtype == MMI_F32 ? 16 : 8) == 0 && row % 4 == 0 && head % 4 == 0; }
 
@@ -219,6 +224,7 @@ extern "C" int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs,
     if (rc) return rc;
     if (!a.q.n || !a.q.T) return MMI_OK;
     if ((rc = check_rows(q, q_row, q_head, dtype, "mmi_kv_attend")) || (rc = check_rows(out, out_row, out_head, dtype, "mmi_kv_attend"))) return rc;
+    if (!rows_apart(a.q.T, out_row, heads, out_head, a.c.vdim)) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: rows or heads of the output share memory");
     if (!aligned4(out, out_row, out_head, dtype)) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: four elements of the output must be aligned");
     if (flags & ~(MMI_KV_SINK | MMI_KV_ZERO_REST)) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: unknown flags");
     if (!(scale == scale) || scale - scale != 0.f) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: the scale is not finite");

@@ -133,7 +133,7 @@ class PagedKVCache:
         """Attention of queries [rows, heads, dim] over the positions up to their own, those rows' keys having been appended: [rows, heads, vdim]
         in the queries' type.  scale: default dim ** -0.5.  window > 0: the last `window` positions and the first `keep_first`.  sink: one is
         added to the softmax's denominator.  Rows that see nothing are zeros.  Rows that no sequence brings - behind the last one, or of one that
-        is passed over - are zeros too in a new tensor, and left as they were in `out`."""
+        is passed over - are zeros too in a new tensor, and left as they were in `out`, whose rows and heads lie apart."""
         heads, dtype, qp = self._rows(q, "q", None, self.dim)
         total = q.shape[0]
         seqs = self._seqs(table, positions, rows, total)

@@ -1179,3 +1179,26 @@ def check_reorder_views(dev, lib):
     one = (C.c_int64 * 1)(flat.data_ptr())
     assert place.call(lib.mmi_beam_reorder, (1 << 16) + 1, one, one, one, 2, 4, p.data_ptr()) == _capi.MMI_ERR_SHAPE
     assert place.call(lib.mmi_beam_reorder, 1, one, (C.c_int64 * 1)(1 << 60), (C.c_int64 * 1)(4), 2, 4, p.data_ptr()) == _capi.MMI_ERR_SHAPE
+
+
+def check_output_rows(dev, lib):
+    """Outputs whose rows or heads share memory are refused; rows within heads, and gaps, are taken."""
+    cache, table, _, i32, g = _filled(dev, lib, 2, 70)
+    q = torch.randn((3, 2, 32), generator=g).to(dev)
+    args = (q, table, i32(67), i32(0, 3))
+    want = cache.attend(*args)
+    flat = torch.full((400,), 7.0, device=dev)
+    view = lambda row, head: torch.as_strided(flat, (3, 2, 32), (row, head, 1))  # noqa: E731
+    for row, head in ((64, 32), (32, 96), (32, 100), (100, 36), (80, 48), (96, 64), (64, 200)):
+        flat.fill_(7.0)
+        out = view(row, head)
+        assert cache.attend(*args, out=out) is out and torch.equal(out, want), (row, head)
+        out.fill_(7.0)
+        assert (flat == 7).all()
+    for row, head in ((0, 32), (32, 0), (64, 0), (32, 32), (60, 32), (64, 28), (28, 200), (90, 64), (48, 32)):
+        with pytest.raises(ValueError, match="share"):
+            cache.attend(*args, out=view(row, head))
+    assert (flat == 7).all()
+    one = (q[:1], table, i32(67))
+    out = view(0, 32)[:1]
+    assert torch.equal(cache.attend(*one, out=out), cache.attend(*one))      # (a row alone has no distance)

@@ -239,3 +239,7 @@ def test_flags(lib):
 
 def test_reorder_views(lib):
     oc.check_reorder_views(DEV, lib)
+
+
+def test_output_rows(lib):
+    oc.check_output_rows(DEV, lib)

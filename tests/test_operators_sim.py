@@ -163,3 +163,7 @@ def test_flags(tlm_lib):  # noqa: F811
 
 def test_reorder_views(tlm_lib):  # noqa: F811
     oc.check_reorder_views(DEV, tlm_lib)
+
+
+def test_output_rows(tlm_lib):  # noqa: F811
+    oc.check_output_rows(DEV, tlm_lib)
