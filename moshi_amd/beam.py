@@ -55,6 +55,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
             (all but one at a request's start).
         lengths: int32 [requests, beams], tokens so far; needed for a length penalty.
         finished: bool [requests, beams]; a finished beam has one candidate, `eos` at the score and length it has.
+        eos: token that ends a beam; negative: none does.
         length_penalty: candidates are ranked by score / length ** length_penalty; between -16 and 16.
     Equal ranks go to the lower beam, then the lower token.  At most 32 beams.
     """
@@ -71,6 +72,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
             raise ValueError(f"{name} is a contiguous {kind} tensor [requests, beams] on the logits' device")
     if length_penalty and lengths is None:
         raise ValueError("a length penalty needs lengths")
+    if eos >= vocab > 0:
+        raise ValueError("the end token is outside the vocabulary")
     need = _need.get((batch, beams, vocab))
     if need is None:
         need = lib.mmi_beam_select_workspace(batch, beams, vocab)

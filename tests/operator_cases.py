@@ -1202,3 +1202,17 @@ def check_output_rows(dev, lib):
     one = (q[:1], table, i32(67))
     out = view(0, 32)[:1]
     assert torch.equal(cache.attend(*one, out=out), cache.attend(*one))      # (a row alone has no distance)
+
+
+def check_wide_integers(dev, lib):
+    """Integers beyond 32 bits mean what they say: windows are no shorter for it, and an end token is outside the vocabulary."""
+    cache, table, _, i32, g = _filled(dev, lib, 2, 70)
+    q = torch.randn((1, 2, 32), generator=g).to(dev)
+    want = cache.attend(q, table, i32(69))
+    for kw in (dict(window=2 ** 31), dict(window=2 ** 32 + 3), dict(window=2 ** 63), dict(window=3, keep_first=2 ** 31), dict(window=3, keep_first=2 ** 32 + 1)):
+        assert torch.allclose(cache.attend(q, table, i32(69), **kw), want, rtol=2.0 ** -16, atol=2.0 ** -18), kw
+    x, s = torch.zeros((3, 50), device=dev), torch.zeros((1, 3), device=dev)
+    for eos in (50, 2 ** 32 + 3, 2 ** 63):
+        with pytest.raises(ValueError, match="end token"):
+            beam_select(x, s, eos=eos, lib=lib)
+    assert beam_select(x, s, eos=49, lib=lib).finished.shape == (1, 3) and beam_select(x, s, eos=-5, lib=lib).finished is None

@@ -243,3 +243,7 @@ def test_reorder_views(lib):
 
 def test_output_rows(lib):
     oc.check_output_rows(DEV, lib)
+
+
+def test_wide_integers(lib):
+    oc.check_wide_integers(DEV, lib)

@@ -167,3 +167,7 @@ def test_reorder_views(tlm_lib):  # noqa: F811
 
 def test_output_rows(tlm_lib):  # noqa: F811
     oc.check_output_rows(DEV, tlm_lib)
+
+
+def test_wide_integers(tlm_lib):  # noqa: F811
+    oc.check_wide_integers(DEV, tlm_lib)
