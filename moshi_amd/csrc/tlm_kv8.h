@@ -49,11 +49,11 @@ __device__ __forceinline__ TlmKv8Seq kv8_seq(const TlmKv8Seqs& a, int e) {
     return s;
 }
 // Rows that no sequence brings: those before the first sequence, and those from the sequence's end to the next one's start (all of its own, if it is
-// passed over) or to the tensors'.  f(first, end)
+// passed over) or to the tensors'
 template <class F>
 __device__ __forceinline__ void kv8_rest(const TlmKv8Seqs& a, const TlmKv8Seq& s, F f) {
-    if (s.e == 0) f(0, s.row0);
-    f(s.row0 + s.len, s.e == a.n - 1 ? a.T : mmi_uniform(kv8_row0(a, s.e + 1)));
+    const int before = s.e == 0 ? s.row0 : 0, from = s.row0 + s.len, behind = max((s.e == a.n - 1 ? a.T : mmi_uniform(kv8_row0(a, s.e + 1))) - from, 0);
+    for (int i = 0; i < before + behind; ++i) f(i < before ? i : from + i - before);
 }
 // page number of the sequence's tokens 64 i .. 64 i + 63; -1: there is none
 __device__ __forceinline__ int kv8_page(const TlmKv8Seqs& a, int n_pages, const int* row, int i) {
@@ -398,9 +398,8 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
     const int lane = mmi_lane(), g = (int)blockIdx.y;
     if (s.first) {
         const int n = blockIdx.z ? a.c.vdim : a.c.dim;
-        kv8_rest(a.q, s.s, [&](int first, int end) __attribute__((always_inline)) {
-            for (int row = first; row < end; ++row)
-                for (int d = 4 * lane; d < n; d += 256) kv8_put4((Out*)(blockIdx.z ? a.v : a.k) + ((long)row * a.c.kv_heads + g) * n + d, f32x4{0.f, 0.f, 0.f, 0.f});
+        kv8_rest(a.q, s.s, [&](int row) __attribute__((always_inline)) {
+            if (4 * lane < n) kv8_put4((Out*)(blockIdx.z ? a.v : a.k) + ((long)row * a.c.kv_heads + g) * n + 4 * lane, f32x4{0.f, 0.f, 0.f, 0.f});
         });
     }
     if (s.none) return;
@@ -466,8 +465,8 @@ struct Kv8Share {                        // one kernel's part of a call
     Kv8Cut z;                            // of columns (token, head of the group), by groups of z.per
     int cols;                            // columns that a slot can have: z.per, or fewer where no group has more
     int pages, nsplit;                   // pages per split; splits that a group can need
-    float* po;                           // nsplit > 1: [group slot][kv head][split][z.per columns][vdim] un-normalised sums
-    float* pml;                          // [group slot][kv head][split][3][z.per]: references (Kv8Refs: r, off) and sum of weights
+    float* po;                           // nsplit > 1: [group slot][kv head][split][z.per columns][vdim] results of the split alone, without the sink
+    float* pml;                          // [group slot][kv head][split][2][z.per]: reference of the scores, sum of weights
     int* what;                           // [group slot][4]: its columns, the splits that were needed, first row and column of its sequence
 };
 struct TlmKv8Attn {
@@ -528,33 +527,30 @@ __device__ __forceinline__ void kv8_tell(const Kv8Share& h, const Kv8Cols& c, in
     if (h.nsplit > 1 && g == 0 && split == 0 && threadIdx.x == 0)
         *(u32x4*)(h.what + 4 * slot) = u32x4{(unsigned)max(0, c.ncol - c.c0), (unsigned)max(1, (c.n + h.pages - 1) / h.pages), (unsigned)c.s.row0, (unsigned)c.c0};
 }
-// 2^x, x whole (a NaN, where nothing has been seen yet: zero)
-__device__ __forceinline__ float kv8_two(float x) { return __builtin_ldexpf(1.f, (int)fminf(fmaxf(x, -200.f), 200.f)); }
-// exponent of a value scale, at least -100: what lies below fits into the weights' 2^7 and more
-__device__ __forceinline__ float kv8_exponent(float scale) { return (float)min(max((int)(__builtin_bit_cast(unsigned, scale) >> 23 & 255u) - 127, -100), 126); }
+// exponent of a value scale as it is stored, 127 for [1, 2); at least 27: what lies below 2^-100 fits into the weights' 2^7 and more
+__device__ __forceinline__ float kv8_exponent(float scale) { return (float)max(__builtin_bit_cast(unsigned, scale) >> 23 & 255u, 27u); }
 // A column's references: r = ceil(maximum of the scores) when it was moved last, off the same of score - r + exponent of the value scale.
 struct Kv8Refs {
-    float r = -INFINITY, off = -INFINITY;
-    float up = 0.f;                      // 2^(KV8_UP - off): weights times value scale times this are the product's operand
+    static constexpr float LEAST = -3.4028234663852886e38f, NONE = -1024.f;      // nothing has been seen (finite, so that differences are numbers)
+    float r = LEAST, off = NONE;
+    float up = 0.f;                      // 2^(KV8_UP + 127 - off): weights times value scale times this are the product's operand
     // does a lane's maximum `top` of scores in a block of exponent e outgrow one of them?
-    __device__ __forceinline__ bool outgrown(float top, float e) const { return top > r + KV8_SLACK || top - r + e > off + KV8_SLACK; }
+    __device__ __forceinline__ bool outgrown(float top, float e) const { return top - r + fmaxf(e - off, 0.f) > KV8_SLACK; }
     // moved to the column's maxima (max over its lanes: `across`); factors of the sum of weights and of the weighted sums
     template <class F>
     __device__ __forceinline__ void move(float top, float e, F across, float& fewer, float& less) {
-        const float to = fmaxf(r, ceilf(across(top))), step = to - r;
-        const float held = off - step, out = fmaxf(held, ceilf(across(top - (to == -INFINITY ? 0.f : to) + e)));
-        fewer = kv8_two(-step);
-        less = kv8_two(held - out);
+        const float to = fmaxf(r, ceilf(across(top))), held = off - (to - r), out = fmaxf(held, ceilf(across(top - to + e)));
+        fewer = mmi_fast_exp2f(r - to);
+        less = mmi_fast_exp2f(held - out);
         r = to;
         off = out;
-        up = kv8_two(KV8_UP - off);
+        up = mmi_fast_exp2f(KV8_UP + 127.f - off);
     }
-    __device__ __forceinline__ float base() const { return r == -INFINITY ? 0.f : r; }
-    // what a block's weights are multiplied by: its scale and `up` (where that is beyond fp32, all of its weights are below 2^-100 of the largest); a block
-    // that the column does not see may have any scale
+    // what a block's weights are multiplied by: its scale and `up` (where that leaves fp32, all of its weights are below 2^-100 of the largest); a block that
+    // the column does not see may have any scale
     __device__ __forceinline__ float times(float scale, float top) const {
         const float x = scale * up;
-        return top == -INFINITY ? 0.f : (fabsf(x) > 0x1p126f && fabsf(scale) < INFINITY ? 0x1p126f : x);
+        return top == -INFINITY ? 0.f : (fabsf(x) > 0x1p126f ? 0x1p126f : x);
     }
 };
 // scores of keys key0 .. key0 + 15 for a query at `pos`, -infinity where it does not see them
@@ -680,10 +676,8 @@ __device__ __forceinline__ void kv8_store(const TlmKv8Attn& a, int row, int head
 // 1 / denominator of weights that were summed relative to 2^r; nothing seen: zero
 __device__ __forceinline__ float kv8_inverse(float L, float r, int sink) {
     const float sum = sink ? L + exp2f(-r) : L;
-    return r == -INFINITY && sum == sum ? 0.f : 1.f / sum;
+    return sum == 0.f ? 0.f : 1.f / sum;
 }
-// weighted sums -> outputs (two factors: at the scales' ends either alone is in range)
-__device__ __forceinline__ f32x4 kv8_result(f32x4 v, float inverse, float off) { return v * inverse * kv8_two(off - KV8_UP); }
 
 // Few columns: four waves share one tile of 16 columns, each takes every fourth of its pages straight from the cache - the page after it is
 // asked for before the products of this one - and their sums meet in LDS.  Bound by the codes' way from memory: 100 003 keys of 8 heads of 128
@@ -697,11 +691,10 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     const int lane = (int)threadIdx.x & 63, wave = mmi_uniform((int)threadIdx.x >> 6), bl = lane & 15, kq = lane >> 4;
     const Kv8Cols c(a, a.few, true, slot);
     kv8_tell(a.few, c, slot, g, split);
-    if (a.rest && split == 0 && c.c0 == 0)
-        kv8_rest(a.q, c.s, [&](int first, int end) __attribute__((always_inline)) {
-            const int n = a.c.vdim / 4 * a.rep;
-            for (int row = first; row < end; ++row)
-                for (int i = (int)threadIdx.x; i < n; i += 256) kv8_store<Tr>(a, row, g * a.rep + i / (a.c.vdim / 4), i % (a.c.vdim / 4) * 4, f32x4{0.f, 0.f, 0.f, 0.f});
+    if (a.rest && split == 0 && c.c0 == 0 && (a.both || c.ncol == 0))
+        kv8_rest(a.q, c.s, [&](int row) __attribute__((always_inline)) {
+            for (int head = wave; head < a.rep; head += 4)
+                if (4 * lane < a.c.vdim) kv8_store<Tr>(a, row, g * a.rep + head, 4 * lane, f32x4{0.f, 0.f, 0.f, 0.f});
         });
     const int i0 = split * a.few.pages, i1 = min(c.n, i0 + a.few.pages);
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
@@ -790,12 +783,12 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
 #pragma unroll
             for (int d = 0; d < ND; ++d) acc[d] *= less;
         }
-        const float base = ref.base(), times = ref.times(vsn, mx);
+        const float times = ref.times(vsn, mx);
         u32x4 pf[2][NS];
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            y[r] = mmi_fast_exp2f(y[r] - base);
+            y[r] = mmi_fast_exp2f(y[r] - ref.r);
             sum += y[r];
         }
         l += sum;
@@ -820,17 +813,17 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         ml[2][wave][bl] = l;
     }
     __syncthreads();
-    float R = -INFINITY, O = -INFINITY, L = 0.f;
+    float R = Kv8Refs::LEAST, O = Kv8Refs::NONE, L = 0.f;
 #pragma unroll
     for (int v = 0; v < WK; ++v) R = fmaxf(R, ml[0][v][bl]);
 #pragma unroll
     for (int v = 0; v < WK; ++v) {
         O = fmaxf(O, ml[1][v][bl] + (ml[0][v][bl] - R));
-        L += ml[2][v][bl] * kv8_two(ml[0][v][bl] - R);
+        L += ml[2][v][bl] * mmi_fast_exp2f(ml[0][v][bl] - R);
     }
-    const float f = kv8_two(ref.off + (ref.r - R) - O);
+    const float f = mmi_fast_exp2f(ref.off + (ref.r - R) - O);
     const bool parts = a.few.nsplit > 1;
-    const float inv = kv8_inverse(L, R, a.sink);
+    const float inv = kv8_inverse(L, R, !parts && a.sink), up = mmi_fast_exp2f(O - 127.f - KV8_UP);      // (either alone is in range at the scales' ends)
     const long part = ((long)slot * a.c.kv_heads + g) * a.few.nsplit + split;
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += 8) {
@@ -847,17 +840,16 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
             f32x4 v = ob[d * 64 + lane];
 #pragma unroll
             for (int o = 1; o < WK; ++o) v += ob[(o * 8 + d) * 64 + lane];
+            v = v * inv * up;
             if (!live) continue;
-            if (!parts) v = kv8_result(v, inv, O);
             const int dim = (d0 + d) * 16 + 4 * kq, head = g * a.rep + col - tok * a.rep;
             if (parts) *reinterpret_cast<f32x4*>(a.few.po + (part * 16 + bl) * a.c.vdim + dim) = v;
             else kv8_store<Tr>(a, c.s.row0 + tok, head, dim, v);
         }
     }
     if (parts && wave == 0 && kq == 0) {
-        a.few.pml[part * 48 + bl] = R;
-        a.few.pml[part * 48 + 16 + bl] = O;
-        a.few.pml[part * 48 + 32 + bl] = L;
+        a.few.pml[part * 32 + bl] = R;
+        a.few.pml[part * 32 + 16 + bl] = L;
     }
 }
 // grid: slots of tiles, kv heads, splits
@@ -1068,11 +1060,11 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
             }
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float base = ref[t].base(), times = ref[t].times(vsn, mx[t]);
+                const float times = ref[t].times(vsn, mx[t]);
                 float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    y[t][r] = mmi_fast_exp2f(y[t][r] - base);
+                    y[t][r] = mmi_fast_exp2f(y[t][r] - ref[t].r);
                     sum += y[t][r];
                 }
                 l[t] += sum;
@@ -1127,22 +1119,21 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int n = wave * 32 * QT + 32 * t + cl;        // column of the group
-        const float L = mmi_halves_sum(l[t]), inv = kv8_inverse(L, ref[t].r, a.sink);
+        const float L = mmi_halves_sum(l[t]), inv = kv8_inverse(L, ref[t].r, !parts && a.sink), up = mmi_fast_exp2f(ref[t].off - 127.f - KV8_UP);
         if (c.c0 + n >= c.ncol) continue;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int dim = 32 * d + 8 * r + 4 * hi;
-                const f32x4 v = f32x4{acc[t][d][4 * r], acc[t][d][4 * r + 1], acc[t][d][4 * r + 2], acc[t][d][4 * r + 3]};
+                const f32x4 v = f32x4{acc[t][d][4 * r], acc[t][d][4 * r + 1], acc[t][d][4 * r + 2], acc[t][d][4 * r + 3]} * inv * up;
                 if (dim >= a.c.vdim) continue;
                 if (parts) *reinterpret_cast<f32x4*>(a.many.po + (part * Z::PER + n) * a.c.vdim + dim) = v;
-                else kv8_store<Tr>(a, c.s.row0 + tok[t], head[t], dim, kv8_result(v, inv, ref[t].off));
+                else kv8_store<Tr>(a, c.s.row0 + tok[t], head[t], dim, v);
             }
         if (parts && hi == 0) {
-            a.many.pml[part * 3 * Z::PER + n] = ref[t].r;
-            a.many.pml[part * 3 * Z::PER + Z::PER + n] = ref[t].off;
-            a.many.pml[part * 3 * Z::PER + 2 * Z::PER + n] = L;
+            a.many.pml[part * 2 * Z::PER + n] = ref[t].r;
+            a.many.pml[part * 2 * Z::PER + Z::PER + n] = L;
         }
     }
 }
@@ -1182,19 +1173,18 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
     if constexpr (!WIDE) {
         const int lane = tid & 63, G = a.c.vdim / 4, at_once = 64 / G, n = (b - slot * each) * at_once + lane / G, d = 4 * (lane % G);
         const bool on = lane / G < at_once && n < h.cols;
-        const float *ml0 = h.pml + part * 3 * per, *po0 = h.po + part * per * a.c.vdim;
+        const float *ml0 = h.pml + part * 2 * per, *po0 = h.po + part * per * a.c.vdim;
         const unsigned at_ml = on ? n : 0, at_po = at_ml * a.c.vdim + d;
         const int step = per * a.c.vdim;                   // (a split's part: addresses are a scalar and a lane's offset)
-        float m[8], e[8], l[8];
+        float m[8], l[8];
         f32x4 v[8];
         auto load = [&](int k0, int ns) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (k0 + k < ns) {
-                    const float* ml = ml0 + (k0 + k) * 3 * per;
+                    const float* ml = ml0 + (k0 + k) * 2 * per;
                     m[k] = ml[at_ml];
-                    e[k] = (ml + per)[at_ml];
-                    l[k] = (ml + 2 * per)[at_ml];
+                    l[k] = (ml + per)[at_ml];
                     v[k] = *(const f32x4*)(po0 + (k0 + k) * step + at_po);
                 }
         };
@@ -1202,65 +1192,52 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
         const int col = c0 + n;
         if (!on || n >= cols) return;
         if (!few) load(0, ns);                             // (of the slots that portions might need, half are empty)
-        float R = -INFINITY, O = -INFINITY, L = 0.f;
+        float R = Kv8Refs::LEAST, L = 0.f;                 // the splits so far: their reference, sum, and result (a mean: no sum of values leaves fp32)
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         for (int k0 = 0;;) {
             float r = R;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (k0 + k < ns) r = fmaxf(r, m[k]);
-            const float held = O + (R - r);
-            float off = held;
+            L *= mmi_fast_exp2f(R - r);
+            float all = L;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (k0 + k < ns) off = fmaxf(off, e[k] + (m[k] - r));
-            L *= kv8_two(R - r);
-            o *= kv8_two(held - off);
+                if (k0 + k < ns) all += l[k] *= mmi_fast_exp2f(m[k] - r);
+            const float inv = kv8_inverse(all, r, k0 + 8 >= ns && a.sink);
+            o *= L * inv;
             R = r;
-            O = off;
+            L = all;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (k0 + k < ns) {
-                    L += l[k] * kv8_two(m[k] - r);
-                    o += v[k] * kv8_two(e[k] + (m[k] - r) - off);
-                }
+                if (k0 + k < ns) o += v[k] * (l[k] * inv);
             if ((k0 += 8) >= ns) break;
             load(k0, ns);
         }
         const int tok = col / a.rep;
-        kv8_store<Tr>(a, row0 + tok, g * a.rep + col - tok * a.rep, d, kv8_result(o, kv8_inverse(L, R, a.sink), O));
+        kv8_store<Tr>(a, row0 + tok, g * a.rep + col - tok * a.rep, d, o);
     } else {
-        MMI_SHARED float wt[256], red[4][3];
+        MMI_SHARED float wt[256], red[4][2];
         MMI_SHARED __attribute__((aligned(16))) f32x4 sum[256];
         const int n = b - slot * each;
         const int col = c0 + n;                            // (ns: at most 256)
         if (n >= cols) return;
         const int tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
-        float m = -INFINITY, e = -INFINITY, l = 0.f;
+        float m = Kv8Refs::LEAST, l = 0.f;
         if (tid < ns) {
-            const float* ml = h.pml + (part + tid) * 3 * per + n;
-            m = ml[0];
-            e = ml[per];
-            l = ml[2 * per];
+            m = h.pml[(part + tid) * 2 * per + n];
+            l = h.pml[(part + tid) * 2 * per + per + n];
         }
         const float wm = mmi_wave_max_f32(m);
         if ((tid & 63) == 0) red[wave][0] = wm;
         __syncthreads();
-        float R = -INFINITY, O = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) R = fmaxf(R, red[w][0]);
-        e += m - R;                                        // (nothing seen: -infinity or a NaN, which maxima pass over)
-        const float we = mmi_wave_max_f32(e), wl = mmi_wave_sum_down(tid < ns ? l * kv8_two(m - R) : 0.f);
-        if ((tid & 63) == 0) {
-            red[wave][1] = wl;
-            red[wave][2] = we;
-        }
+        const float R = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+        l *= mmi_fast_exp2f(m - R);
+        const float wl = mmi_wave_sum_down(l);
+        if ((tid & 63) == 0) red[wave][1] = wl;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 4; ++w) O = fmaxf(O, red[w][2]);
-        wt[tid] = kv8_two(e - O);
+        wt[tid] = l * kv8_inverse((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]), R, a.sink);
         __syncthreads();
-        const float inv = kv8_inverse((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]), R, a.sink);
         const int q = tid & 15, k = tid >> 4;
         for (int d0 = 0; d0 < a.c.vdim; d0 += 64) {
             const int d = d0 + 4 * q;
@@ -1274,7 +1251,7 @@ __global__ __launch_bounds__(256) void k_tlm_kv8_combine(TlmKv8Attn a, int first
             if (k == 0 && d < a.c.vdim) {
 #pragma unroll
                 for (int i = 1; i < 16; ++i) v += sum[16 * i + q];
-                kv8_store<Tr>(a, row0 + tok, head, d, kv8_result(v, inv, O));
+                kv8_store<Tr>(a, row0 + tok, head, d, v);
             }
         }
     }

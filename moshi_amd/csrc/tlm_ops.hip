@@ -99,7 +99,7 @@ size_t split_pages(const TlmKv8Attn& a, Kv8Share& h, long groups, long cap, size
         cap = std::min<long>(cap, ((long)a.mask.window + h.z.per / a.rep + 1) / TLM_PAGE + 2 + mmi_cdiv(a.mask.keep, TLM_PAGE));
     cap = std::max(cap, 1l);
     const long units = std::max(1l, groups * a.c.kv_heads);
-    const size_t each = (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.z.per * (a.c.vdim + 3);      // floats per split
+    const size_t each = (size_t)kv8_slots(a.q, h.z) * a.c.kv_heads * h.z.per * (a.c.vdim + 2);      // floats per split
     const size_t what = 4 * (size_t)kv8_slots(a.q, h.z);
     long most = room > what ? std::min<long>(KV8_MAX_SPLIT, (long)((room - what) / std::max<size_t>(1, each))) : 1;
     if (most < 2) most = 1;
@@ -144,7 +144,7 @@ void tlm_kv8_workspace(TlmKv8Attn& a, float* w) {
         const size_t parts = (size_t)kv8_slots(a.q, h->z) * a.c.kv_heads * h->nsplit * h->z.per;
         h->po = w;
         h->pml = w + parts * a.c.vdim;
-        w += parts * (a.c.vdim + 3);
+        w += parts * (a.c.vdim + 2);
         h->what = (int*)w;
         w += 4 * kv8_slots(a.q, h->z);
     }

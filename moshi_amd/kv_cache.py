@@ -23,6 +23,7 @@ from . import _capi
 
 PAGE_TOKENS, BLOCK_TOKENS = 64, 16
 _LONGEST = 2 ** 31 - 1                   # no sequence has more positions
+_SINK, _ZERO_REST = _capi.MMI_KV_SINK, _capi.MMI_KV_ZERO_REST
 _CODES = {torch.int8: _capi.MMI_I8, torch.float8_e4m3fn: _capi.MMI_F8E4M3}
 _NAMES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 _DTYPES = {torch.bfloat16: _capi.MMI_BF16, torch.float32: _capi.MMI_F32}
@@ -135,13 +136,14 @@ class PagedKVCache:
         in the queries' type.  scale: default dim ** -0.5.  window > 0: the last `window` positions and the first `keep_first`.  sink: one is
         added to the softmax's denominator.  Rows that see nothing are zeros.  Rows that no sequence brings - behind the last one, or of one that
         is passed over - are zeros too in a new tensor, and left as they were in `out`, whose rows and heads lie apart."""
-        window, keep_first = min(window, _LONGEST), min(keep_first, _LONGEST)
+        if window > _LONGEST or keep_first > _LONGEST:
+            window, keep_first = min(window, _LONGEST), min(keep_first, _LONGEST)
         heads, dtype, qp = self._rows(q, "q", None, self.dim)
         total = q.shape[0]
         seqs = self._seqs(table, positions, rows, total)
-        flags = _capi.MMI_KV_SINK if sink else 0
+        flags = _SINK if sink else 0
         if out is None:
-            flags |= _capi.MMI_KV_ZERO_REST
+            flags |= _ZERO_REST
             out = torch.empty_like(q) if self.vdim == self.dim and q.is_contiguous() else q.new_empty((total, heads, self.vdim))
             op = (out.data_ptr(), heads * self.vdim, self.vdim)
             if not seqs.n:
