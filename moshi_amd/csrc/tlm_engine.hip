@@ -1478,7 +1478,6 @@ MixerOut build_attention_8(mmi_tlm* m, MmiProgram& P, const Shape& sh, const Lay
     a.wide = 1;
     a.out = m->o;
     a.out_ks = L.out.KS;
-    a.heads = H;
     a.rep = H / G;
     a.nd = L.nd;
     a.mask = TlmMask{L.c.window, L.c.window > 0 ? L.c.keep_first : 0, L.c.scale * 1.44269504088896340736f};

@@ -476,7 +476,7 @@ struct TlmKv8Attn {
     int wide;                            // every 4 of their elements are aligned
     void* out; long out_row, out_head;   // rows; out_ks > 0: fragment-packed rows (tlm_index), columns head * 16 nd + d
     int out_ks;
-    int heads, rep, nd;                  // rep: query heads per key/value head; nd: vdim / 16
+    int rep, nd;                         // query heads per key/value head; vdim / 16
     TlmMask mask;                        // scale: log2 e times the softmax's
     int sink;                            // one is added to the denominator
     int rest;                            // rows that no sequence brings become zeros (few's, which has a slot for every sequence)
@@ -863,7 +863,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8At
 // 128 columns and not 256: with two tiles a wave, accumulators leave one workgroup on a CU and moves between register files (422 us instead of 227).
 // A prompt of 4001 tokens, 32 heads of 128 over 8: 215 us, 610 TFLOP/s, half of what a large bf16 product reaches here; bound by the vector work between
 // the products (exponentials, masks, the conversion of codes and weights).
-// Many columns: four waves x QT tiles of 32 columns of one sequence and kv head walk the same keys, 32 at a time.  Codes become operand
+// Many columns: four waves of 32 columns of one sequence and kv head walk the same keys, 32 at a time.  Codes become operand
 // fragments on their way into LDS, once for all waves; 32 x 32 products read an operand half as often as 16 x 16 ones.  The scores of step
 // i + 1 are formed beside the softmax of step i; keys lie two steps ahead of their use and values one, one barrier a step.
 //   score rows: row 8 a + 4 h + i of the product is key 16 h + 4 a + i, so lane half h holds block h's 16 keys in order
@@ -871,7 +871,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_tlm_kv8_attn(TlmKv8At
 //   lane ^ 4 (lane / 32): what lets the writers, who have 16 codes of one key or dimension each, meet no bank twice
 template <int NS, int D>
 struct Kv8Tile {
-    static constexpr int QT = 1, PER = KV8_MANY, KS = D / 16, DT = D / 32;
+    static constexpr int PER = KV8_MANY, KS = D / 16, DT = D / 32;
     static constexpr int KF = KS * 64, VF = DT * 2 * 64;                       // vectors per buffer
     static constexpr size_t smem() { return std::max({(size_t)2 * (KF + VF) * 16, (size_t)PER * D * NS * 2 + PER * 4 + KV8_ANGLES * 8, (size_t)KV8_LDS * 16}); }
 };
@@ -879,7 +879,7 @@ template <class In, class Tr, int NS, int D, bool E4M3>
 __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, int slot, int g, int split) {
     typedef Kv8Code<E4M3> C;
     typedef Kv8Tile<NS, D> Z;
-    constexpr int QT = Z::QT, KS = Z::KS, DT = Z::DT, KU = D > 128 ? 2 : 1;      // units of 16 codes per thread and side
+    constexpr int KS = Z::KS, DT = Z::DT, KU = D > 128 ? 2 : 1;      // units of 16 codes per thread and side
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = mmi_uniform(tid >> 6), cl = lane & 31, hi = lane >> 5;
     const Kv8Cols c(a, a.many, false, slot);
     kv8_tell(a.many, c, slot, g, split);
@@ -888,16 +888,10 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
     if (i1 == 2 * c.n && c.n > 0 && c.page(c.n - 1) * TLM_PAGE + 32 > c.phi) --i1;      // (the last page's second half lies ahead of every column)
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
     const int* bt = kv8_table(a.q, c.s.e);
-    const int w0 = c.c0 + wave * 32 * QT;                  // the wave's first column
+    const int w0 = c.c0 + wave * 32;                  // the wave's first column
     const bool busy = w0 < c.ncol;
-    const int plo = c.s.pos0 + min(w0, c.ncol - 1) / a.rep, phi = c.s.pos0 + min(w0 + 32 * QT - 1, c.ncol - 1) / a.rep;
-    int tok[QT], head[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int col = min(w0 + 32 * t + cl, c.ncol - 1);
-        tok[t] = col / a.rep;
-        head[t] = g * a.rep + col - tok[t] * a.rep;
-    }
+    const int plo = c.s.pos0 + min(w0, c.ncol - 1) / a.rep, phi = c.s.pos0 + min(w0 + 31, c.ncol - 1) / a.rep;
+    const int col = min(w0 + cl, c.ncol - 1), tok = col / a.rep, head = g * a.rep + col - tok * a.rep;
     // ---- codes -> LDS
     u32x4 *kb = lds, *vb = lds + 2 * Z::KF;
     u32x4 kr[KU], vr[KU];
@@ -938,21 +932,18 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         z0 = find(i0);
         load_k(z0);
     }
-    u32x4 q[QT][KS][NS];                                   // dimensions 16 s + 8 hi ..
-    float back[QT];
+    u32x4 q[KS][NS];                                       // dimensions 16 s + 8 hi ..
+    float back;
     {
         float* turned = reinterpret_cast<float*>(lds + Z::PER * D * NS / 8);      // inverse factors, then angles
         kv8_queries<In, NS, D>(a, c, Z::PER, g, turned + Z::PER, turned, [&](int n, int k, int p) __attribute__((always_inline)) {
             return lds + (((n >> 5) * KS + (k >> 1)) * NS + p) * 64 + 32 * (k & 1) + (n & 31);
         });
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
+        for (int j = 0; j < KS; ++j)
 #pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int p = 0; p < NS; ++p) q[t][j][p] = lds[(((wave * QT + t) * KS + j) * NS + p) * 64 + lane];
-            back[t] = turned[(wave * QT + t) * 32 + cl] * a.mask.scale;
-        }
+            for (int p = 0; p < NS; ++p) q[j][p] = lds[((wave * KS + j) * NS + p) * 64 + lane];
+        back = turned[wave * 32 + cl] * a.mask.scale;
         __syncthreads();                                   // (their memory takes keys and values)
     }
     for (int i = tid; i < 2 * Z::KF; i += 256)
@@ -986,18 +977,14 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         ks = a.c.ks[n];
         vs = a.c.vs[n];
     };
-    f32x16 acc[QT][DT];
-    Kv8Refs ref[QT];
-    float l[QT];
+    f32x16 acc[DT];
+    Kv8Refs ref;
+    float l = 0.f;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        l[t] = 0.f;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[t][d][r] = 0.f;
-    }
-    f32x16 s[2][QT];
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    f32x16 s[2];
     u32x4 fr[8];                                           // operand fragments, asked for eight at a time
     auto ask_k = [&](int buf, int j0) __attribute__((always_inline)) {
 #pragma unroll
@@ -1006,9 +993,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
     };
     auto scores = [&](int set, int buf) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[set][t][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[set][r] = 0.f;
 #pragma unroll
         for (int j0 = 0; j0 < KS; j0 += 8) {
             ask_k(buf, j0);
@@ -1017,9 +1002,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
             for (int j = 0; j < 8; ++j)
                 if (j0 + j < KS)
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
-#pragma unroll
-                        for (int n = NS - 1; n >= 0; --n) s[set][t] = mmi_mfma_f16_32x32x16(fr[j], q[t][j0 + j][n], s[set][t]);
+                    for (int n = NS - 1; n >= 0; --n) s[set] = mmi_mfma_f16_32x32x16(fr[j], q[j0 + j][n], s[set]);
         }
     };
     const int vl = lane ^ (4 * hi);
@@ -1032,45 +1015,30 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         if (busy && now && key0 <= phi) {
             const bool whole = kv8_whole(a.mask, plo, phi, key0, 32);
             const float ev = kv8_exponent(vsn);
-            u32x4 pf[QT][2][NS];
-            float mx[QT], y[QT][16];
-            bool moved = false;
+            u32x4 pf[2][NS];
+            const float sc = ksn * back;
+            float mx = -INFINITY, sum = 0.f, y[16];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                const float sc = ksn * back[t];
-                const int pos = c.s.pos0 + tok[t];
-                float x = -INFINITY;
+            for (int r = 0; r < 16; ++r) y[r] = s[set][r] * sc;
+            if (!whole) kv8_masked(a.mask, c.s.pos0 + tok, key0 + 16 * hi, y);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) y[t][r] = s[set][t][r] * sc;
-                if (!whole) kv8_masked(a.mask, pos, key0 + 16 * hi, y[t]);
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[r]);
+            if (mmi_any(w0 + cl < c.ncol && ref.outgrown(mx, ev))) {       // (the tile's other columns hold anything)
+                float fewer, less;
+                ref.move(mx, ev, [](float x) { return mmi_halves_max(x); }, fewer, less);
+                l *= fewer;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x = fmaxf(x, y[t][r]);
-                mx[t] = x;
-                moved = moved || (w0 + 32 * t + cl < c.ncol && ref[t].outgrown(x, ev));      // (the tile's other columns hold anything)
+                for (int d = 0; d < DT; ++d) acc[d] *= less;
             }
-            if (mmi_any(moved)) {
+            const float times = ref.times(vsn, mx);
 #pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    float fewer, less;
-                    ref[t].move(mx[t], ev, [](float x) { return mmi_halves_max(x); }, fewer, less);
-                    l[t] *= fewer;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[t][d] *= less;
-                }
+            for (int r = 0; r < 16; ++r) {
+                y[r] = mmi_fast_exp2f(y[r] - ref.r);
+                sum += y[r];
             }
+            l += sum;
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                const float times = ref[t].times(vsn, mx[t]);
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    y[t][r] = mmi_fast_exp2f(y[t][r] - ref[t].r);
-                    sum += y[t][r];
-                }
-                l[t] += sum;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) kv8_split8<NS>(y[t] + 8 * u, times, pf[t][u]);
-            }
+            for (int u = 0; u < 2; ++u) kv8_split8<NS>(y + 8 * u, times, pf[u]);
 #pragma unroll
             for (int d0 = 0; d0 < DT; d0 += 4) {
 #pragma unroll
@@ -1081,9 +1049,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
                 for (int k = 0; k < 8; ++k)
                     if (d0 + k / 2 < DT)
 #pragma unroll
-                        for (int t = 0; t < QT; ++t)
-#pragma unroll
-                            for (int n = NS - 1; n >= 0; --n) acc[t][d0 + k / 2] = mmi_mfma_f16_32x32x16(fr[k], pf[t][k & 1][n], acc[t][d0 + k / 2]);
+                        for (int n = NS - 1; n >= 0; --n) acc[d0 + k / 2] = mmi_mfma_f16_32x32x16(fr[k], pf[k & 1][n], acc[d0 + k / 2]);
             }
         }
         put_k(set);
@@ -1116,25 +1082,22 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
     }
     const bool parts = a.many.nsplit > 1;
     const long part = ((long)slot * a.c.kv_heads + g) * a.many.nsplit + split;
+    const int n = wave * 32 + cl;                          // column of the group
+    const float L = mmi_halves_sum(l), inv = kv8_inverse(L, ref.r, !parts && a.sink), up = mmi_fast_exp2f(ref.off - 127.f - KV8_UP);
+    if (c.c0 + n >= c.ncol) return;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int n = wave * 32 * QT + 32 * t + cl;        // column of the group
-        const float L = mmi_halves_sum(l[t]), inv = kv8_inverse(L, ref[t].r, !parts && a.sink), up = mmi_fast_exp2f(ref[t].off - 127.f - KV8_UP);
-        if (c.c0 + n >= c.ncol) continue;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int dim = 32 * d + 8 * r + 4 * hi;
-                const f32x4 v = f32x4{acc[t][d][4 * r], acc[t][d][4 * r + 1], acc[t][d][4 * r + 2], acc[t][d][4 * r + 3]} * inv * up;
-                if (dim >= a.c.vdim) continue;
-                if (parts) *reinterpret_cast<f32x4*>(a.many.po + (part * Z::PER + n) * a.c.vdim + dim) = v;
-                else kv8_store<Tr>(a, c.s.row0 + tok[t], head[t], dim, v);
-            }
-        if (parts && hi == 0) {
-            a.many.pml[part * 2 * Z::PER + n] = ref[t].r;
-            a.many.pml[part * 2 * Z::PER + Z::PER + n] = L;
+        for (int r = 0; r < 4; ++r) {
+            const int dim = 32 * d + 8 * r + 4 * hi;
+            const f32x4 v = f32x4{acc[d][4 * r], acc[d][4 * r + 1], acc[d][4 * r + 2], acc[d][4 * r + 3]} * inv * up;
+            if (dim >= a.c.vdim) continue;
+            if (parts) *reinterpret_cast<f32x4*>(a.many.po + (part * Z::PER + n) * a.c.vdim + dim) = v;
+            else kv8_store<Tr>(a, c.s.row0 + tok, head, dim, v);
         }
+    if (parts && hi == 0) {
+        a.many.pml[part * 2 * Z::PER + n] = ref.r;
+        a.many.pml[part * 2 * Z::PER + Z::PER + n] = L;
     }
 }
 // Calls that may bring sequences of either kind: both in one launch, they share nothing.  grid: the many's kv heads x group slots (a head's groups

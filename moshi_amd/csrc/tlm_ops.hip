@@ -194,7 +194,6 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     if ((rc = check_cache(cache, &a->c, "mmi_kv_attend")) || (rc = check_seqs(seqs, &a->q, "mmi_kv_attend"))) return rc;
     if (heads < 1 || heads % cache->kv_heads || heads / cache->kv_heads > 1024) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: query heads are a multiple of the key/value heads, at most 1024 times");
     if (window < 0 || keep_first < 0) return mmi_fail(MMI_ERR_INVALID, "mmi_kv_attend: negative window");
-    a->heads = heads;
     a->rep = heads / cache->kv_heads;
     a->nd = cache->vdim / 16;
     a->mask = TlmMask{window, window > 0 ? std::min(keep_first, TLM_KEEP) : 0, 0.f};
