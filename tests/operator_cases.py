@@ -1216,3 +1216,56 @@ def check_wide_integers(dev, lib):
         with pytest.raises(ValueError, match="end token"):
             beam_select(x, s, eos=eos, lib=lib)
     assert beam_select(x, s, eos=49, lib=lib).finished.shape == (1, 3) and beam_select(x, s, eos=-5, lib=lib).finished is None
+
+
+# ---- the search's choices, whatever the model's rounding -------------------------------------------------------------------------------
+def _search64(lm, prompts, beams, steps, eos, alpha, step_tokens):
+    """Beam search that ranks in 64 bits what the model says of sequences fed from their start, in slots of their own for every step: same batches, no reordering."""
+    from moshi_amd.beam import _prefill
+    R = len(prompts)
+    scores = torch.full((R, beams), -math.inf)
+    scores[:, 0] = 0.0
+    lengths, finished = torch.zeros((R, beams), dtype=torch.int32), torch.zeros((R, beams), dtype=torch.bool)
+    paths, live, was_live = [[[] for _ in range(beams)] for _ in range(R)], list(range(R)), []
+    for n in range(steps):
+        slots = [[lm.open() for _ in range(beams)] for _ in range(R)]
+        for i in range(beams):                             # (a beam at a time: the same portions as where one sequence stands for all)
+            first = _prefill(lm, prompts, [s[i] for s in slots], step_tokens).cpu()
+        logits = first.repeat_interleave(beams, dim=0).view(R, beams, -1)
+        for k, who in enumerate(was_live):
+            y = lm.step([(slots[r][i], [paths[r][i][k]], [0]) for r in who for i in range(beams)]).cpu().view(len(who), beams, -1)
+            for at, r in enumerate(who):
+                logits[r] = y[at]
+        for row in slots:
+            for s in row:
+                lm.close(s)
+        total, parents, tokens, fin, lens = select64(logits[live].flatten(0, 1), scores[live], lengths[live], finished[live], eos, alpha)
+        for at, r in enumerate(live):
+            paths[r] = [paths[r][int(p)] + [int(t)] for p, t in zip(parents[at], tokens[at])]
+            scores[r], lengths[r], finished[r] = torch.from_numpy(total[at]).float(), torch.from_numpy(lens[at]), torch.from_numpy(fin[at])
+        live = [r for r in live if not finished[r].all()]
+        if not live:
+            break
+        was_live.append(list(live))
+    return [[(paths[r][i][:int(lengths[r, i])], float(scores[r, i])) for i in range(beams) if scores[r, i] > -math.inf] for r in range(R)]
+
+
+def check_beam_search_choices(dev, lib, name, dtype=F32, codes=None, beams=4, steps=7, alpha=0.0):
+    """Every hypothesis, token by token, is the one that the model's own logits lead to."""
+    cfg = tc.MECHANISMS[name]
+    sd = random_token_lm_state_dict(cfg, seed=5)
+    prompts = [tc.tokens_of(cfg, n, seed=n) for n in (5, 61, 16)]
+    lm = TokenLM(sd, cfg, device=dev, dtype=dtype, lib=lib, kv_cache=codes, max_slots=3 * beams, max_tokens=64 * 3 * 3 * beams)
+    probe = beam_search(lm, prompts, beams, steps, -1, alpha, step_tokens=14)
+    assert all(len(set(tuple(h.tokens) for h in hyps)) == beams for hyps in probe)
+    for eos in (-1, probe[0][0].tokens[1], probe[1][-1].tokens[2]):      # none; tokens that beams end with early, all of a request's perhaps
+        got = beam_search(lm, prompts, beams, steps, eos, alpha, step_tokens=14)
+        want = _search64(lm, prompts, beams, steps, eos, alpha, 14)
+        assert [[h.tokens for h in hyps] for hyps in got] == [[t for t, _ in hyps] for hyps in want], eos
+        # a score: a rounding and the error of a sum's logarithm for every token
+        for a, b in zip([h.score for hyps in got for h in hyps], [s for hyps in want for _, s in hyps]):
+            assert abs(a - b) <= steps * (abs(b) * 2.0 ** -24 + 2.0 ** -22)
+    for bad in (16.5, -17.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match="penalty"):
+            beam_search(lm, prompts, beams, steps, -1, bad)
+    assert lm.free_pages == lm.total_pages and lm.free_slots == lm.max_slots

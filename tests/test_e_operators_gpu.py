@@ -247,3 +247,9 @@ def test_output_rows(lib):
 
 def test_wide_integers(lib):
     oc.check_wide_integers(DEV, lib)
+
+
+@pytest.mark.parametrize("name, codes, alpha", [("mixed", None, 0.0), ("bibapel", None, 0.7), ("grouped_attention", "int8", 1.0), ("bibapel", "e4m3", 0.0), ("two_kept_windows", "int8", -0.5)])
+@pytest.mark.parametrize("dtype", [oc.F32, oc.BF16], ids=["fp32", "bf16"])
+def test_beam_search_choices(lib, name, codes, alpha, dtype):
+    oc.check_beam_search_choices(DEV, lib, name, dtype, codes, alpha=alpha)

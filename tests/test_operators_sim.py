@@ -171,3 +171,9 @@ def test_output_rows(tlm_lib):  # noqa: F811
 
 def test_wide_integers(tlm_lib):  # noqa: F811
     oc.check_wide_integers(DEV, tlm_lib)
+
+
+@pytest.mark.parametrize("name, codes, alpha, dtype", [("mixed", None, 0.0, oc.F32), ("bibapel", None, 0.7, oc.BF16), ("grouped_attention", "int8", 1.0, oc.F32),
+                                                       ("two_kept_windows", "e4m3", 0.0, oc.BF16)])
+def test_beam_search_choices(tlm_lib, name, codes, alpha, dtype):  # noqa: F811
+    oc.check_beam_search_choices(DEV, tlm_lib, name, dtype, codes, beams=3, steps=4, alpha=alpha)
