@@ -768,7 +768,8 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
         load(i + WK);
         mmi_sched_barrier();
         if (!now) continue;
-        // (scalars: an element of a vector written behind a branch has come out as its neighbour where the vector was kept in accumulation registers)
+        // (Scalars, changed in selects: where elements of s were changed one at a time behind `if (!whole)` while it lived in accumulation registers, the
+        // compiler wrote its first element over the others on that path.  What is changed behind branches here, acc, is changed whole.)
         float y[16], mx = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; ++r) y[r] = s[r >> 2][r & 3] * sc;
