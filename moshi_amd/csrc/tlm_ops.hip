@@ -198,7 +198,7 @@ int attn_args(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads,
     a->nd = cache->vdim / 16;
     a->mask = TlmMask{window, window > 0 ? std::min(keep_first, TLM_KEEP) : 0, 0.f};
     if ((long)a->q.T * a->rep > 1l << 26) return mmi_fail(MMI_ERR_SHAPE, "mmi_kv_attend: at most 2^26 rows times query heads of a group");
-    *floats = tlm_kv8_plan(*a, seqs->n ? seqs->table_ld : 1, (size_t)1 << 30);
+    *floats = tlm_kv8_plan(*a, seqs->n ? std::min(seqs->table_ld, 1 << 25) : 1, (size_t)1 << 30);      // (2^31 positions; twice a page's number has to stay in 31 bits)
     long groups = 0;
     for (const Kv8Share* h : {&a->few, &a->many})
         if (h->nsplit) groups += kv8_slots(a->q, h->z) * (long)cache->kv_heads * h->nsplit;

@@ -1269,3 +1269,15 @@ def check_beam_search_choices(dev, lib, name, dtype=F32, codes=None, beams=4, st
         with pytest.raises(ValueError, match="penalty"):
             beam_search(lm, prompts, beams, steps, -1, bad)
     assert lm.free_pages == lm.total_pages and lm.free_slots == lm.max_slots
+
+
+def check_long_tables(dev, lib):
+    """Page tables with more entries than there are positions: no more splits, whose first pages would leave 31 bits."""
+    import ctypes as C
+    from moshi_amd import _capi
+    cache, _, _, i32, _ = _filled(dev, lib, 2, 70)
+    here = i32(0, 1)
+    for row0 in (None, here.data_ptr()):
+        need = [lib.mmi_kv_attend_workspace(C.byref(cache._desc), C.byref(_capi.KVSeqs(1, 1, row0, here.data_ptr(), here.data_ptr(), ld)), 2, 0, 0)
+                for ld in (1 << 25, (1 << 25) + 1, 1 << 30, (1 << 31) - 1)]
+        assert need[0] > 0 and need == [need[0]] * 4, need

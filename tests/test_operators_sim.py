@@ -177,3 +177,7 @@ def test_wide_integers(tlm_lib):  # noqa: F811
                                                        ("two_kept_windows", "e4m3", 0.0, oc.BF16)])
 def test_beam_search_choices(tlm_lib, name, codes, alpha, dtype):  # noqa: F811
     oc.check_beam_search_choices(DEV, tlm_lib, name, dtype, codes, beams=3, steps=4, alpha=alpha)
+
+
+def test_long_tables(tlm_lib):  # noqa: F811
+    oc.check_long_tables(DEV, tlm_lib)
