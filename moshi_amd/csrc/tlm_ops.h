@@ -2,7 +2,7 @@
 #pragma once
 #include "tlm_kv8.h"
 
-// dtype of keys, values and queries: MMI_BF16 or MMI_F32 (a.k / a.v / a.x); exact: fp32 arithmetic for fp32 queries
+// dtype of keys, values and queries: MMI_BF16 or MMI_F32 (a.k / a.v / a.x); f32: fp32 results, from operands of two parts (fp32 queries; otherwise bf16 from one)
 int tlm_kv8_append(hipStream_t s, TlmKv8Append a, int dtype);
 // fills in how the work is split (`cap`: pages that a sequence can have at most; `room`: floats that a workspace may have) and says what workspace
 // that takes, in floats

@@ -6,8 +6,13 @@
 
 namespace {
 
-constexpr long KV8_WORKGROUPS = 512;     // that a split of the pages aims at: 2 per CU, all at once (512, 1024, 2048: 48, 59, 69 us for one sequence of 100 003 keys, 78, 86, 99 us for 64)
-constexpr long KV8_TILES = 384;           // the same of k_tlm_kv8_tile, which works faster alone on a CU and writes its parts for longer (128, 256, 384, 512: 60, 46, 45, 49 us for 16 sequences with 560 tokens)
+// Workgroups that a split of the pages aims at.  Few columns: one per CU (128, 256, 512, 1024 of them: 100 003 keys of 8 heads of 128 62, 44, 47, 59 us, of 4 heads of 256 72, 55, 73,
+// 91, 64 sequences of 800 to 4096 keys 77, 77, 77, 86, eight of 8000 27, 21, 23, 30, 24 of 1500 20, 24, 25, 28); more are more parts to join.
+constexpr long KV8_WORKGROUPS = 256;
+// The same of k_tlm_kv8_tile (256, 384, 512: 16 sequences with 560 tokens 43, 41, 45 us, 24 with 540 tokens of 64 dimensions 53, 44, 43, a prompt of 1200 on one kv head 35, 34, 37, one
+// of 100 behind 900 keys 30, 30, 36, 1260 tokens behind 2000 80, 73, 64), and where heads above 128 leave a CU one workgroup (192, 256, 384, 512: 720 tokens of 256 dimensions
+// behind 1500 keys 65, 59, 91, 88).
+constexpr long KV8_TILES = 384, KV8_TILES_WIDE = 256;
 constexpr int KV8_MAX_SPLIT = 256;       // (k_tlm_kv8_combine: a lane each)
 
 int check_cache(const mmi_kv_cache* c, TlmKv8Cache* out, const char* at) {
@@ -136,7 +141,7 @@ size_t tlm_kv8_plan(TlmKv8Attn& a, long cap, size_t room) {
     if ((long)a.q.T * a.rep / (KV8_FEW + 1) < a.q.n) a.many.z = Kv8Cut{a.rep, KV8_MANY, 0, KV8_FEW + 1};
     a.many.cols = KV8_MANY;
     const long full = (long)a.q.T * a.rep / KV8_MANY + 1;
-    return few + split_pages(a, a.many, full + (kv8_slots(a.q, a.many.z) - full) / 4, cap, room - few, KV8_TILES, 1);
+    return few + split_pages(a, a.many, full + (kv8_slots(a.q, a.many.z) - full) / 4, cap, room - few, attn_bound(a.c) > 128 ? KV8_TILES_WIDE : KV8_TILES, 1);
 }
 void tlm_kv8_workspace(TlmKv8Attn& a, float* w) {
     for (Kv8Share* h : {&a.few, &a.many}) {
