@@ -45,8 +45,9 @@ __device__ __forceinline__ f32x4 beam_load4(const uint16_t* p) {
 __device__ __forceinline__ float beam_load(const float* p) { return *p; }
 __device__ __forceinline__ float beam_load(const uint16_t* p) { return mmi_bf16_to_f32(*p); }
 
-// e^(d + low), d <= 0, as 2^(d log2 e) with the product's low part carried along: a sum's relative error stays near 2^-28, where its logarithm is
-// added to scores whose order it decides
+// e^(d + low), d <= 0, as 2^(d log2 e) with the product's low part carried along: a term's error is that of two exponentials good to one unit and of
+// their product's rounding, 2^-21.7 at most, however large d.  A row's sum, whose logarithm is added to scores that it puts in order, has been off by
+// up to 2^-22.3 (40 960 rows of 2 to 65521 logits).
 __device__ __forceinline__ float beam_exp(float d, float low) {
     constexpr float L = 1.44269504f, LL = 1.92596299e-8f;
     d = d < -200.f ? -200.f : d;                           // (zero either way; a mask's -3e38 would leave infinities)
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(256) void k_tlm_beam_rows(TlmBeamArgs a) {
 // A workgroup per request: 4096 of its candidates at a time in registers, 16 a lane, beside the best found so far.  As in the rows, a bound that
 // `beams` lanes of one wave reach leaves few to be ranked by counting; ranks rounded to 32 bits keep their order, which is all a bound needs.  A
 // candidate's place is beam * V + token.  Latency from end to end, chunks' sums, their logarithms,
-// candidates, bound, ranks: 6.8 us for 4 beams of 32000, 12.7 us for 16 requests with 8 beams of 65521.  (Candidates taken one at a time, a maximum over the
+// candidates, bound, ranks: 6.6 us for 4 beams of 32000, 11.4 us for 16 requests with 8 beams of 65521.  (Candidates taken one at a time, a maximum over the
 // workgroup for each: 25 us there.)
 __global__ __launch_bounds__(256) void k_tlm_beam_pick(TlmBeamArgs a) {
     constexpr int N = 16;
@@ -424,8 +425,8 @@ struct TlmReorder {
 };
 // A lane owns a unit of the request's rows: it has read all of it before it writes any, so rows may change places.  Rows that stay are not written,
 // and in their place a row that some other one needs is asked for again: a load behind a branch would wait for the one before it (315 us
-// instead of 188 for 64 rows of 13 MB, with random parents 1.2 GB: 6.6 TB/s, above a large copy's 4.9, since a row that two children
-// take is read once).  Four rows of 3.4 MB: 5.5 us, a launch and one round trip.  Instances by the beams, since their registers are a lane's.
+// instead of 188 for 64 rows of 13 MB, of which random parents have 30 read and 43 written: 0.98 GB at 5.3 TB/s, a copy of 1 GiB 5.2; a row that
+// two children take is read once).  Four rows of 3.4 MB: 5.5 us, a launch and one round trip.  Instances by the beams, since their registers are a lane's.
 template <class U, int K>
 __device__ __forceinline__ void beam_move(const TlmReorder::T& t, const int (&from)[K], const int (&to)[K], unsigned moved, unsigned u) {
     U v[K];

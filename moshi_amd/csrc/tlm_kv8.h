@@ -681,7 +681,7 @@ __device__ __forceinline__ float kv8_inverse(float L, float r, int sink) {
 
 // Few columns: four waves share one tile of 16 columns, each takes every fourth of its pages straight from the cache - the page after it is
 // asked for before the products of this one - and their sums meet in LDS.  Bound by the codes' way from memory: 100 003 keys of 8 heads of 128
-// 41.5 us at 4.9 TB/s, as fast as a large copy; 64 sequences of 800 to 4096 keys 77 us at 4.2 TB/s, the longest ones' end is not full.
+// 38.8 us at 5.3 TB/s, as fast as a large copy; 64 sequences of 800 to 4096 keys 76 us at 4.2 TB/s, the longest ones' end is not full.
 // LDS: the queries and their angles, then (the same memory) the waves' sums
 constexpr int KV8_LDS = 4 * 8 * 64;                        // vectors of four floats: 8 waves' worth of 8 x 16 dimensions; queries of 256 in two parts and angles take 2048 too
 template <class In, class Tr, int NS, int D, bool E4M3>
@@ -1119,8 +1119,8 @@ __global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(Tlm
     }
 }
 
-// The splits of one column -> output.  A chain of two round trips behind a launch: 3.9 us for 5 sequences (the wide one: 5.0), 5.6 us for 56 splits of
-// one (the other: 8.6), 7.8 us for 16 sequences with 560 tokens (the wide one: 46).
+// The splits of one column -> output.  A chain of two round trips behind a launch: 3.9 us for 5 sequences (the wide one: 5.0), 5.3 us for 31 splits of
+// one and 5.6 for 56 (the other: 8.6), 7.9 us for 16 sequences with 560 tokens (the wide one: 46).
 //  grid: columns of all slots (first the few's, then the many's), kv heads.
 // Up to 16 splits (WIDE false): a wave for every 64 / (vdim / 4) columns, four dimensions a lane, eight partial sums asked for at once.  More: a
 // workgroup per column, 16 groups of lanes take every 16th split, and their sums meet in LDS.
