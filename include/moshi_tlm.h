@@ -128,7 +128,8 @@ typedef struct mmi_kv_cache {
 } mmi_kv_cache;
 /* The sequences of a call, all of it in device memory: sequence e brings rows row0[e] .. row0[e + 1] - 1 of the tensors, its positions
  * position[e] .., and finds position p in page table[e][p / 64].  row0 NULL: one row each, in order.  A page number outside the cache
- * holds nothing: rows that belong there are not written, and nobody sees its tokens.  A sequence with a negative position is passed over. */
+ * holds nothing: rows that belong there are not written, and nobody sees its tokens.  A sequence with a negative position is passed over.  Calls without a
+ * sequence (n 0) do nothing. */
 typedef struct mmi_kv_seqs {
     int32_t n, rows;                              /* sequences, rows of the tensors */
     const int32_t* row0;

@@ -74,6 +74,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, lengths: Optional[to
         raise ValueError("a length penalty needs lengths")
     if eos >= vocab > 0:
         raise ValueError("the end token is outside the vocabulary")
+    eos = max(eos, -1)
     need = _need.get((batch, beams, vocab))
     if need is None:
         need = lib.mmi_beam_select_workspace(batch, beams, vocab)

@@ -136,7 +136,9 @@ class PagedKVCache:
         in the queries' type.  scale: default dim ** -0.5.  window > 0: the last `window` positions and the first `keep_first`.  sink: one is
         added to the softmax's denominator.  Rows that see nothing are zeros.  Rows that no sequence brings - behind the last one, or of one that
         is passed over - are zeros too in a new tensor, and left as they were in `out`, whose rows and heads lie apart."""
-        if window > _LONGEST or keep_first > _LONGEST:
+        if not (0 <= window <= _LONGEST and 0 <= keep_first <= _LONGEST):
+            if window < 0 or keep_first < 0:
+                raise ValueError("a window, and the first positions kept beside it, are not negative")
             window, keep_first = min(window, _LONGEST), min(keep_first, _LONGEST)
         heads, dtype, qp = self._rows(q, "q", None, self.dim)
         total = q.shape[0]

@@ -1281,3 +1281,17 @@ def check_long_tables(dev, lib):
         need = [lib.mmi_kv_attend_workspace(C.byref(cache._desc), C.byref(_capi.KVSeqs(1, 1, row0, here.data_ptr(), here.data_ptr(), ld)), 2, 0, 0)
                 for ld in (1 << 25, (1 << 25) + 1, 1 << 30, (1 << 31) - 1)]
         assert need[0] > 0 and need == [need[0]] * 4, need
+
+
+def check_wide_negative_integers(dev, lib):
+    """Below 32 bits too: a negative window is none, and no token ends a beam."""
+    cache, table, _, i32, g = _filled(dev, lib, 2, 70)
+    q = torch.randn((1, 2, 32), generator=g).to(dev)
+    for kw in (dict(window=-2 ** 32), dict(window=-2 ** 32 + 3), dict(window=3, keep_first=-2 ** 32), dict(keep_first=-2 ** 63)):
+        with pytest.raises(ValueError):
+            cache.attend(q, table, i32(69), **kw)
+    x, s = torch.zeros((3, 50), device=dev), torch.zeros((1, 3), device=dev)
+    n, f = torch.ones((1, 3), dtype=torch.int32, device=dev), torch.ones((1, 3), dtype=torch.bool, device=dev)
+    with pytest.raises(ValueError):                        # (finished beams need an end token)
+        beam_select(x, s, n, f, eos=-2 ** 32 + 5, lib=lib)
+    assert beam_select(x, s, n, eos=-2 ** 32 + 5, lib=lib).finished is None

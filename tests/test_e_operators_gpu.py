@@ -253,3 +253,7 @@ def test_wide_integers(lib):
 @pytest.mark.parametrize("dtype", [oc.F32, oc.BF16], ids=["fp32", "bf16"])
 def test_beam_search_choices(lib, name, codes, alpha, dtype):
     oc.check_beam_search_choices(DEV, lib, name, dtype, codes, alpha=alpha)
+
+
+def test_wide_negative_integers(lib):
+    oc.check_wide_negative_integers(DEV, lib)

@@ -181,3 +181,7 @@ def test_beam_search_choices(tlm_lib, name, codes, alpha, dtype):  # noqa: F811
 
 def test_long_tables(tlm_lib):  # noqa: F811
     oc.check_long_tables(DEV, tlm_lib)
+
+
+def test_wide_negative_integers(tlm_lib):  # noqa: F811
+    oc.check_wide_negative_integers(DEV, tlm_lib)
