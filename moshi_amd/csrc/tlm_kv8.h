@@ -881,6 +881,11 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
     typedef Kv8Code<E4M3> C;
     typedef Kv8Tile<NS, D> Z;
     constexpr int KS = Z::KS, DT = Z::DT, KU = D > 128 ? 2 : 1;      // units of 16 codes per thread and side
+    // Two-part operands of 256 dimensions fill the registers: fewer fragments on their way, and the last k-steps' queries stay in LDS, where the angles were (with
+    // all of them in registers 28 spilled)
+    constexpr bool TIGHT = D * NS > 256;
+    constexpr int FR = TIGHT ? 4 : 8, KR = TIGHT ? KS - 2 : KS;      // KR: k-steps whose queries are in registers
+    static_assert((KS - KR) * NS * 64 * 4 * sizeof(u32x4) <= KV8_ANGLES * 8, "queries in the angles' place");
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = mmi_uniform(tid >> 6), cl = lane & 31, hi = lane >> 5;
     const Kv8Cols c(a, a.many, false, slot);
     kv8_tell(a.many, c, slot, g, split);
@@ -933,7 +938,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
         z0 = find(i0);
         load_k(z0);
     }
-    u32x4 q[KS][NS];                                       // dimensions 16 s + 8 hi ..
+    u32x4 q[KR][NS], *ql = lds + Z::PER * D * NS / 8 + Z::PER / 4 + wave * (KS - KR) * NS * 64 + lane;      // dimensions 16 s + 8 hi ..
     float back;
     {
         float* turned = reinterpret_cast<float*>(lds + Z::PER * D * NS / 8);      // inverse factors, then angles
@@ -943,7 +948,7 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 #pragma unroll
         for (int j = 0; j < KS; ++j)
 #pragma unroll
-            for (int p = 0; p < NS; ++p) q[j][p] = lds[((wave * KS + j) * NS + p) * 64 + lane];
+            for (int p = 0; p < NS; ++p) (j < KR ? q[j < KR ? j : 0][p] : ql[((j - KR) * NS + p) * 64]) = lds[((wave * KS + j) * NS + p) * 64 + lane];
         back = turned[wave * 32 + cl] * a.mask.scale;
         __syncthreads();                                   // (their memory takes keys and values)
     }
@@ -986,24 +991,22 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     f32x16 s[2];
-    u32x4 fr[8];                                           // operand fragments, asked for eight at a time
-    auto ask_k = [&](int buf, int j0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j0 + j < KS) fr[j] = kb[buf * Z::KF + (j0 + j) * 64 + (lane ^ j)];
-    };
+    u32x4 fr[FR];                                          // operand fragments, asked for so many at a time
     auto scores = [&](int set, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[set][r] = 0.f;
 #pragma unroll
-        for (int j0 = 0; j0 < KS; j0 += 8) {
-            ask_k(buf, j0);
+        for (int j0 = 0; j0 < KS; j0 += FR) {
+#pragma unroll
+            for (int j = 0; j < FR; ++j)
+                if (j0 + j < KS) fr[j] = kb[buf * Z::KF + (j0 + j) * 64 + (lane ^ ((j0 + j) & 7))];
             mmi_sched_barrier();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < FR; ++j)
                 if (j0 + j < KS)
 #pragma unroll
-                    for (int n = NS - 1; n >= 0; --n) s[set] = mmi_mfma_f16_32x32x16(fr[j], q[j0 + j][n], s[set]);
+                    for (int n = NS - 1; n >= 0; --n)
+                        s[set] = mmi_mfma_f16_32x32x16(fr[j], j0 + j < KR ? q[j0 + j < KR ? j0 + j : 0][n] : ql[((j0 + j - KR) * NS + n) * 64], s[set]);
         }
     };
     const int vl = lane ^ (4 * hi);
@@ -1041,13 +1044,13 @@ __device__ __forceinline__ void tlm_kv8_tile(const TlmKv8Attn& a, u32x4* lds, in
 #pragma unroll
             for (int u = 0; u < 2; ++u) kv8_split8<NS>(y + 8 * u, times, pf[u]);
 #pragma unroll
-            for (int d0 = 0; d0 < DT; d0 += 4) {
+            for (int d0 = 0; d0 < DT; d0 += FR / 2) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < FR; ++k)
                     if (d0 + k / 2 < DT) fr[k] = vb[set * Z::VF + (2 * d0 + k) * 64 + vl];
                 mmi_sched_barrier();
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < FR; ++k)
                     if (d0 + k / 2 < DT)
 #pragma unroll
                         for (int n = NS - 1; n >= 0; --n) acc[d0 + k / 2] = mmi_mfma_f16_32x32x16(fr[k], pf[k & 1][n], acc[d0 + k / 2]);

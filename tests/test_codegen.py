@@ -55,6 +55,52 @@ def copies_of_one(lines):
     return found
 
 
+SPILL = re.compile(r"scratch_store_dword(?:x\d)? off, v(?:\[(\d+):(\d+)\]|(\d+)), off(?: offset:(\d+))?$")
+RELOAD = re.compile(r"scratch_load_dword(?:x\d)? ([av])(?:\[(\d+):(\d+)\]|(\d+)), off, off(?: offset:(\d+))?$")
+
+
+def lost_elements(lines):
+    """Reloads of a part of a vector whose next element waits in an accumulation register and is not fetched beside them."""
+    functions, code = [], None
+    for line in lines:
+        t = line.split("//")[0].split(";")[0].strip()
+        m = re.match(r"[0-9a-f]+ <(\w+)>:", t) or re.match(r"(_Z\w+):", t)
+        if m:
+            code = []
+            functions.append((m.group(1), code))
+        elif t and code is not None:
+            code.append(t)
+    found = []
+    for name, code in functions:
+        waiting = {}                                       # (place, elements): the accumulation registers that hold the element behind them
+        for k, t in enumerate(code):
+            m = SPILL.match(t)
+            if m:
+                lo, hi = (int(m.group(1)), int(m.group(2))) if m.group(1) else (int(m.group(3)),) * 2
+                for near in code[max(0, k - 4):k + 5]:
+                    w = WRITE.match(near)
+                    if w and w.group(2) == f"v{hi + 1}":
+                        waiting.setdefault((m.group(4), hi - lo), set()).add(w.group(1))
+        for k, t in enumerate(code):
+            m = RELOAD.match(t)
+            if not m:
+                continue
+            lo, hi = (int(m.group(2)), int(m.group(3))) if m.group(2) else (int(m.group(4)),) * 2
+            held = waiting.get((m.group(5), hi - lo))
+            fetch = held and re.compile(rf"v_accvgpr_(?:read|mov)_b32 {m.group(1)}{hi + 1}, a(?:{'|'.join(held)})$")
+            if held and not any(fetch.match(near) for near in code[max(0, k - 6):k + 7]):
+                found.append((name, t))
+    return found
+
+
+def test_the_lost_element_is_seen():
+    spill = ["_Zk:", "v_accvgpr_write_b32 a255, v7", "scratch_store_dwordx3 off, v[4:6], off", "scratch_store_dwordx4 off, v[4:7], off offset:16"]
+    bad = ["scratch_load_dwordx4 a[16:19], off, off offset:16", "scratch_load_dwordx3 a[170:172], off, off", "v_mfma_f32_32x32x16_f16 a[16:31], v[0:3], a[170:173], a[16:31]"]
+    assert lost_elements(spill + bad) == [("_Zk", bad[1])]
+    assert not lost_elements(spill + ["v_accvgpr_read_b32 v57, a255", "scratch_load_dwordx3 v[54:56], off, off"])
+    assert not lost_elements(spill + ["v_accvgpr_mov_b32 a173, a255"] + bad) and not lost_elements(["_Zk:", spill[3]] + bad[:1])
+
+
 def test_the_fault_is_seen():
     bad = ["_Zk:", "v_accvgpr_read_b32 v102, a64", "v_cndmask_b32_e32 v103, v4, v103, vcc", "v_accvgpr_write_b32 a65, v102", "v_accvgpr_write_b32 a66, v102",
            "v_accvgpr_write_b32 a67, v102", "s_branch 12"]
@@ -79,7 +125,7 @@ def test_no_vector_is_copied_back_as_its_first_element(which, tmp_path):
             lines = dump.stdout.readlines()
         assert dump.returncode == 0
         seen += sum("v_accvgpr_write" in x for x in lines)
-        assert not copies_of_one(lines)
+        assert not copies_of_one(lines) and not lost_elements(lines)
     assert seen
 
 
