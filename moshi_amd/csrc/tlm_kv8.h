@@ -48,12 +48,19 @@ __device__ __forceinline__ TlmKv8Seq kv8_seq(const TlmKv8Seqs& a, int e) {
     s.pos0 = mmi_uniform(pos0);
     return s;
 }
-// Rows that no sequence brings: those before the first sequence, and those from the sequence's end to the next one's start (all of its own, if it is
-// passed over) or to the tensors'
+// Rows that no sequence brings.  From a sequence's end to the next one's start: all of its own, if it is passed over
 template <class F>
-__device__ __forceinline__ void kv8_rest(const TlmKv8Seqs& a, const TlmKv8Seq& s, F f) {
-    const int before = s.e == 0 ? s.row0 : 0, from = s.row0 + s.len, behind = max((s.e == a.n - 1 ? a.T : mmi_uniform(kv8_row0(a, s.e + 1))) - from, 0);
-    for (int i = 0; i < before + behind; ++i) f(i < before ? i : from + i - before);
+__device__ __forceinline__ void kv8_rest_of(const TlmKv8Seqs& a, const TlmKv8Seq& s, F f) {
+    const int end = mmi_uniform(kv8_row0(a, s.e + 1));
+    for (int i = s.row0 + s.len; i < end; ++i) f(i);
+}
+// Before the first sequence and behind the last one, which may be most rows of a padded call: shared by all workgroups, `n` (of 8000 rows
+// of 32 heads of 128, 100 brought: 68 us, 49 of it the attention itself; by one workgroup for each kv head 994)
+template <class F>
+__device__ __forceinline__ void kv8_rest_around(const TlmKv8Seqs& a, int first, int n, F f) {
+    if (!a.row0) return;
+    const int head = mmi_uniform(kv8_row0(a, 0)), tail = mmi_uniform(kv8_row0(a, a.n));
+    for (int i = first; i < head + a.T - tail; i += n) f(i < head ? i : tail + i - head);
 }
 // page number of the sequence's tokens 64 i .. 64 i + 63; -1: there is none
 __device__ __forceinline__ int kv8_page(const TlmKv8Seqs& a, int n_pages, const int* row, int i) {
@@ -396,12 +403,12 @@ __global__ __launch_bounds__(64) void k_tlm_kv8_read(TlmKv8Read a) {
     typedef Kv8Code<E4M3> C;
     const Kv8Span s = kv8_span(a.q, a.z, a.c.n_pages, (int)blockIdx.x);
     const int lane = mmi_lane(), g = (int)blockIdx.y;
-    if (s.first) {
+    auto clear = [&](int row) __attribute__((always_inline)) {
         const int n = blockIdx.z ? a.c.vdim : a.c.dim;
-        kv8_rest(a.q, s.s, [&](int row) __attribute__((always_inline)) {
-            if (4 * lane < n) kv8_put4((Out*)(blockIdx.z ? a.v : a.k) + ((long)row * a.c.kv_heads + g) * n + 4 * lane, f32x4{0.f, 0.f, 0.f, 0.f});
-        });
-    }
+        if (4 * lane < n) kv8_put4((Out*)(blockIdx.z ? a.v : a.k) + ((long)row * a.c.kv_heads + g) * n + 4 * lane, f32x4{0.f, 0.f, 0.f, 0.f});
+    };
+    kv8_rest_around(a.q, (int)blockIdx.x, (int)gridDim.x, clear);
+    if (s.first) kv8_rest_of(a.q, s.s, clear);
     if (s.none) return;
     const bool lost = s.page < 0;
     const long unit = (long)max(s.page, 0) * a.c.kv_heads + g;
@@ -479,7 +486,7 @@ struct TlmKv8Attn {
     int rep, nd;                         // query heads per key/value head; vdim / 16
     TlmMask mask;                        // scale: log2 e times the softmax's
     int sink;                            // one is added to the denominator
-    int rest;                            // rows that no sequence brings become zeros (few's, which has a slot for every sequence)
+    int rest;                            // rows that no sequence brings become zeros
     int both;                            // sequences of more than KV8_FEW columns are `many`'s; otherwise all are `few`'s
     Kv8Share few, many;
 };
@@ -673,6 +680,13 @@ __device__ __forceinline__ void kv8_store(const TlmKv8Attn& a, int row, int head
     typedef typename Tr::elem E;
     Tr::store4((E*)a.out + (a.out_ks ? tlm_index<Tr>(row, head * 16 * a.nd + d, a.out_ks) : row * a.out_row + head * a.out_head + d), v);
 }
+// zeros for a group's heads of a row
+template <class Tr>
+__device__ __forceinline__ void kv8_clear(const TlmKv8Attn& a, int row, int g) {
+    const int d = 4 * ((int)threadIdx.x & 63);
+    for (int head = (int)threadIdx.x >> 6; head < a.rep; head += 4)
+        if (d < a.c.vdim) kv8_store<Tr>(a, row, g * a.rep + head, d, f32x4{0.f, 0.f, 0.f, 0.f});
+}
 // 1 / denominator of weights that were summed relative to 2^r; nothing seen: zero
 __device__ __forceinline__ float kv8_inverse(float L, float r, int sink) {
     const float sum = sink ? L + exp2f(-r) : L;
@@ -691,11 +705,7 @@ __device__ __forceinline__ void tlm_kv8_attn(const TlmKv8Attn& a, f32x4* ob, flo
     const int lane = (int)threadIdx.x & 63, wave = mmi_uniform((int)threadIdx.x >> 6), bl = lane & 15, kq = lane >> 4;
     const Kv8Cols c(a, a.few, true, slot);
     kv8_tell(a.few, c, slot, g, split);
-    if (a.rest && split == 0 && c.c0 == 0 && (a.both || c.ncol == 0))
-        kv8_rest(a.q, c.s, [&](int row) __attribute__((always_inline)) {
-            for (int head = wave; head < a.rep; head += 4)
-                if (4 * lane < a.c.vdim) kv8_store<Tr>(a, row, g * a.rep + head, 4 * lane, f32x4{0.f, 0.f, 0.f, 0.f});
-        });
+    if (a.rest && split == 0 && c.c0 == 0 && c.s.len == 0) kv8_rest_of(a.q, c.s, [&](int row) __attribute__((always_inline)) { kv8_clear<Tr>(a, row, g); });
     const int i0 = split * a.few.pages, i1 = min(c.n, i0 + a.few.pages);
     if (c.c0 >= c.ncol || (i0 >= i1 && split > 0)) return;
     const int col = min(c.c0 + bl, c.ncol - 1), tok = col / a.rep, pos = c.s.pos0 + tok;
@@ -1112,6 +1122,9 @@ __global__ __launch_bounds__(256, D * NS <= 128 ? 2 : 1) void k_tlm_kv8_tile(Tlm
     MMI_SHARED float ml[3][4][16];
     const int G = a.c.kv_heads;
     int b = (int)blockIdx.x;
+    if (a.rest) kv8_rest_around(a.q, b, (int)gridDim.x, [&](int row) __attribute__((always_inline)) {
+        for (int g = 0; g < G; ++g) kv8_clear<Tr>(a, row, g);
+    });
     if (b < many) {
         const int slots = many / (G * a.many.nsplit), split = b / (G * slots);
         b -= split * G * slots;
