@@ -23,7 +23,7 @@ from . import _capi
 
 PAGE_TOKENS, BLOCK_TOKENS = 64, 16
 _LONGEST = 2 ** 31 - 1                   # no sequence has more positions
-_SINK, _ZERO_REST = _capi.MMI_KV_SINK, _capi.MMI_KV_ZERO_REST
+_SINK, _ZERO_REST, _SINK_ZERO_REST = _capi.MMI_KV_SINK, _capi.MMI_KV_ZERO_REST, _capi.MMI_KV_SINK | _capi.MMI_KV_ZERO_REST
 _CODES = {torch.int8: _capi.MMI_I8, torch.float8_e4m3fn: _capi.MMI_F8E4M3}
 _NAMES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 _DTYPES = {torch.bfloat16: _capi.MMI_BF16, torch.float32: _capi.MMI_F32}
@@ -136,21 +136,21 @@ class PagedKVCache:
         in the queries' type.  scale: default dim ** -0.5.  window > 0: the last `window` positions and the first `keep_first`.  sink: one is
         added to the softmax's denominator.  Rows that see nothing are zeros.  Rows that no sequence brings - behind the last one, or of one that
         is passed over - are zeros too in a new tensor, and left as they were in `out`, whose rows and heads lie apart."""
-        if not (0 <= window <= _LONGEST and 0 <= keep_first <= _LONGEST):
+        if window >> 31 or keep_first >> 31:                   # (below 0, or beyond 31 bits)
             if window < 0 or keep_first < 0:
                 raise ValueError("a window, and the first positions kept beside it, are not negative")
             window, keep_first = min(window, _LONGEST), min(keep_first, _LONGEST)
         heads, dtype, qp = self._rows(q, "q", None, self.dim)
         total = q.shape[0]
         seqs = self._seqs(table, positions, rows, total)
-        flags = _SINK if sink else 0
         if out is None:
-            flags |= _ZERO_REST
+            flags = _SINK_ZERO_REST if sink else _ZERO_REST
             out = torch.empty_like(q) if self.vdim == self.dim and q.is_contiguous() else q.new_empty((total, heads, self.vdim))
             op = (out.data_ptr(), heads * self.vdim, self.vdim)
-            if not seqs.n:
+            if not positions.shape[0]:
                 out.zero_()
         else:
+            flags = _SINK if sink else 0
             if out.shape != (total, heads, self.vdim) or out.dtype != q.dtype:
                 raise AssertionError("out is [rows, heads, vdim] in the queries' type")
             op = self._rows(out, "out", heads, self.vdim)[2]
