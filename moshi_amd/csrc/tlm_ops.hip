@@ -317,7 +317,16 @@ extern "C" int mmi_beam_select(int32_t batch, int32_t beams, int32_t vocab, int3
     return MMI_OK;
 }
 
+namespace {
+int reorder_unit(const TlmReorderTensor& t) {              // bytes that are moved at once
+    const uintptr_t all = (uintptr_t)t.p | (uintptr_t)t.stride | (uintptr_t)t.bytes;
+    return all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
+}
+}  // namespace
+
 int tlm_reorder(hipStream_t s, int n, const TlmReorderTensor* tensors, int groups, int beams, const int* parent, const int* row) {
+    for (int i = 0; i < n; ++i)                            // (before any of them has moved)
+        if (tensors[i].bytes / reorder_unit(tensors[i]) > 0x3fffffffl) return mmi_fail(MMI_ERR_SHAPE, "reorder: a row is too long");
     for (int i = 0; i < n;) {
         TlmReorder a;
         memset(&a, 0, sizeof(a));
@@ -327,10 +336,8 @@ int tlm_reorder(hipStream_t s, int n, const TlmReorderTensor* tensors, int group
         unsigned blocks = 0;
         for (; i < n && a.n < BEAM_TENSORS; ++i) {
             const TlmReorderTensor& t = tensors[i];
-            const uintptr_t all = (uintptr_t)t.p | (uintptr_t)t.stride | (uintptr_t)t.bytes;
-            const int unit = all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
+            const int unit = reorder_unit(t);
             const long units = t.bytes / unit;
-            if (units > 0x3fffffffl) return mmi_fail(MMI_ERR_SHAPE, "reorder: a row is too long");
             if (!units) continue;
             const unsigned more = (unsigned)mmi_cdiv64(units, 256);
             if (blocks + more > 0x7fffffu) break;          // (2^31 lanes a launch)

@@ -1295,3 +1295,18 @@ def check_wide_negative_integers(dev, lib):
     with pytest.raises(ValueError):                        # (finished beams need an end token)
         beam_select(x, s, n, f, eos=-2 ** 32 + 5, lib=lib)
     assert beam_select(x, s, n, eos=-2 ** 32 + 5, lib=lib).finished is None
+
+
+def check_reorder_of_too_long_rows(dev, lib):
+    """A row beyond what a launch takes is refused before the tensors in front of it have moved."""
+    import ctypes as C
+    from moshi_amd import _capi
+    place = _capi.LaunchOn(torch.device(dev, 0) if dev == "cuda" else torch.device(dev))
+    states = [torch.arange(8, dtype=torch.int32, device=dev).view(4, 2) + 100 * i for i in range(60)]
+    before, parents = [t.clone() for t in states], torch.tensor([[3, 2, 1, 0]], dtype=torch.int32, device=dev)
+    at = [t.data_ptr() for t in states] + [1 << 44]        # (never read: the lengths are refused)
+    ints = lambda x: (C.c_int64 * len(x))(*x)  # noqa: E731
+    for size in ((1 << 30) + 1, 16 << 30):
+        lists = [ints(x) for x in (at, [8] * 60 + [size], [8] * 60 + [size])]
+        assert place.call(lib.mmi_beam_reorder, 61, *lists, 1, 4, parents.data_ptr()) == _capi.MMI_ERR_SHAPE
+        assert all(torch.equal(a, b) for a, b in zip(states, before))

@@ -257,3 +257,7 @@ def test_beam_search_choices(lib, name, codes, alpha, dtype):
 
 def test_wide_negative_integers(lib):
     oc.check_wide_negative_integers(DEV, lib)
+
+
+def test_reorder_of_too_long_rows(lib):
+    oc.check_reorder_of_too_long_rows(DEV, lib)

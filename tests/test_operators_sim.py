@@ -185,3 +185,7 @@ def test_long_tables(tlm_lib):  # noqa: F811
 
 def test_wide_negative_integers(tlm_lib):  # noqa: F811
     oc.check_wide_negative_integers(DEV, tlm_lib)
+
+
+def test_reorder_of_too_long_rows(tlm_lib):  # noqa: F811
+    oc.check_reorder_of_too_long_rows(DEV, tlm_lib)
