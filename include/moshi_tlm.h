@@ -150,7 +150,8 @@ int mmi_kv_read(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtyp
  * MMI_KV_SINK: one is added to the softmax's denominator; MMI_KV_ZERO_REST: rows that no sequence brings (one that is passed over brings none)
  * become zeros, where they otherwise stay as they were.  Query head h reads key/value head h / (heads / kv_heads).  Sums are
  * fp32; bf16 queries and the weights beside them are fp16 operands, fp32 ones two fp16 parts each (22 bits).  A row that sees nothing gets zeros.
- * The output's heads lie apart, within rows or rows within heads, four elements aligned.  workspace: device memory of mmi_kv_attend_workspace bytes (a negative status in its place where the arguments are refused), one per call in flight. */
+ * The output's heads lie apart, within rows or rows within heads, four elements aligned.  workspace: device memory of mmi_kv_attend_workspace bytes
+ * (a negative status in its place where the arguments are refused), one per call in flight. */
 enum { MMI_KV_SINK = 1, MMI_KV_ZERO_REST = 2 };
 int64_t mmi_kv_attend_workspace(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t heads, int32_t window, int32_t keep_first);
 int mmi_kv_attend(const mmi_kv_cache* cache, const mmi_kv_seqs* seqs, int32_t dtype, int32_t heads, const void* q, int64_t q_row, int64_t q_head, void* out,
